@@ -271,6 +271,72 @@ int sugar_topk_stats(const float* d_scores, int64_t n_rows, int n_cols, int ntop
 int sugar_snorm_trials(const float* d_scores, const int32_t* d_enroll, const int32_t* d_test, int64_t n_trials,
                        const float* d_mean, const float* d_std, float std_eps, float* d_out, void* stream);
 
+/* ---- 8-bit operands with block scales -----------------------------------------------------------------------------
+ * No counterpart in the reference.  An operand of `rows` x `cols` is e4m3 values (OCP: largest 448, NaN, no infinities)
+ * d_q [rows][ldq] and exponent bytes d_e [rows][lde], one per row and block of 128 columns:
+ *     value[r][c] = e4m3(d_q[r][c]) * 2^(d_e[r][c / 128] - 127)          (byte 255: NaN)
+ * Columns cols .. round_up(cols, 128) of d_q are zero.  d_q 16-byte aligned, ldq a multiple of 16 and at least
+ * round_up(cols, 128); d_e 4-byte aligned, lde a multiple of 4 and at least round_up(ceil(cols / 128), 4).
+ * ldx / ldy / lda / ldw count elements.  rows == 0 is a call that does nothing.
+ *
+ * sugar_fp8_quant: per block the smallest exponent >= -127 that keeps the largest finite magnitude within 448, values to
+ *   nearest with ties to even; infinities and NaN become NaN and take no part in the exponent.  d_x [rows][ldx] dtype
+ *   (any alignment of its type).  Also writes the zero columns and the bytes (127) up to round_up(blocks, 4).
+ * sugar_fp8_dequant: d_y [rows][ldy] dtype <- the values (exact in either dtype within its normal range; a float32
+ *   magnitude that rounded up to 2^128 reads back as infinity).
+ * sugar_fp8_linear: d_y[r][o] = epilogue(sum_k a[r][k] w[o][k]), f32 accumulation.  SUGAR_F32 outputs: exact
+ *   products, float32 sums.  SUGAR_BF16 outputs: the 8-bit matrix instruction, which aligns 8 neighbouring products to the
+ *   largest and cuts them 2^-13 below its leading bit (1.5e-5 of the result on random operands; bf16 rounds by 1.7e-3).
+ *   flags bit0 ReLU, bit1 * d_scale[o] + d_shift[o] after it (float32 [n]); d_y [rows][ldy] dtype.  The left operand is
+ *   rows x k, the weights n x k; a call allocates nothing and needs no workspace. */
+int sugar_fp8_quant(const void* d_x, int64_t ldx, int dtype, int64_t rows, int cols, uint8_t* d_q, int64_t ldq,
+                    uint8_t* d_e, int64_t lde, void* stream);
+int sugar_fp8_dequant(const uint8_t* d_q, int64_t ldq, const uint8_t* d_e, int64_t lde, int64_t rows, int cols, void* d_y,
+                      int64_t ldy, int dtype, void* stream);
+int sugar_fp8_linear(const uint8_t* d_a, int64_t lda, const uint8_t* d_ae, int64_t ldae, int64_t rows, const uint8_t* d_w,
+                     int64_t ldw, const uint8_t* d_we, int64_t ldwe, int n, int k, const float* d_scale,
+                     const float* d_shift, int flags, void* d_y, int64_t ldy, int dtype, void* stream);
+
+/* ---- join of a block with its residual stream ----------------------------------------------------------------------
+ * Per row (frame), f32 between the loads and the stores:
+ *     v = post(u);   s = residual + alpha * gate * v;   stream = s, or residual + s when `dense`;   z = pre(s)
+ * Generalises the end of an SE-Res2 block, out = y * scale + S, S += out (sugar/models/dynamictdnn.py:98-100, 657-660:
+ * no norms, gate per utterance, dense), to norms over the channels behind the block (post) and in front of the next (pre):
+ *     SUGAR_NORM_AFFINE  x * w + b       (a folded BatchNorm)
+ *     SUGAR_NORM_RMS     x / sqrt(mean(x^2) + eps) * w + b
+ *     SUGAR_NORM_LAYER   (x - mean(x)) / sqrt(var(x) + eps) * w + b       (biased variance);   w, b float32 [cols] or NULL
+ * Outputs (each may be NULL, not all): d_stream [rows][lds], d_z [rows][ldz], d_q / d_e = z as an 8-bit operand
+ * (quantised from the unrounded z, laid out as sugar_fp8_quant writes it).  d_stream may be d_residual or d_u, d_z may be d_u (same type and stride); other overlaps
+ * are the caller's error.  With d_row_off (int32 [n_utts + 1], ascending) rows outside [row_off[0], row_off[n_utts]) are
+ * not touched. */
+#define SUGAR_NORM_NONE 0
+#define SUGAR_NORM_AFFINE 1
+#define SUGAR_NORM_RMS 2
+#define SUGAR_NORM_LAYER 3
+#define SUGAR_GATE_NONE 0
+#define SUGAR_GATE_CHANNEL 1    /* float32 [cols]                       */
+#define SUGAR_GATE_UTTERANCE 2  /* float32 [n_utts][ldg], needs row_off */
+#define SUGAR_GATE_ROW 3        /* u_dtype [rows][ldg]                  */
+#define SUGAR_JOIN_MAX_COLS 8192
+typedef struct {
+  int64_t rows;
+  int cols, n_utts;
+  int u_dtype, stream_dtype, z_dtype;   /* stream_dtype: residual and stream; SUGAR_F32 when u_dtype is          */
+  int post_kind, pre_kind, gate_kind, dense;
+  float alpha, post_eps, pre_eps;
+  int64_t ldu, ldr, ldg, lds, ldz, ldq, lde;
+  const void* d_u;
+  const void* d_residual;
+  const float *d_post_w, *d_post_b, *d_pre_w, *d_pre_b;
+  const void* d_gate;
+  const int32_t* d_row_off;
+  void* d_stream;
+  void* d_z;
+  uint8_t* d_q;
+  uint8_t* d_e;
+} SugarBlockJoin;
+int sugar_block_join(const SugarBlockJoin* h_join, void* stream);
+
 /* ------------------------------------------------------------------------------------------------------------
  * Live per-stage timing (bench.py's roofline figures).  No reference counterpart; the reference times whole
  * forwards with torch.cuda.synchronize (sugar/metrics.py:389-404).

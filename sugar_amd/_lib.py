@@ -38,6 +38,15 @@ class SugarSubnetDesc(C.Structure):
                 ("linear_w", _fp), ("linear_b", _fp), ("bnembed", SugarBN)]
 
 
+class SugarBlockJoin(C.Structure):
+    _fields_ = ([("rows", C.c_int64)] + [(n, C.c_int) for n in ("cols", "n_utts", "u_dtype", "stream_dtype", "z_dtype",
+                                                               "post_kind", "pre_kind", "gate_kind", "dense")]
+                + [(n, C.c_float) for n in ("alpha", "post_eps", "pre_eps")]
+                + [(n, C.c_int64) for n in ("ldu", "ldr", "ldg", "lds", "ldz", "ldq", "lde")]
+                + [(n, C.c_void_p) for n in ("d_u", "d_residual", "d_post_w", "d_post_b", "d_pre_w", "d_pre_b", "d_gate",
+                                             "d_row_off", "d_stream", "d_z", "d_q", "d_e")])
+
+
 # every symbol include/sugar_amd.h declares: (restype, argtypes)
 _vp, _i, _i64 = C.c_void_p, C.c_int, C.c_int64
 SYMBOLS = {
@@ -65,6 +74,10 @@ SYMBOLS = {
     "sugar_cohort_scores": (_i, [_vp, _i, _vp, _i, _vp, _i, _vp, _vp, _vp]),
     "sugar_topk_stats": (_i, [_vp, _i64, _i, _i, C.c_float, _vp, _vp, _vp]),
     "sugar_snorm_trials": (_i, [_vp, _vp, _vp, _i64, _vp, _vp, C.c_float, _vp, _vp]),
+    "sugar_fp8_quant": (_i, [_vp, _i64, _i, _i64, _i, _vp, _i64, _vp, _i64, _vp]),
+    "sugar_fp8_dequant": (_i, [_vp, _i64, _vp, _i64, _i64, _i, _vp, _i64, _i, _vp]),
+    "sugar_fp8_linear": (_i, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i, _i, _vp, _vp, _i, _vp, _i64, _i, _vp]),
+    "sugar_block_join": (_i, [C.POINTER(SugarBlockJoin), _vp]),
     "sugar_tdnn_recalibrate": (_i, [_vp, _vp, _vp, _i, _i64, _i, _vp, _i64, C.c_float, _vp, _vp]),
     "sugar_embed_recalibrate": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i64, _i, _vp, _i64, C.c_float, _vp, _vp]),
     "sugar_subnet_bn_count": (_i, [_vp]),

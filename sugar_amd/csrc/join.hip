@@ -1,0 +1,241 @@
+// The join of a block with its residual stream (gfx950): the norm behind the block, the gate, the residual sum, the norm
+// in front of the next block and, where that block multiplies in 8 bits, its operand -- one pass over the rows.
+//
+//   v = post(u);  s = residual + alpha * gate * v;  stream = s  (or residual + s);  z = pre(s)
+//
+// The SE-Res2 stack of DynamicTDNN.forward (sugar/models/dynamictdnn.py:98-100, 657-660) is the case without row norms:
+// gate = the squeeze-excite scale of the row's utterance, out = y * gate + S, S += out.
+// Everything between the loads and the stores is f32 in registers: a wave (or four, for wide or few rows) holds its row,
+// so a norm's mean and its sum of squares about that mean are two exact passes over registers, not over memory, and z
+// comes from the unrounded s.  Bound: HBM (u and residual in, stream and z out).
+#include "blockfp8.h"
+
+namespace sugar {
+
+namespace {
+
+enum { NORM_NONE = SUGAR_NORM_NONE, NORM_AFFINE = SUGAR_NORM_AFFINE, NORM_RMS = SUGAR_NORM_RMS, NORM_LAYER = SUGAR_NORM_LAYER };
+
+struct JoinArgs {
+  SugarBlockJoin j;
+  int vec_u, vec_r, vec_s, vec_z, vec_g;     // rows that can be read / written 16 bytes at a time
+};
+
+// Sum over the 64 lanes, the same in every lane, by DPP (rows of 16, then across rows).
+__device__ __forceinline__ float wave_total(float v) {
+  v += dpp_row_f32<0xB1>(v);
+  v += dpp_row_f32<0x4E>(v);
+  v += dpp_row_f32<0x141>(v);
+  v += dpp_row_f32<0x140>(v);
+  v += __shfl_xor(v, 16);
+  v += __shfl_xor(v, 32);
+  return v;
+}
+
+template <int WPR>
+__device__ __forceinline__ float row_total(float v, float* red, int wv) {
+  v = wave_total(v);
+  if constexpr (WPR > 1) {
+    __syncthreads();                         // the previous total has been read
+    if ((threadIdx.x & 63) == 0) red[wv] = v;
+    __syncthreads();
+    v = red[0];
+#pragma unroll
+    for (int i = 1; i < WPR; ++i) v += red[i];
+  }
+  return v;
+}
+
+// x <- norm(x) over the row's C channels; lanes past the row hold zeros before and whatever the weights say after.
+template <int NCH, int WPR>
+__device__ __forceinline__ void row_norm(float (&x)[NCH][8], int kind, const float* __restrict__ w, const float* __restrict__ b,
+                                         float eps, int C, int cw, float* red, int wv) {
+  if (kind == NORM_NONE) return;
+  const float inv_c = 1.0f / (float)C;
+  float mean = 0.f, mul = 1.f;
+  if (kind == NORM_LAYER) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < NCH; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t += x[k][i];
+    mean = row_total<WPR>(t, red, wv) * inv_c;
+  }
+  if (kind != NORM_AFFINE) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < NCH; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float d = cw + k * (512 * WPR) + i < C ? x[k][i] - mean : 0.f;
+        t = fmaf(d, d, t);
+      }
+    mul = 1.0f / sqrtf(fmaf(row_total<WPR>(t, red, wv), inv_c, eps));
+  }
+#pragma unroll
+  for (int k = 0; k < NCH; ++k) {
+    const int c = cw + k * (512 * WPR);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (c + i >= C) continue;
+      float t = (x[k][i] - mean) * mul;
+      if (w) t *= w[c + i];
+      if (b) t += b[c + i];
+      x[k][i] = t;
+    }
+  }
+}
+
+template <typename TU, typename TS, int NCH, int WPR>
+__global__ __launch_bounds__(256) void block_join_kernel(JoinArgs a) {
+  __shared__ float red[4];
+  const SugarBlockJoin& j = a.j;
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const int C = j.cols;
+  const int cw = (WPR > 1 ? wv * 512 : 0) + lane * 8;          // first channel of this lane's chunk 0
+  constexpr int RPB = 4 / WPR;                                 // rows a workgroup holds
+  const int64_t per = (j.rows + (int64_t)gridDim.x * RPB - 1) / ((int64_t)gridDim.x * RPB);
+  const int64_t first = ((int64_t)blockIdx.x * RPB + (WPR > 1 ? 0 : wv)) * per;
+  const int64_t last = first + per < j.rows ? first + per : j.rows;
+  int b = 0, b_end = 0;
+  if (j.d_row_off && first < last) {                           // last utterance that begins at or before the first row
+    int lo = 0, hi = j.n_utts;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (j.d_row_off[mid] <= first) lo = mid; else hi = mid;
+    }
+    b = lo;
+    b_end = j.d_row_off[b + 1];
+  }
+  for (int64_t r = first; r < last; ++r) {
+    if (j.d_row_off) {
+      while (r >= b_end && b + 1 < j.n_utts) { ++b; b_end = j.d_row_off[b + 1]; }
+      if (r >= b_end || r < j.d_row_off[0]) continue;           // a row of no utterance: left as it is
+    }
+    float v[NCH][8], s[NCH][8];
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) load8((const TU*)j.d_u + r * j.ldu, cw + k * (512 * WPR), C, a.vec_u, v[k]);
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) load8((const TS*)j.d_residual + r * j.ldr, cw + k * (512 * WPR), C, a.vec_r, s[k]);
+    row_norm<NCH, WPR>(v, j.post_kind, j.d_post_w, j.d_post_b, j.post_eps, C, cw, red, wv);
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+      const int c = cw + k * (512 * WPR);
+      float g[8];
+      if (j.gate_kind == SUGAR_GATE_ROW) load8((const TU*)j.d_gate + r * j.ldg, c, C, a.vec_g, g);
+      else if (j.gate_kind == SUGAR_GATE_UTTERANCE) load8((const float*)j.d_gate + b * j.ldg, c, C, a.vec_g, g);
+      else if (j.gate_kind == SUGAR_GATE_CHANNEL) load8((const float*)j.d_gate, c, C, a.vec_g, g);
+      else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] = 1.f;
+      }
+      float st[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float res = s[k][i];
+        s[k][i] = fmaf(j.alpha * g[i], v[k][i], res);
+        st[i] = j.dense ? res + s[k][i] : s[k][i];
+      }
+      if (j.d_stream) store8((TS*)j.d_stream + r * j.lds, c, C, a.vec_s, st);
+    }
+    if (!j.d_z && !j.d_q) continue;
+    row_norm<NCH, WPR>(s, j.pre_kind, j.d_pre_w, j.d_pre_b, j.pre_eps, C, cw, red, wv);
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+      const int c = cw + k * (512 * WPR);
+      if (j.d_z) {
+        if (j.z_dtype == SUGAR_F32) store8((float*)j.d_z + r * j.ldz, c, C, a.vec_z, s[k]);
+        else store8((bf16*)j.d_z + r * j.ldz, c, C, a.vec_z, s[k]);
+      }
+      if (j.d_q) {
+        unsigned big = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (c + i >= C) s[k][i] = 0.f;                        // padding columns of the operand
+          const unsigned u = fp8_finite_bits(s[k][i]);
+          big = u > big ? u : big;
+        }
+        const int byte = fp8_exponent(row16_max(big)), kb = c / FP8_BLOCK, blocks = (C + FP8_BLOCK - 1) / FP8_BLOCK;
+        if (kb < blocks) {
+          *(u32x2*)(j.d_q + r * j.ldq + c) = fp8_pack8(s[k], fp8_inverse(byte));
+          const int l16 = lane & 15;
+          if (l16 == 0) j.d_e[r * j.lde + kb] = (uint8_t)byte;
+          else if (kb == blocks - 1 && kb + l16 < ((blocks + 3) & ~3)) j.d_e[r * j.lde + kb + l16] = 127;   // padding bytes
+        }
+      }
+    }
+  }
+}
+
+template <typename TU, typename TS, int NCH, int WPR>
+int launch_join(const JoinArgs& a, hipStream_t s) {
+  int n_cu = 0;
+  if (int rc = device_cu_count(&n_cu)) return rc;
+  const int64_t want = ceil_div(a.j.rows, 4 / WPR);
+  const unsigned grid = (unsigned)(want < 8ll * n_cu ? want : 8ll * n_cu);
+  hipLaunchKernelGGL((block_join_kernel<TU, TS, NCH, WPR>), dim3(grid), dim3(256), 0, s, a);
+  SUGAR_LAUNCH_CHECK();
+  return SUGAR_OK;
+}
+
+template <typename TU, typename TS>
+int launch_join_t(const JoinArgs& a, hipStream_t s) {
+  const int C = a.j.cols;
+  if (C <= 512) return launch_join<TU, TS, 1, 1>(a, s);
+  if (C <= 2048) return launch_join<TU, TS, 1, 4>(a, s);
+  if (C <= 4096) return launch_join<TU, TS, 2, 4>(a, s);
+  return launch_join<TU, TS, 4, 4>(a, s);
+}
+
+bool norm_ok(int kind) { return kind == NORM_NONE || kind == NORM_AFFINE || kind == NORM_RMS || kind == NORM_LAYER; }
+
+}  // namespace
+
+int launch_block_join(const SugarBlockJoin& j, hipStream_t s) {
+  JoinArgs a;
+  a.j = j;
+  const int eu = j.u_dtype == SUGAR_F32 ? 4 : 2, es = j.stream_dtype == SUGAR_F32 ? 4 : 2, ez = j.z_dtype == SUGAR_F32 ? 4 : 2;
+  a.vec_u = rows_vec(j.d_u, j.ldu, j.cols, eu);
+  a.vec_r = rows_vec(j.d_residual, j.ldr, j.cols, es);
+  a.vec_s = rows_vec(j.d_stream, j.lds, j.cols, es);
+  a.vec_z = rows_vec(j.d_z, j.ldz, j.cols, ez);
+  a.vec_g = rows_vec(j.d_gate, j.gate_kind == SUGAR_GATE_CHANNEL ? j.cols : j.ldg, j.cols, j.gate_kind == SUGAR_GATE_ROW ? eu : 4);
+  if (j.u_dtype == SUGAR_F32) return launch_join_t<float, float>(a, s);
+  return j.stream_dtype == SUGAR_F32 ? launch_join_t<bf16, float>(a, s) : launch_join_t<bf16, bf16>(a, s);
+}
+
+}  // namespace sugar
+
+using namespace sugar;
+
+extern "C" int sugar_block_join(const SugarBlockJoin* h, void* stream) {
+  SUGAR_CHECK_ARG(h, "block_join: null descriptor");
+  const SugarBlockJoin& j = *h;
+  SUGAR_CHECK_ARG(j.rows >= 0 && j.rows < (1ll << 40) && j.cols > 0 && j.cols <= SUGAR_JOIN_MAX_COLS,
+                  "block_join: rows %lld, columns %d out of range (1..%d)", (long long)j.rows, j.cols, SUGAR_JOIN_MAX_COLS);
+  SUGAR_CHECK_ARG((j.u_dtype == SUGAR_F32 || j.u_dtype == SUGAR_BF16) && (j.stream_dtype == SUGAR_F32 || j.stream_dtype == SUGAR_BF16) &&
+                      (j.z_dtype == SUGAR_F32 || j.z_dtype == SUGAR_BF16),
+                  "block_join: bad dtype");
+  SUGAR_CHECK_ARG(!(j.u_dtype == SUGAR_F32 && j.stream_dtype == SUGAR_BF16), "block_join: a 32-bit block output needs a 32-bit stream");
+  SUGAR_CHECK_ARG(j.d_u && j.d_residual && (j.d_stream || j.d_z || j.d_q), "block_join: null pointer");
+  SUGAR_CHECK_ARG(norm_ok(j.post_kind) && norm_ok(j.pre_kind), "block_join: unknown norm");
+  SUGAR_CHECK_ARG(j.post_eps >= 0.f && j.pre_eps >= 0.f, "block_join: negative eps");
+  SUGAR_CHECK_ARG(j.gate_kind >= SUGAR_GATE_NONE && j.gate_kind <= SUGAR_GATE_ROW && (j.gate_kind == SUGAR_GATE_NONE) == !j.d_gate,
+                  "block_join: gate kind %d does not fit its pointer", j.gate_kind);
+  SUGAR_CHECK_ARG(j.gate_kind != SUGAR_GATE_UTTERANCE || j.d_row_off, "block_join: a gate per utterance needs row offsets");
+  SUGAR_CHECK_ARG(!j.d_row_off || j.n_utts > 0, "block_join: row offsets of no utterance");
+  SUGAR_CHECK_ARG(j.ldu >= j.cols && j.ldr >= j.cols && (!j.d_stream || j.lds >= j.cols) && (!j.d_z || j.ldz >= j.cols) &&
+                      (j.gate_kind < SUGAR_GATE_UTTERANCE || j.ldg >= j.cols),
+                  "block_join: a row stride is shorter than the row");
+  const uintptr_t eu = j.u_dtype == SUGAR_F32 ? 3 : 1, es = j.stream_dtype == SUGAR_F32 ? 3 : 1, ez = j.z_dtype == SUGAR_F32 ? 3 : 1;
+  SUGAR_CHECK_ARG(!((uintptr_t)j.d_u & eu) && !((uintptr_t)j.d_residual & es) && !((uintptr_t)j.d_stream & es) &&
+                      !((uintptr_t)j.d_z & ez) && !((uintptr_t)j.d_gate & (j.gate_kind == SUGAR_GATE_ROW ? eu : 3)) &&
+                      !((uintptr_t)j.d_post_w & 3) && !((uintptr_t)j.d_post_b & 3) && !((uintptr_t)j.d_pre_w & 3) &&
+                      !((uintptr_t)j.d_pre_b & 3) && !((uintptr_t)j.d_row_off & 3),
+                  "block_join: a pointer is not aligned to its type");
+  if (j.d_q)
+    SUGAR_CHECK_ARG(j.d_e && !((uintptr_t)j.d_q & 15) && j.ldq % 16 == 0 && j.ldq >= fp8_ldq(j.cols) && j.lde >= fp8_lds(j.cols),
+                    "block_join: bad 8-bit output");
+  if (j.rows == 0) return SUGAR_OK;
+  return launch_block_join(j, (hipStream_t)stream);
+}
