@@ -1,4 +1,4 @@
-// Quantisation to 8-bit operands with block scales, their reading back, and the matrix product of two of them (gfx950).
+// Quantisation to 8-bit operands with block scales, their reading back, and the C entries (gfx950; product: fp8_gemm.hip).
 // The format is described in blockfp8.h.
 #include "blockfp8.h"
 
@@ -52,85 +52,6 @@ __global__ __launch_bounds__(256) void fp8_dequant_kernel(const uint8_t* __restr
   }
 }
 
-// ------------------------------------------------------------------------------------------ matrix product
-struct LinearArgs {
-  const uint8_t *a, *ae, *w, *we;
-  int64_t lda, ldae, ldw, ldwe, ldy;
-  void* y;
-  const float *scale, *shift;
-  int rows, n, kb, flags, out_f32, vec;
-};
-
-// Epilogue of four consecutive channels of one row.
-__device__ __forceinline__ void store_out4(const LinearArgs& p, int64_t r, int co, f32x4 v) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (co + i >= p.n) break;
-    float t = v[i];
-    if (p.flags & EPI_RELU) t = t < 0.f ? 0.f : t;            // (NaN stays NaN)
-    if (p.flags & EPI_AFFINE) t = fmaf(t, p.scale[co + i], p.shift[co + i]);
-    if (p.out_f32) ((float*)p.y)[r * p.ldy + co + i] = t;
-    else ((bf16*)p.y)[r * p.ldy + co + i] = (bf16)t;
-  }
-}
-
-// Operands straight from memory into the matrix instruction's registers, K dealt out over the workgroup's waves and their
-// sums joined in LDS in wave order: 16 channels x 16 NT rows a workgroup.  WIDE: 16-bit products (float32 outputs).
-template <int NT, int NW, bool WIDE>
-__global__ __launch_bounds__(64 * NW) void fp8_linear_direct_kernel(LinearArgs p) {
-  __shared__ f32x4 part[NW][NT][64];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
-  const int co = blockIdx.x * 16, r0 = blockIdx.y * (16 * NT);
-  const int wrow = min(co + fr, p.n - 1);
-  const uint8_t* wp = p.w + (int64_t)wrow * p.ldw + fq * 32;
-  const uint8_t* wep = p.we + (int64_t)wrow * p.ldwe;
-  f32x4 acc[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) acc[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  for (int kb = wv; kb < p.kb; kb += NW) {
-    i32x8 wf;
-    *(i32x4*)&wf = *(const i32x4*)(wp + kb * 128);
-    *((i32x4*)&wf + 1) = *(const i32x4*)(wp + kb * 128 + 16);
-    bf16x8 wh[4];
-    int ew[4];
-    if constexpr (WIDE) {
-      fp8_to_bf16(wf, wh);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ew[i] = p.we[(int64_t)min(co + 4 * fq + i, p.n - 1) * p.ldwe + kb];
-    } else {
-      ew[0] = wep[kb];
-    }
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int ar = min(r0 + t * 16 + fr, p.rows - 1);
-      const uint8_t* ap = p.a + (int64_t)ar * p.lda + kb * 128 + fq * 32;
-      i32x8 af;
-      *(i32x4*)&af = *(const i32x4*)ap;
-      *((i32x4*)&af + 1) = *(const i32x4*)(ap + 16);
-      const int ea = p.ae[(int64_t)ar * p.ldae + kb];
-      if constexpr (WIDE) {
-        bf16x8 ah[4];
-        fp8_to_bf16(af, ah);
-        const f32x4 z = mfma_wide(wh, ah);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][i] = add_scaled(acc[t][i], z[i], ea, ew[i]);
-      } else {
-        acc[t] = mfma_fp8<0, 0>(wf, af, acc[t], ew[0], ea);
-      }
-    }
-  }
-#pragma unroll
-  for (int t = 0; t < NT; ++t) part[wv][t][lane] = acc[t];
-  __syncthreads();
-  for (int t = wv; t < NT; t += NW) {
-    f32x4 v = part[0][t][lane];
-#pragma unroll
-    for (int k = 1; k < NW; ++k) v += part[k][t][lane];
-    const int r = r0 + t * 16 + fr;
-    if (r < p.rows) store_out4(p, r, co + 4 * fq, v);
-  }
-}
-
 }  // namespace
 
 static int check_operand(const char* what, const uint8_t* q, int64_t ldq, const uint8_t* e, int64_t lde, int64_t cols) {
@@ -141,22 +62,6 @@ static int check_operand(const char* what, const uint8_t* q, int64_t ldq, const 
   SUGAR_CHECK_ARG(((uintptr_t)e & 3) == 0 && lde % 4 == 0 && lde >= fp8_lds(cols),
                   "%s: rows of exponent bytes must be 4-byte aligned and hold %lld bytes (stride %lld)", what,
                   (long long)fp8_lds(cols), (long long)lde);
-  return SUGAR_OK;
-}
-
-int launch_fp8_linear(const Fp8Operand& a, int64_t rows, const Fp8Operand& w, int n, int k, const float* scale,
-                      const float* shift, int flags, void* d_y, int64_t ldy, int dtype, hipStream_t s) {
-  LinearArgs p;
-  p.a = a.q; p.ae = a.e; p.lda = a.ldq; p.ldae = a.lde;
-  p.w = w.q; p.we = w.e; p.ldw = w.ldq; p.ldwe = w.lde;
-  p.y = d_y; p.ldy = ldy; p.scale = scale; p.shift = shift;
-  p.rows = (int)rows; p.n = n; p.kb = (int)fp8_blocks(k); p.flags = flags; p.out_f32 = dtype == SUGAR_F32;
-  p.vec = 0;
-  constexpr int NT = 2, NW = 4;
-  const dim3 grid((unsigned)ceil_div(n, 16), (unsigned)ceil_div(rows, 16 * NT));
-  if (p.out_f32) hipLaunchKernelGGL((fp8_linear_direct_kernel<NT, NW, true>), grid, dim3(64 * NW), 0, s, p);
-  else hipLaunchKernelGGL((fp8_linear_direct_kernel<NT, NW, false>), grid, dim3(64 * NW), 0, s, p);
-  SUGAR_LAUNCH_CHECK();
   return SUGAR_OK;
 }
 

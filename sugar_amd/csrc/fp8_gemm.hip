@@ -1,0 +1,623 @@
+// Matrix product of two 8-bit operands with block scales (format and instructions: blockfp8.h), gfx950.
+//
+//   y[r][o] = relu(sum_k a[r][k] w[o][k]) * scale[o] + shift[o]
+//
+//   direct     few rows: operands from memory into registers, K dealt out over the waves of a workgroup
+//   tile       TM channels x TN rows a workgroup, k-tiles of one 128-column block through an LDS ring filled by DMA
+//   persist    256 x 256 tiles walked by one workgroup per CU (bf16 outputs of large products)
+//
+// A k-tile row is 128 bytes in LDS as it is in the 16-bit GEMMs of conv1x1.hip (there 64 columns): the same bytes per
+// step, the same chunk swizzle, the same matrix-pipe time per step, and twice the operations.
+#include "blockfp8.h"
+
+namespace sugar {
+
+namespace {
+
+struct LinearArgs {
+  const uint8_t *a, *ae, *w, *we;
+  unsigned lda, ldae, ldw, ldwe;      // rows x stride fits 32 bits (launch_fp8_linear cuts longer operands)
+  int64_t ldy;
+  void* y;
+  const float *scale, *shift;
+  int rows, n, kb, flags, out_f32;
+  int vec;                            // 16-byte stores: y aligned, n and ldy multiples of 16 bytes
+  int n_co_tiles;
+};
+
+// ReLU in one instruction that hands NaN on (a maximum, not a maxNum)
+__device__ __forceinline__ float relu_nan(float v) { return __builtin_elementwise_maximum(v, 0.f); }
+
+__device__ __forceinline__ int swz(int row, int chunk) { return row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4); }
+
+__device__ __forceinline__ int xcd_remap(int bid, int nwg) {
+  const int q = nwg >> 3, r = nwg & 7, xcd = bid & 7, seq = bid >> 3;
+  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + seq;
+}
+
+// Memory -> LDS, BYTES a lane to consecutive LDS addresses: uniform base (in scalar registers, kept apart from the lane's
+// 32-bit offset: hipcc would otherwise carry a 64-bit address per instruction through the k-loop and spill) + offset.
+template <int BYTES>
+__device__ __forceinline__ void dma(const uint8_t* base, unsigned off, unsigned char* lds) {
+  asm("" : "+s"(base));
+  const auto src = (const __attribute__((address_space(1))) void*)(base + off);
+  const auto dst = (__attribute__((address_space(3))) void*)lds;
+  if constexpr (BYTES == 16) __builtin_amdgcn_global_load_lds(src, dst, 16, 0, 0);
+  else __builtin_amdgcn_global_load_lds(src, dst, 4, 0, 0);
+}
+
+// lane (fr, fq)'s 32 bytes of a k-tile row: chunks fq and 4 + fq (any 32, the same for both operands)
+__device__ __forceinline__ i32x8 frag(const unsigned char* base, int row, int fq) {
+  i32x8 f;
+  *(i32x4*)&f = *(const i32x4*)(base + swz(row, fq));
+  *((i32x4*)&f + 1) = *(const i32x4*)(base + swz(row, 4 + fq));
+  return f;
+}
+
+// Epilogue and store of four consecutive channels of one row, straight from the accumulators.
+__device__ __forceinline__ void store_out4(const LinearArgs& p, int64_t r, int co, f32x4 v) {
+  if (p.flags & EPI_RELU) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = relu_nan(v[i]);
+  }
+  if (p.vec && p.out_f32) {
+    if (co >= p.n) return;
+    if (p.flags & EPI_AFFINE) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = fmaf(v[i], p.scale[co + i], p.shift[co + i]);
+    }
+    *(f32x4*)((float*)p.y + r * p.ldy + co) = v;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (co + i >= p.n) break;
+    const float t = p.flags & EPI_AFFINE ? fmaf(v[i], p.scale[co + i], p.shift[co + i]) : v[i];
+    if (p.out_f32) ((float*)p.y)[r * p.ldy + co + i] = t;
+    else ((bf16*)p.y)[r * p.ldy + co + i] = (bf16)t;
+  }
+}
+
+// ------------------------------------------------------------------------------------------ few rows
+// Operands straight from memory into the matrix instruction's registers, K dealt out over the workgroup's waves and their
+// sums joined in LDS in wave order: 16 channels x 16 NT rows a workgroup.  WIDE: 16-bit products (float32 outputs).
+template <int NT, int NW, bool WIDE>
+__global__ __launch_bounds__(64 * NW) void fp8_linear_direct_kernel(LinearArgs p) {
+  __shared__ f32x4 part[NW][NT][64];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
+  const int co = blockIdx.x * 16, r0 = blockIdx.y * (16 * NT);
+  const int wrow = min(co + fr, p.n - 1);
+  const uint8_t* wp = p.w + (unsigned)wrow * p.ldw + fq * 32;
+  const uint8_t* wep = p.we + (unsigned)wrow * p.ldwe;
+  f32x4 acc[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) acc[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  for (int kb = wv; kb < p.kb; kb += NW) {
+    i32x8 wf;
+    *(i32x4*)&wf = *(const i32x4*)(wp + kb * 128);
+    *((i32x4*)&wf + 1) = *(const i32x4*)(wp + kb * 128 + 16);
+    bf16x8 wh[4];
+    int ew[4];
+    if constexpr (WIDE) {
+      fp8_to_bf16(wf, wh);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ew[i] = p.we[(unsigned)min(co + 4 * fq + i, p.n - 1) * p.ldwe + kb];
+    } else {
+      ew[0] = wep[kb];
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int ar = min(r0 + t * 16 + fr, p.rows - 1);
+      const uint8_t* ap = p.a + (unsigned)ar * p.lda + kb * 128 + fq * 32;
+      i32x8 af;
+      *(i32x4*)&af = *(const i32x4*)ap;
+      *((i32x4*)&af + 1) = *(const i32x4*)(ap + 16);
+      const int ea = p.ae[(unsigned)ar * p.ldae + kb];
+      if constexpr (WIDE) {
+        bf16x8 ah[4];
+        fp8_to_bf16(af, ah);
+        const f32x4 z = mfma_wide(wh, ah);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][i] = add_scaled(acc[t][i], z[i], ea, ew[i]);
+      } else {
+        acc[t] = mfma_fp8<0, 0>(wf, af, acc[t], ew[0], ea);
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) part[wv][t][lane] = acc[t];
+  __syncthreads();
+  for (int t = wv; t < NT; t += NW) {
+    f32x4 v = part[0][t][lane];
+#pragma unroll
+    for (int k = 1; k < NW; ++k) v += part[k][t][lane];
+    const int r = r0 + t * 16 + fr;
+    if (r < p.rows) store_out4(p, r, co + 4 * fq, v);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ one tile
+// One TM x TN output tile by a workgroup of 8 waves = 2 (channels) x 4 (rows).  Ring of NS stages: wait for this wave's
+// share of k-tile t, barrier, issue the DMA of k-tile t + NS - 1 into the buffer k-tile t - 1 was read from, compute.
+// Exponents travel as one dword per row and four k-tiles, staged with the first of the four (double buffer) and shifted
+// down a byte per k-tile.
+constexpr int linear_tile_lds(int TM, int TN, int NS) { return (TM + TN) * (NS * 128 + 8); }
+
+template <int TM, int TN, int NS, bool WIDE>
+__device__ __forceinline__ void fp8_tile(const LinearArgs& p, const int co_base, const int r_base) {
+  constexpr int STAGE_BYTES = (TM + TN) * 128;
+  constexpr int MI = TM / 32, NJ = TN / 64, CW = TM / 2, FW = TN / 4, WI = TM / 64, XI = TN / 64, SI = (TM + TN) / 64;
+  constexpr int D = NS - 1, NDMA = WI + XI;
+  static_assert(SI <= 8, "one exponent instruction per wave");
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wv >> 2, wn = wv & 3, fr = lane & 15, fq = lane >> 4;
+  unsigned* exps = (unsigned*)(smem + NS * STAGE_BYTES);         // [2][TM + TN]
+  const int nk = p.kb;
+
+  unsigned woff[WI], xoff[XI];
+#pragma unroll
+  for (int i = 0; i < WI; ++i) {
+    const int row = wv * (WI * 8) + i * 8 + (lane >> 3);         // rows past n: any valid one, masked at the store
+    woff[i] = (unsigned)min(co_base + row, p.n - 1) * p.ldw + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+  }
+#pragma unroll
+  for (int i = 0; i < XI; ++i) {
+    const int row = wv * (XI * 8) + i * 8 + (lane >> 3);
+    xoff[i] = (unsigned)min(r_base + row, p.rows - 1) * p.lda + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+  }
+  const int erow = wv * 64 + lane;
+  const uint8_t* ebase = wv * 64 < TM ? p.we : p.ae;
+  const unsigned eoff = wv * 64 < TM ? (unsigned)min(co_base + erow, p.n - 1) * p.ldwe
+                                     : (unsigned)min(r_base + erow - TM, p.rows - 1) * p.ldae;
+  auto stage = [&](int buf, int kt) {
+    if ((kt & 3) == 0 && wv < SI) dma<4>(ebase + kt, eoff, (unsigned char*)(exps + ((kt >> 2) & 1) * (TM + TN) + wv * 64));
+    unsigned char* wbase = smem + buf * STAGE_BYTES + wv * (WI * 8) * 128;
+    unsigned char* xbase = smem + buf * STAGE_BYTES + TM * 128 + wv * (XI * 8) * 128;
+#pragma unroll
+    for (int i = 0; i < WI; ++i) dma<16>(p.w + kt * 128, woff[i], wbase + i * 1024);
+#pragma unroll
+    for (int i = 0; i < XI; ++i) dma<16>(p.a + kt * 128, xoff[i], xbase + i * 1024);
+  };
+
+  f32x4 acc[MI][NJ];
+#pragma unroll
+  for (int m = 0; m < MI; ++m)
+#pragma unroll
+    for (int n = 0; n < NJ; ++n) acc[m][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  int ew[WIDE ? 4 * MI : MI], ex[NJ];
+  unsigned bad_w = 0, bad_x = 0;                                 // WIDE: bit per channel / row of this lane with a NaN exponent
+
+#pragma unroll
+  for (int t = 0; t < D; ++t)
+    if (t < nk) stage(t, t);
+  int cur = 0, nxt = D;
+  for (int kt = 0; kt < nk; ++kt) {
+    // this wave's share of k-tile kt has landed (younger ones may stay in flight; an exponent instruction among them only
+    // makes the wait longer), then everyone's has
+    if (D > 1 && kt + D - 1 < nk) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * NDMA) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (kt + D < nk) stage(nxt, kt + D);
+    const unsigned char* wb = smem + cur * STAGE_BYTES;
+    const unsigned char* xb = wb + TM * 128;
+    if ((kt & 3) == 0) {
+      const unsigned* e = exps + ((kt >> 2) & 1) * (TM + TN);
+#pragma unroll
+      for (int m = 0; m < MI; ++m) {
+        if constexpr (WIDE) {
+          const i32x4 t = *(const i32x4*)(e + wm * CW + m * 16 + 4 * fq);    // the channels of this lane's results
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ew[4 * m + i] = t[i];
+        } else {
+          ew[m] = e[wm * CW + m * 16 + fr];
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NJ; ++n) ex[n] = e[TM + wn * FW + n * 16 + fr];
+    }
+    if constexpr (WIDE) {
+      bf16x8 xh[NJ][4];
+#pragma unroll
+      for (int n = 0; n < NJ; ++n) {
+        fp8_to_bf16(frag(xb, wn * FW + n * 16 + fr, fq), xh[n]);
+        bad_x |= (ex[n] & 255) == 255 ? 1u << n : 0u;
+      }
+#pragma unroll
+      for (int m = 0; m < MI; ++m) {
+        bf16x8 wh[4];
+        fp8_to_bf16(frag(wb, wm * CW + m * 16 + fr, fq), wh);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bad_w |= (ew[4 * m + i] & 255) == 255 ? 1u << (4 * m + i) : 0u;
+#pragma unroll
+        for (int n = 0; n < NJ; ++n) {
+          const f32x4 z = mfma_wide(wh, xh[n]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[m][n][i] += __builtin_amdgcn_ldexpf(z[i], (ew[4 * m + i] & 255) + (ex[n] & 255) - 254);
+        }
+      }
+    } else {
+      i32x8 xf[NJ];
+#pragma unroll
+      for (int n = 0; n < NJ; ++n) xf[n] = frag(xb, wn * FW + n * 16 + fr, fq);
+#pragma unroll
+      for (int m = 0; m < MI; ++m) {
+        const i32x8 wf = frag(wb, wm * CW + m * 16 + fr, fq);
+#pragma unroll
+        for (int n = 0; n < NJ; ++n) acc[m][n] = mfma_fp8<0, 0>(wf, xf[n], acc[m][n], ew[m], ex[n]);
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < (WIDE ? 4 * MI : MI); ++m) ew[m] = (int)((unsigned)ew[m] >> 8);
+#pragma unroll
+    for (int n = 0; n < NJ; ++n) ex[n] = (int)((unsigned)ex[n] >> 8);
+    cur = cur + 1 == NS ? 0 : cur + 1;
+    nxt = nxt + 1 == NS ? 0 : nxt + 1;
+  }
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int m = 0; m < MI; ++m)
+#pragma unroll
+      for (int n = 0; n < NJ; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if ((bad_w >> (4 * m + i) | bad_x >> n) & 1) acc[m][n][i] = __uint_as_float(0x7fc00000u);
+  }
+
+  // ---- epilogue: accumulator tile (m, n): lane (fr, fq) holds row wn FW + n 16 + fr, channels wm CW + m 16 + 4 fq + 0..3
+  if (p.out_f32 || !p.vec) {                                     // 16 bytes a lane, 64 in a row (or odd widths)
+#pragma unroll
+    for (int n = 0; n < NJ; ++n) {
+      const int r = r_base + wn * FW + n * 16 + fr;
+      if (r >= p.rows) continue;
+#pragma unroll
+      for (int m = 0; m < MI; ++m) store_out4(p, r, co_base + wm * CW + m * 16 + 4 * fq, acc[m][n]);
+    }
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // stage memory free: epilogue staging, or the caller's next tile
+  if (p.out_f32 || !p.vec) return;
+  constexpr int EPI_STRIDE = CW * 2 + 16, CPR = CW / 8, RPP = 64 / CPR;
+  static_assert(8 * 16 * EPI_STRIDE <= NS * STAGE_BYTES, "epilogue staging fits the stages");
+  unsigned char* ep = smem + wv * (16 * EPI_STRIDE);             // this wave's [16 rows][CW channels]
+#pragma unroll
+  for (int n = 0; n < NJ; ++n) {
+#pragma unroll
+    for (int m = 0; m < MI; ++m) {
+      const int col = m * 16 + 4 * fq, co = co_base + wm * CW + col;
+      f32x4 v = acc[m][n];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (p.flags & EPI_RELU) v[i] = relu_nan(v[i]);
+        if (p.flags & EPI_AFFINE) v[i] = fmaf(v[i], p.scale[min(co + i, p.n - 1)], p.shift[min(co + i, p.n - 1)]);
+      }
+      const bf16x4 o = {(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
+      *(bf16x4*)(ep + fr * EPI_STRIDE + col * 2) = o;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // the staging is the wave's own: no workgroup barrier
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < 16 / RPP; ++i) {
+      const int f = i * RPP + lane / CPR, ch = lane % CPR;
+      const int r = r_base + wn * FW + n * 16 + f, co = co_base + wm * CW + ch * 8;
+      const u32x4 v = *(const u32x4*)(ep + f * EPI_STRIDE + ch * 16);
+      if (r < p.rows && co < p.n) *(u32x4*)((bf16*)p.y + (int64_t)r * p.ldy + co) = v;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+template <int TM, int TN, int NS, bool WIDE>
+__global__ __launch_bounds__(512, 4) void fp8_linear_tile_kernel(LinearArgs p) {
+  const int vid = xcd_remap(blockIdx.x, gridDim.x);
+  fp8_tile<TM, TN, NS, WIDE>(p, (vid % p.n_co_tiles) * TM, (vid / p.n_co_tiles) * TN);
+}
+
+template <int TM, int TN, int NS, bool WIDE>
+int launch_tile(LinearArgs p, hipStream_t s) {
+  constexpr int smem = linear_tile_lds(TM, TN, NS);
+  static OptInMask opted{0};
+  if (int rc = lds_opt_in((const void*)fp8_linear_tile_kernel<TM, TN, NS, WIDE>, smem, &opted)) return rc;
+  p.n_co_tiles = (int)ceil_div(p.n, TM);
+  const int64_t grid = p.n_co_tiles * ceil_div(p.rows, TN);
+  hipLaunchKernelGGL((fp8_linear_tile_kernel<TM, TN, NS, WIDE>), dim3((unsigned)grid), dim3(512), smem, s, p);
+  SUGAR_LAUNCH_CHECK();
+  return SUGAR_OK;
+}
+
+// ------------------------------------------------------------------------------------------ persistent 256 x 256 tiles
+// One workgroup per CU walks its tiles; the schedule is that of gemm_tiles_persist (conv1x1.hip, two phases a k-tile):
+//   phase 1   reads b0, a0, b1 | barrier | a0 x b0, a0 x b1      DMA: weights of the next k-tile
+//   phase 2   reads a1         | barrier | a1 x b1, a1 x b0      DMA: activations of the k-tile after next
+// on a 128 x 64 wave tile of 16 x 16 x 128 products, operand fragments in registers; the two waves of a SIMD run one
+// barrier apart, so one's reads lie under the other's products.  The DMA stream runs on into the next tile under the
+// epilogue.  Beside it: exponents, one dword a row and four k-tiles, issued with the weights of the first of the four; the
+// affine vectors of the tile's 256 channels, issued with its first k-tile.
+// k-tiles alternate between the two stages across tiles too (any number of them), the epilogue is staged through the one
+// the last k-tile was in; it needs 4 KiB more than a stage, which lie between the two.
+constexpr int PT = 256, PSTAGE = 2 * PT * 128, PGAP = 4096;
+constexpr int PEXPS = 2 * PSTAGE + PGAP, PAFF = PEXPS + 2 * 512 * 4, PERSIST_LDS = PAFF + 2 * PT * 4;
+
+__device__ __forceinline__ void fp8_tiles_persist(const LinearArgs& p, const int first, const int stride, const int rounds) {
+  constexpr int MI = 8, NJ = 4, CW = 128, FW = 64, XI = 4;
+  constexpr int EPI_STRIDE = CW * 2 + 16, HN = 2, CPR = CW / 8, RPP = 64 / CPR, NSTORE = (NJ / HN) * (16 * HN / RPP);
+  static_assert(8 * 16 * HN * EPI_STRIDE <= PSTAGE + PGAP, "epilogue staging");
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wv >> 2, wn = wv & 3, srow = lane >> 3, fr = lane & 15, fq = lane >> 4;
+  const int nk = p.kb;
+  const bool relu = p.flags & EPI_RELU, affine = p.flags & EPI_AFFINE;
+  unsigned* exps = (unsigned*)(smem + PEXPS);                    // [2][256 channels | 256 rows]
+  float* aff = (float*)(smem + PAFF);                            // [scale 256 | shift 256]
+
+  unsigned woff[4], xoff[4], eoff;
+  const uint8_t* ebase = wv < 4 ? p.we : p.ae;                   // exponents: waves 0..3 the channels', 4..7 the rows'
+  auto point_w = [&](int co_base, int r_base) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = wv * 32 + i * 8 + srow;                    // rows past the end: any valid one, masked at the store
+      woff[i] = (unsigned)min(co_base + row, p.n - 1) * p.ldw + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+    }
+    eoff = wv < 4 ? (unsigned)min(co_base + wv * 64 + lane, p.n - 1) * p.ldwe
+                  : (unsigned)min(r_base + (wv - 4) * 64 + lane, p.rows - 1) * p.ldae;
+  };
+  auto point_x = [&](int r_base) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = wv * 32 + i * 8 + srow;
+      xoff[i] = (unsigned)min(r_base + row, p.rows - 1) * p.lda + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+    }
+  };
+  auto stage_at = [&](int buf) { return smem + buf * (PSTAGE + PGAP); };
+  auto dma_w = [&](int buf, int kt, int i0) {
+    unsigned char* base = stage_at(buf) + wv * 4096;
+#pragma unroll
+    for (int i = i0; i < i0 + 2; ++i) dma<16>(p.w + kt * 128, woff[i], base + i * 1024);
+  };
+  auto dma_x = [&](int buf, int kt, int i0) {
+    unsigned char* base = stage_at(buf) + PT * 128 + wv * 4096;
+#pragma unroll
+    for (int i = i0; i < i0 + 2; ++i) dma<16>(p.a + kt * 128, xoff[i], base + i * 1024);
+  };
+  int gbuf = 0;                                                  // exponent buffer the next group goes to, then is read from
+  auto dma_e = [&](int kt) { dma<4>(ebase + kt, eoff, (unsigned char*)(exps + gbuf * 512 + wv * 64)); };
+  auto tile_at = [&](int r, int& co_base, int& r_base) {
+    const int vid = first + r * stride;
+    co_base = (vid % p.n_co_tiles) * PT;
+    r_base = (vid / p.n_co_tiles) * PT;
+  };
+  // fragment addresses within a stage: chunks fq and 4 + fq of row fr, 16 rows further are 2 KiB further
+  const int a0 = swz(wm * CW + fr, fq), a1 = swz(wm * CW + fr, 4 + fq);
+  const int b0 = PT * 128 + swz(wn * FW + fr, fq), b1 = PT * 128 + swz(wn * FW + fr, 4 + fq);
+
+  f32x4 acc[MI][NJ];
+#pragma unroll
+  for (int m = 0; m < MI; ++m)
+#pragma unroll
+    for (int n = 0; n < NJ; ++n) acc[m][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  int ew[MI], ex[NJ];
+
+  int co_base, r_base, par = 0;                                  // par: stage of the tile's first k-tile
+  tile_at(0, co_base, r_base);
+  point_w(co_base, r_base);
+  point_x(r_base);
+  dma_e(0);
+  dma_w(0, 0, 0);
+  dma_w(0, 0, 2);
+  dma_x(0, 0, 0);
+  dma_x(0, 0, 2);
+  bool counted = false;                                          // the wait below may leave NSTORE younger stores in flight
+  for (int r = 0; r < rounds; ++r) {
+    if (counted) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NSTORE) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the tile's first k-tile is there, every wave out of its epilogue
+    if (affine) {                                                // the tile's 256 scales | 256 shifts, 64 a wave
+      const int c = min(co_base + (wv & 3) * 64 + lane, p.n - 1);
+      dma<4>((const uint8_t*)(wv < 4 ? p.scale : p.shift), 4 * c, (unsigned char*)(aff + wv * 64));
+    }
+    dma_x(par ^ 1, 1, 0);                                        // (not staged earlier: the epilogue went through that stage)
+    dma_x(par ^ 1, 1, 2);
+    if (wm) asm volatile("s_barrier" ::: "memory");              // group 1 runs one barrier behind
+    // the last tile prefetches itself again: the loop stays without conditions, nobody reads what arrives
+    int co_next, r_next;
+    tile_at(r + 1 < rounds ? r + 1 : r, co_next, r_next);
+    for (int kt = 0; kt < nk; ++kt) {
+      const int cur = (par + kt) & 1;
+      const unsigned char* st = stage_at(cur);
+      i32x8 af[4], bl[2], bh[2];
+      auto read = [&](int lo, int hi, int t) {
+        i32x8 f;
+        *(i32x4*)&f = *(const i32x4*)(st + lo + t * 2048);
+        *((i32x4*)&f + 1) = *(const i32x4*)(st + hi + t * 2048);
+        return f;
+      };
+      // products of one 64 x 32 quadrant; the empty asm holds them on this side of the barriers (they have no side effects
+      // and hipcc sinks them to the next use otherwise)
+      auto quad = [&](int m0, i32x8 (&b)[2], int n0) {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+            acc[m0 + m][n0 + n] = mfma_fp8<0, 0>(af[m], b[n], acc[m0 + m][n0 + n], ew[m0 + m], ex[n0 + n]);
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+          for (int n = 0; n < 2; ++n) asm volatile("" : "+v"(acc[m0 + m][n0 + n]));
+        __builtin_amdgcn_s_setprio(0);
+      };
+      auto close_read = [&]() {
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      auto close_mfma = [&](bool last) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (!last) asm volatile("s_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      // ---- phase 1
+      const unsigned* e = exps + gbuf * 512;
+#pragma unroll
+      for (int m = 0; m < MI; ++m) ew[m] = (int)(e[wm * CW + m * 16 + fr] >> (8 * (kt & 3)));
+#pragma unroll
+      for (int n = 0; n < NJ; ++n) ex[n] = (int)(e[256 + wn * FW + n * 16 + fr] >> (8 * (kt & 3)));
+      // (opaque: hipcc would peel the last two k-tiles off into copies of the loop body that spill)
+      int left = nk - 1 - kt;
+      asm volatile("" : "+s"(left));
+      const bool end = left == 0;
+      const int kw = end ? 0 : kt + 1;                           // k-tile whose weights are staged now
+      if (end) point_w(co_next, r_next);
+      if ((kw & 3) == 0) {                                       // its group of exponents
+        gbuf ^= 1;
+        dma_e(kw);
+      }
+      dma_w(cur ^ 1, kw, 0);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) bl[n] = read(b0, b1, n);
+#pragma unroll
+      for (int m = 0; m < 4; ++m) af[m] = read(a0, a1, m);
+      dma_w(cur ^ 1, kw, 2);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) bh[n] = read(b0, b1, 2 + n);
+      close_read();
+      quad(0, bl, 0);
+      quad(0, bh, 2);
+      close_mfma(false);
+      // ---- phase 2: activations two k-tiles ahead, into the half of THIS stage that nobody reads any more
+      const int kx = left > 1 ? kt + 2 : 0;
+      if (left == 1) point_x(r_next);
+      if (!end) dma_x(cur, kx, 0);
+#pragma unroll
+      for (int m = 0; m < 4; ++m) af[m] = read(a0, a1, 4 + m);
+      if (!end) {
+        dma_x(cur, kx, 2);
+        // k-tile kt + 1 has landed (this wave's share) once only the activations issued in this phase are outstanding
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(XI) : "memory");
+      }
+      close_read();
+      quad(4, bh, 2);
+      quad(4, bl, 0);
+      close_mfma(wm && end);
+    }
+    // ---- epilogue, staged where the last k-tile was (nobody reads it any more)
+    const int co_cur = co_base, r_cur = r_base;
+    counted = r_cur + PT <= p.rows && co_cur + PT <= p.n;        // exactly NSTORE stores follow, none masked off
+    unsigned char* ep = smem + (((par + nk - 1) & 1) ? PSTAGE : 0) + wv * (16 * HN * EPI_STRIDE);
+#pragma unroll
+    for (int pass = 0; pass < NJ / HN; ++pass) {
+#pragma unroll
+      for (int m = 0; m < MI; ++m) {
+        const int col = m * 16 + 4 * fq;
+        f32x4 sc = {1.f, 1.f, 1.f, 1.f}, sh = {0.f, 0.f, 0.f, 0.f};
+        if (affine) {
+          sc = *(const f32x4*)(aff + wm * CW + col);
+          sh = *(const f32x4*)(aff + PT + wm * CW + col);
+        }
+#pragma unroll
+        for (int nn = 0; nn < HN; ++nn) {
+          f32x4 v = acc[m][pass * HN + nn];
+          acc[m][pass * HN + nn] = (f32x4){0.f, 0.f, 0.f, 0.f};
+          if (relu) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = relu_nan(v[e]);
+          }
+          if (affine) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = fmaf(v[e], sc[e], sh[e]);
+          }
+          const bf16x4 o = {(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
+          *(bf16x4*)(ep + (nn * 16 + fr) * EPI_STRIDE + col * 2) = o;
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int i = 0; i < 16 * HN / RPP; ++i) {
+        const int f = i * RPP + lane / CPR, ch = lane % CPR;
+        const int rr = r_cur + wn * FW + pass * (16 * HN) + f, co = co_cur + wm * CW + ch * 8;
+        const u32x4 v = *(const u32x4*)(ep + f * EPI_STRIDE + ch * 16);
+        if (rr < p.rows && co < p.n) *(u32x4*)((bf16*)p.y + (int64_t)rr * p.ldy + co) = v;
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_wave_barrier();
+    }
+    par = (par + nk) & 1;
+    co_base = co_next;
+    r_base = r_next;
+  }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");     // nothing on its way to LDS, staging free: a tail piece may use it
+}
+
+// grid = the CU count (a multiple of 8); rounds * grid tiles of 256 x 256, then `tail` tiles cut into 256 x 128 or 256 x 64
+// pieces, so that a last round that is not full is also shorter
+__global__ __launch_bounds__(512, 2) void fp8_linear_persist_kernel(LinearArgs p, int rounds, int tail, int split) {
+  const int bid = blockIdx.x, nwg = gridDim.x, xcd = bid & 7, seq = bid >> 3, wpx = nwg >> 3;
+  // XCD x owns the contiguous tile range [x rounds wpx, (x + 1) rounds wpx); its workgroups take consecutive tiles of it,
+  // so tiles that share activation rows run at the same time on one XCD (shared L2)
+  if (rounds) fp8_tiles_persist(p, xcd * rounds * wpx + seq, wpx, rounds);
+  for (int i = bid; i < tail * split; i += nwg) {
+    const int tile = rounds * nwg + i / split, sub = i % split;
+    const int co_base = (tile % p.n_co_tiles) * PT, r_tile = (tile / p.n_co_tiles) * PT;
+    if (split == 4) {
+      if (r_tile + sub * 64 < p.rows) fp8_tile<256, 64, 2, false>(p, co_base, r_tile + sub * 64);
+    } else {
+      if (r_tile + sub * 128 < p.rows) fp8_tile<256, 128, 2, false>(p, co_base, r_tile + sub * 128);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the piece's epilogue staging has been read
+  }
+}
+
+int launch_persist(LinearArgs p, int n_cu, hipStream_t s) {
+  static OptInMask opted{0};
+  if (int rc = lds_opt_in((const void*)fp8_linear_persist_kernel, PERSIST_LDS, &opted)) return rc;
+  p.n_co_tiles = (int)ceil_div(p.n, PT);
+  const int total = (int)(p.n_co_tiles * ceil_div(p.rows, PT)), rounds = total / n_cu, tail = total - rounds * n_cu;
+  hipLaunchKernelGGL(fp8_linear_persist_kernel, dim3(n_cu), dim3(512), PERSIST_LDS, s, p, rounds, tail, tail * 4 <= n_cu ? 4 : 2);
+  SUGAR_LAUNCH_CHECK();
+  return SUGAR_OK;
+}
+
+int launch_rows(const LinearArgs& p, hipStream_t s) {
+  int n_cu = 0;
+  if (int rc = device_cu_count(&n_cu)) return rc;
+  const int64_t t128 = ceil_div(p.n, 128) * ceil_div(p.rows, 128);
+  if (!p.out_f32 && p.vec && p.kb >= 2 && n_cu % 8 == 0 && ceil_div(p.n, 256) * ceil_div(p.rows, 256) >= n_cu)
+    return launch_persist(p, n_cu, s);
+  if (t128 >= n_cu) return p.out_f32 ? launch_tile<128, 128, 2, true>(p, s) : launch_tile<128, 128, 2, false>(p, s);
+  if (p.rows > 64 && ceil_div(p.n, 64) * ceil_div(p.rows, 64) >= 64)
+    return p.out_f32 ? launch_tile<64, 64, 4, true>(p, s) : launch_tile<64, 64, 4, false>(p, s);
+  constexpr int NT = 2, NW = 4;
+  const dim3 grid((unsigned)ceil_div(p.n, 16), (unsigned)ceil_div(p.rows, 16 * NT));
+  if (p.out_f32) hipLaunchKernelGGL((fp8_linear_direct_kernel<NT, NW, true>), grid, dim3(64 * NW), 0, s, p);
+  else hipLaunchKernelGGL((fp8_linear_direct_kernel<NT, NW, false>), grid, dim3(64 * NW), 0, s, p);
+  SUGAR_LAUNCH_CHECK();
+  return SUGAR_OK;
+}
+
+}  // namespace
+
+int launch_fp8_linear(const Fp8Operand& a, int64_t rows, const Fp8Operand& w, int n, int k, const float* scale,
+                      const float* shift, int flags, void* d_y, int64_t ldy, int dtype, hipStream_t s) {
+  // the kernels' row offsets are 32-bit: weights that do not fit are refused, rows beyond go to a launch of their own
+  constexpr int64_t SPAN = (1ll << 32) - 4096;
+  SUGAR_CHECK_ARG(n * w.ldq <= SPAN && n * w.lde <= SPAN, "fp8_linear: weights of %d rows with stride %lld are too large", n,
+                  (long long)w.ldq);
+  SUGAR_CHECK_ARG(a.ldq <= SPAN / 256 && a.lde <= SPAN / 256, "fp8_linear: row stride %lld too large", (long long)a.ldq);
+  const int64_t per = SPAN / (a.ldq > a.lde ? a.ldq : a.lde) / 256 * 256;
+  const int esz = dtype == SUGAR_F32 ? 4 : 2;
+  LinearArgs p;
+  p.lda = (unsigned)a.ldq; p.ldae = (unsigned)a.lde;
+  p.w = w.q; p.we = w.e; p.ldw = (unsigned)w.ldq; p.ldwe = (unsigned)w.lde;
+  p.ldy = ldy; p.scale = scale; p.shift = shift;
+  p.n = n; p.kb = (int)fp8_blocks(k); p.flags = flags; p.out_f32 = dtype == SUGAR_F32; p.n_co_tiles = 0;
+  p.vec = ((uintptr_t)d_y & 15) == 0 && (ldy * esz) % 16 == 0 && (n * esz) % 16 == 0;
+  for (int64_t r0 = 0; r0 < rows; r0 += per) {
+    p.a = a.q + r0 * a.ldq; p.ae = a.e + r0 * a.lde;
+    p.y = (char*)d_y + r0 * ldy * esz;
+    p.rows = (int)(rows - r0 < per ? rows - r0 : per);
+    if (int rc = launch_rows(p, s)) return rc;
+  }
+  return SUGAR_OK;
+}
+
+}  // namespace sugar
