@@ -18,18 +18,19 @@ enum { NORM_NONE = SUGAR_NORM_NONE, NORM_AFFINE = SUGAR_NORM_AFFINE, NORM_RMS = 
 
 struct JoinArgs {
   SugarBlockJoin j;
-  int vec_u, vec_r, vec_s, vec_z, vec_g;     // rows that can be read / written 16 bytes at a time
 };
 
-// Sum over the 64 lanes, the same in every lane, by DPP (rows of 16, then across rows).
+// Sum over the 64 lanes, the same in every lane: within rows of 16 by DPP, across them by the row / half swaps (of a value
+// with itself: the two results are the two halves, each in all lanes).
 __device__ __forceinline__ float wave_total(float v) {
   v += dpp_row_f32<0xB1>(v);
   v += dpp_row_f32<0x4E>(v);
   v += dpp_row_f32<0x141>(v);
   v += dpp_row_f32<0x140>(v);
-  v += __shfl_xor(v, 16);
-  v += __shfl_xor(v, 32);
-  return v;
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
 template <int WPR>
@@ -46,12 +47,61 @@ __device__ __forceinline__ float row_total(float v, float* red, int wv) {
   return v;
 }
 
-// x <- norm(x) over the row's C channels; lanes past the row hold zeros before and whatever the weights say after.
+// Eight channels as they lie in memory, fetched without a branch and without touching the values, so that every load of a
+// row is on its way before the first is used.  VEC: 16-byte loads; a lane past the row reads the row's beginning.
+template <typename T, bool VEC>
+struct Raw8 {
+  u32x4 q[sizeof(T) / 2];
+  float f[VEC ? 1 : 8];
+  __device__ __forceinline__ void load(const T* __restrict__ p, int c, int n) {
+    if constexpr (VEC) {
+      const u32x4* s = (const u32x4*)(p + (c < n ? c : 0));
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) q[i] = s[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = c + i < n ? to_f32(p[c + i]) : 0.f;
+    }
+  }
+  __device__ __forceinline__ void get(float* v, int c, int n) const {
+    if constexpr (VEC) {
+      const bool in = c < n;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float t;
+        if constexpr (sizeof(T) == 2) t = __uint_as_float(i & 1 ? q[0][i / 2] & 0xffff0000u : q[0][i / 2] << 16);
+        else t = __uint_as_float(q[i / 4][i % 4]);
+        v[i] = in ? t : 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = f[i];
+    }
+  }
+};
+
+// weight and bias of a norm for this lane's channels: 1 and 0 where there is no vector, 0 past the row (so that what a
+// norm leaves there is 0)
 template <int NCH, int WPR>
-__device__ __forceinline__ void row_norm(float (&x)[NCH][8], int kind, const float* __restrict__ w, const float* __restrict__ b,
-                                         float eps, int C, int cw, float* red, int wv) {
+struct NormVec {
+  float w[NCH][8], b[NCH][8];
+  __device__ __forceinline__ void load(const float* __restrict__ pw, const float* __restrict__ pb, int cw, int C) {
+#pragma unroll
+    for (int k = 0; k < NCH; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = cw + k * (512 * WPR) + i, cc = c < C ? c : C - 1;
+        w[k][i] = c < C ? (pw ? pw[cc] : 1.f) : 0.f;
+        b[k][i] = c < C && pb ? pb[cc] : 0.f;
+      }
+  }
+};
+
+// x <- norm(x) over the row's C channels; lanes past the row hold zeros before and after.
+template <int NCH, int WPR, bool VEC>
+__device__ __forceinline__ void row_norm(float (&x)[NCH][8], int kind, const NormVec<NCH, WPR>& p, float eps, int C, float inv_c, int cw,
+                                         float* red, int wv) {
   if (kind == NORM_NONE) return;
-  const float inv_c = 1.0f / (float)C;
   float mean = 0.f, mul = 1.f;
   if (kind == NORM_LAYER) {
     float t = 0.f;
@@ -64,41 +114,40 @@ __device__ __forceinline__ void row_norm(float (&x)[NCH][8], int kind, const flo
   if (kind != NORM_AFFINE) {
     float t = 0.f;
 #pragma unroll
-    for (int k = 0; k < NCH; ++k)
+    for (int k = 0; k < NCH; ++k) {
+      const int c = cw + k * (512 * WPR);
+      float tk = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float d = cw + k * (512 * WPR) + i < C ? x[k][i] - mean : 0.f;
-        t = fmaf(d, d, t);
+        const float d = VEC || c + i < C ? x[k][i] - mean : 0.f;
+        tk = fmaf(d, d, tk);
       }
+      t += c < C ? tk : 0.f;
+    }
     mul = 1.0f / sqrtf(fmaf(row_total<WPR>(t, red, wv), inv_c, eps));
   }
 #pragma unroll
-  for (int k = 0; k < NCH; ++k) {
-    const int c = cw + k * (512 * WPR);
+  for (int k = 0; k < NCH; ++k)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (c + i >= C) continue;
-      float t = (x[k][i] - mean) * mul;
-      if (w) t *= w[c + i];
-      if (b) t += b[c + i];
-      x[k][i] = t;
-    }
-  }
+    for (int i = 0; i < 8; ++i) x[k][i] = fmaf((x[k][i] - mean) * mul, p.w[k][i], p.b[k][i]);
 }
 
-template <typename TU, typename TS, int NCH, int WPR>
-__global__ __launch_bounds__(256) void block_join_kernel(JoinArgs a) {
-  __shared__ float red[4];
+// NCH x 8 channels a lane, WPR waves a row.  Each wave (WPR = 1; else each workgroup) takes a run of consecutive rows.
+template <typename TU, typename TS, int NCH, int WPR, bool VEC>
+__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void block_join_kernel(JoinArgs a) {
+  __shared__ float red[WPR > 1 ? WPR : 1];
   const SugarBlockJoin& j = a.j;
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const int C = j.cols;
   const int cw = (WPR > 1 ? wv * 512 : 0) + lane * 8;          // first channel of this lane's chunk 0
-  constexpr int RPB = 4 / WPR;                                 // rows a workgroup holds
+  const float inv_c = 1.0f / (float)C;
+  constexpr int RPB = WPR > 1 ? 1 : 4;                         // rows a workgroup holds
   const int64_t per = (j.rows + (int64_t)gridDim.x * RPB - 1) / ((int64_t)gridDim.x * RPB);
-  const int64_t first = ((int64_t)blockIdx.x * RPB + (WPR > 1 ? 0 : wv)) * per;
+  const int64_t first = ((int64_t)blockIdx.x * RPB + (WPR > 1 ? 0 : __builtin_amdgcn_readfirstlane(wv))) * per;
   const int64_t last = first + per < j.rows ? first + per : j.rows;
-  int b = 0, b_end = 0;
-  if (j.d_row_off && first < last) {                           // last utterance that begins at or before the first row
+  if (first >= last) return;
+  int b = 0, b_end = 0, begin = 0;
+  if (j.d_row_off) {                                           // last utterance that begins at or before the first row
     int lo = 0, hi = j.n_utts;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -106,29 +155,46 @@ __global__ __launch_bounds__(256) void block_join_kernel(JoinArgs a) {
     }
     b = lo;
     b_end = j.d_row_off[b + 1];
+    begin = j.d_row_off[0];
   }
+  NormVec<NCH, WPR> post, pre;                                 // in registers over the rows
+  if (j.post_kind) post.load(j.d_post_w, j.d_post_b, cw, C);
+  if (j.pre_kind) pre.load(j.d_pre_w, j.d_pre_b, cw, C);
   for (int64_t r = first; r < last; ++r) {
     if (j.d_row_off) {
       while (r >= b_end && b + 1 < j.n_utts) { ++b; b_end = j.d_row_off[b + 1]; }
-      if (r >= b_end || r < j.d_row_off[0]) continue;           // a row of no utterance: left as it is
+      if (r >= b_end || r < begin) continue;                   // a row of no utterance: left as it is
+    }
+    Raw8<TU, VEC> ru[NCH], rgu[NCH];
+    Raw8<TS, VEC> rs[NCH];
+    Raw8<float, VEC> rg[NCH];
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) ru[k].load((const TU*)j.d_u + r * j.ldu, cw + k * (512 * WPR), C);
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) rs[k].load((const TS*)j.d_residual + r * j.ldr, cw + k * (512 * WPR), C);
+    if (j.gate_kind == SUGAR_GATE_ROW) {
+#pragma unroll
+      for (int k = 0; k < NCH; ++k) rgu[k].load((const TU*)j.d_gate + r * j.ldg, cw + k * (512 * WPR), C);
+    } else if (j.gate_kind) {
+#pragma unroll
+      for (int k = 0; k < NCH; ++k)
+        rg[k].load((const float*)j.d_gate + (j.gate_kind == SUGAR_GATE_UTTERANCE ? b * j.ldg : 0), cw + k * (512 * WPR), C);
     }
     float v[NCH][8], s[NCH][8];
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) load8((const TU*)j.d_u + r * j.ldu, cw + k * (512 * WPR), C, a.vec_u, v[k]);
-#pragma unroll
-    for (int k = 0; k < NCH; ++k) load8((const TS*)j.d_residual + r * j.ldr, cw + k * (512 * WPR), C, a.vec_r, s[k]);
-    row_norm<NCH, WPR>(v, j.post_kind, j.d_post_w, j.d_post_b, j.post_eps, C, cw, red, wv);
+    for (int k = 0; k < NCH; ++k) ru[k].get(v[k], cw + k * (512 * WPR), C);
+    row_norm<NCH, WPR, VEC>(v, j.post_kind, post, j.post_eps, C, inv_c, cw, red, wv);
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       const int c = cw + k * (512 * WPR);
       float g[8];
-      if (j.gate_kind == SUGAR_GATE_ROW) load8((const TU*)j.d_gate + r * j.ldg, c, C, a.vec_g, g);
-      else if (j.gate_kind == SUGAR_GATE_UTTERANCE) load8((const float*)j.d_gate + b * j.ldg, c, C, a.vec_g, g);
-      else if (j.gate_kind == SUGAR_GATE_CHANNEL) load8((const float*)j.d_gate, c, C, a.vec_g, g);
+      if (j.gate_kind == SUGAR_GATE_ROW) rgu[k].get(g, c, C);
+      else if (j.gate_kind) rg[k].get(g, c, C);
       else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) g[i] = 1.f;
       }
+      rs[k].get(s[k], c, C);
       float st[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -136,25 +202,21 @@ __global__ __launch_bounds__(256) void block_join_kernel(JoinArgs a) {
         s[k][i] = fmaf(j.alpha * g[i], v[k][i], res);
         st[i] = j.dense ? res + s[k][i] : s[k][i];
       }
-      if (j.d_stream) store8((TS*)j.d_stream + r * j.lds, c, C, a.vec_s, st);
+      if (j.d_stream) store8((TS*)j.d_stream + r * j.lds, c, C, VEC, st);
     }
     if (!j.d_z && !j.d_q) continue;
-    row_norm<NCH, WPR>(s, j.pre_kind, j.d_pre_w, j.d_pre_b, j.pre_eps, C, cw, red, wv);
+    row_norm<NCH, WPR, VEC>(s, j.pre_kind, pre, j.pre_eps, C, inv_c, cw, red, wv);
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       const int c = cw + k * (512 * WPR);
       if (j.d_z) {
-        if (j.z_dtype == SUGAR_F32) store8((float*)j.d_z + r * j.ldz, c, C, a.vec_z, s[k]);
-        else store8((bf16*)j.d_z + r * j.ldz, c, C, a.vec_z, s[k]);
+        if (j.z_dtype == SUGAR_F32) store8((float*)j.d_z + r * j.ldz, c, C, VEC, s[k]);
+        else store8((bf16*)j.d_z + r * j.ldz, c, C, VEC, s[k]);
       }
-      if (j.d_q) {
+      if (j.d_q) {                                             // (past the row s is 0: the operand's padding columns)
         unsigned big = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (c + i >= C) s[k][i] = 0.f;                        // padding columns of the operand
-          const unsigned u = fp8_finite_bits(s[k][i]);
-          big = u > big ? u : big;
-        }
+        for (int i = 0; i < 8; ++i) { const unsigned u = fp8_finite_bits(s[k][i]); big = u > big ? u : big; }
         const int byte = fp8_exponent(row16_max(big)), kb = c / FP8_BLOCK, blocks = (C + FP8_BLOCK - 1) / FP8_BLOCK;
         if (kb < blocks) {
           *(u32x2*)(j.d_q + r * j.ldq + c) = fp8_pack8(s[k], fp8_inverse(byte));
@@ -168,23 +230,25 @@ __global__ __launch_bounds__(256) void block_join_kernel(JoinArgs a) {
 }
 
 template <typename TU, typename TS, int NCH, int WPR>
-int launch_join(const JoinArgs& a, hipStream_t s) {
-  int n_cu = 0;
-  if (int rc = device_cu_count(&n_cu)) return rc;
-  const int64_t want = ceil_div(a.j.rows, 4 / WPR);
-  const unsigned grid = (unsigned)(want < 8ll * n_cu ? want : 8ll * n_cu);
-  hipLaunchKernelGGL((block_join_kernel<TU, TS, NCH, WPR>), dim3(grid), dim3(256), 0, s, a);
+int launch_join(const JoinArgs& a, bool vec, int n_cu, hipStream_t s) {
+  constexpr int threads = WPR > 4 ? 64 * WPR : 256;
+  const int64_t want = ceil_div(a.j.rows, WPR > 1 ? 1 : 4), most = 2048ll / threads * n_cu;
+  const unsigned grid = (unsigned)(want < most ? want : most);
+  if (vec) hipLaunchKernelGGL((block_join_kernel<TU, TS, NCH, WPR, true>), dim3(grid), dim3(threads), 0, s, a);
+  else hipLaunchKernelGGL((block_join_kernel<TU, TS, NCH, WPR, false>), dim3(grid), dim3(threads), 0, s, a);
   SUGAR_LAUNCH_CHECK();
   return SUGAR_OK;
 }
 
 template <typename TU, typename TS>
-int launch_join_t(const JoinArgs& a, hipStream_t s) {
+int launch_join_t(const JoinArgs& a, bool vec, hipStream_t s) {
+  int n_cu = 0;
+  if (int rc = device_cu_count(&n_cu)) return rc;
   const int C = a.j.cols;
-  if (C <= 512) return launch_join<TU, TS, 1, 1>(a, s);
-  if (C <= 2048) return launch_join<TU, TS, 1, 4>(a, s);
-  if (C <= 4096) return launch_join<TU, TS, 2, 4>(a, s);
-  return launch_join<TU, TS, 4, 4>(a, s);
+  if (C <= 512) return launch_join<TU, TS, 1, 1>(a, vec, n_cu, s);
+  if (C <= 1024 && a.j.rows >= 16ll * n_cu) return launch_join<TU, TS, 2, 1>(a, vec, n_cu, s);
+  if (C <= 2048) return launch_join<TU, TS, 1, 4>(a, vec, n_cu, s);
+  return launch_join<TU, TS, 1, 16>(a, vec, n_cu, s);
 }
 
 bool norm_ok(int kind) { return kind == NORM_NONE || kind == NORM_AFFINE || kind == NORM_RMS || kind == NORM_LAYER; }
@@ -195,13 +259,13 @@ int launch_block_join(const SugarBlockJoin& j, hipStream_t s) {
   JoinArgs a;
   a.j = j;
   const int eu = j.u_dtype == SUGAR_F32 ? 4 : 2, es = j.stream_dtype == SUGAR_F32 ? 4 : 2, ez = j.z_dtype == SUGAR_F32 ? 4 : 2;
-  a.vec_u = rows_vec(j.d_u, j.ldu, j.cols, eu);
-  a.vec_r = rows_vec(j.d_residual, j.ldr, j.cols, es);
-  a.vec_s = rows_vec(j.d_stream, j.lds, j.cols, es);
-  a.vec_z = rows_vec(j.d_z, j.ldz, j.cols, ez);
-  a.vec_g = rows_vec(j.d_gate, j.gate_kind == SUGAR_GATE_CHANNEL ? j.cols : j.ldg, j.cols, j.gate_kind == SUGAR_GATE_ROW ? eu : 4);
-  if (j.u_dtype == SUGAR_F32) return launch_join_t<float, float>(a, s);
-  return j.stream_dtype == SUGAR_F32 ? launch_join_t<bf16, float>(a, s) : launch_join_t<bf16, bf16>(a, s);
+  const int eg = j.gate_kind == SUGAR_GATE_ROW ? eu : 4;
+  // one path for rows that are all 16-byte aligned in whole chunks of 8 channels, one for everything else
+  const bool vec = rows_vec(j.d_u, j.ldu, j.cols, eu) && rows_vec(j.d_residual, j.ldr, j.cols, es) &&
+                   (!j.d_stream || rows_vec(j.d_stream, j.lds, j.cols, es)) && (!j.d_z || rows_vec(j.d_z, j.ldz, j.cols, ez)) &&
+                   (!j.d_gate || rows_vec(j.d_gate, j.gate_kind == SUGAR_GATE_CHANNEL ? j.cols : j.ldg, j.cols, eg));
+  if (j.u_dtype == SUGAR_F32) return launch_join_t<float, float>(a, vec, s);
+  return j.stream_dtype == SUGAR_F32 ? launch_join_t<bf16, float>(a, vec, s) : launch_join_t<bf16, bf16>(a, vec, s);
 }
 
 }  // namespace sugar
