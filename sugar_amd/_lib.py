@@ -77,7 +77,7 @@ SYMBOLS = {
     "sugar_fp8_quant": (_i, [_vp, _i64, _i, _i64, _i, _vp, _i64, _vp, _i64, _vp]),
     "sugar_fp8_dequant": (_i, [_vp, _i64, _vp, _i64, _i64, _i, _vp, _i64, _i, _vp]),
     "sugar_fp8_linear": (_i, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i, _i, _vp, _vp, _i, _vp, _i64, _i, _vp]),
-    "sugar_block_join": (_i, [C.POINTER(SugarBlockJoin), _vp]),
+    "sugar_block_join": (_i, [_vp, _vp]),          # SugarBlockJoin*, or the bytes of one
     "sugar_tdnn_recalibrate": (_i, [_vp, _vp, _vp, _i, _i64, _i, _vp, _i64, C.c_float, _vp, _vp]),
     "sugar_embed_recalibrate": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i64, _i, _vp, _i64, C.c_float, _vp, _vp]),
     "sugar_subnet_bn_count": (_i, [_vp]),

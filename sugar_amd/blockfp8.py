@@ -13,7 +13,7 @@ device, allocate only their outputs (none when they are passed in) and never syn
 graph; there is no backward pass: tensors that require a gradient are refused while gradients are recorded.
 """
 import collections
-import ctypes as C
+import struct
 
 import torch
 
@@ -22,77 +22,84 @@ from . import _lib
 _DT = {torch.float32: _lib.SUGAR_F32, torch.bfloat16: _lib.SUGAR_BF16}
 NORMS = {None: 0, "affine": 1, "rms": 2, "layer": 3}
 MAX_JOIN_COLS = 8192
+_raw_stream = torch._C._cuda_getCurrentRawStream       # (torch.cuda.current_stream builds an object, 1 us of a 10 us call)
+_FN = {}
 
 
 def _up(v, m):
     return (v + m - 1) // m * m
 
 
-def _need_cuda(*tensors):
+def _same_device(tensors):
+    """The device all of them are on (a GPU), none of them part of a recorded gradient."""
     dev = tensors[0].device
+    grad = torch.is_grad_enabled()
     for t in tensors:
         if not t.is_cuda:
             raise _lib.SugarError("sugar_amd runs on an MI355X only: tensors must be CUDA tensors (no CPU fallback)")
         if t.device != dev:
             raise ValueError("tensors on %s and %s" % (dev, t.device))
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise ValueError("no backward pass: call under torch.no_grad() or detach the inputs")
+        if grad and t.requires_grad:
+            raise ValueError("no backward pass: call under torch.no_grad() or detach the inputs")
     return dev
 
 
 def _call(dev, name, *args):
     """One library call on the current stream of `dev`, with that device current."""
-    fn = getattr(_lib.lib(), name)
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, stream)
+    fn = _FN.get(name)
+    if fn is None:
+        fn = _FN[name] = getattr(_lib.lib(), name)
+    idx = dev.index
+    if torch.cuda.current_device() == idx:
+        rc = fn(*args, _raw_stream(idx))
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, stream)
+        with torch.cuda.device(idx):
+            rc = fn(*args, _raw_stream(idx))
     if rc < 0:
         _lib.check(rc, name)
 
 
-def _rows(what, x, dtypes=_DT):
-    """x as a matrix whose columns lie next to each other (a copy when they do not)."""
-    if x.dim() != 2:
+def _rows(what, x):
+    """x as a matrix whose columns lie next to each other (a copy when they do not), and its row stride."""
+    if x.dim() != 2 or x.shape[1] == 0:
         raise ValueError("%s: expected [rows, columns], got %s" % (what, tuple(x.shape)))
-    if x.dtype not in dtypes:
-        raise ValueError("%s: dtype %s not in %s" % (what, x.dtype, [str(d) for d in dtypes]))
-    if x.shape[1] == 0:
-        raise ValueError("%s: no columns" % what)
-    return x if _plain(x) else x.contiguous()
+    if x.dtype not in _DT:
+        raise ValueError("%s: dtype %s not in %s" % (what, x.dtype, [str(d) for d in _DT]))
+    ld = _row_stride(x)
+    if ld is None:
+        x = x.contiguous()
+        ld = x.shape[1]
+    return x, ld
 
 
-def _plain(x):
-    return (x.stride(1) == 1 or x.shape[1] == 1) and (x.stride(0) >= x.shape[1] or x.shape[0] <= 1)
-
-
-def _ld(x):
-    """Row stride (a single row has none of its own: torch leaves any number there)."""
-    return x.stride(0) if x.shape[0] > 1 else max(x.shape[1], x.stride(0))
+def _row_stride(x):
+    """Elements from row to row of a matrix with adjacent columns, None for any other (a single row has no stride of its own:
+    torch leaves any number there)."""
+    r, c = x.shape
+    ld, step = x.stride()
+    if step != 1 and c != 1:
+        return None
+    if r <= 1:
+        return max(c, ld)
+    return ld if ld >= c else None
 
 
 def _out(what, out, shape, dtypes, dev):
+    """Row stride of a tensor to write into."""
     if tuple(out.shape) != tuple(shape) or out.dtype not in dtypes or out.device != dev:
         raise ValueError("%s: expected %s %s on %s, got %s %s on %s" % (what, tuple(shape), "/".join(str(d) for d in dtypes), dev,
                                                                         tuple(out.shape), out.dtype, out.device))
-    if not _plain(out):
-        raise ValueError("%s: the columns of an output must be contiguous" % what)
-    return out
+    ld = _row_stride(out)
+    if ld is None:
+        raise ValueError("%s: the columns of an output must be contiguous, its rows apart" % what)
+    return ld
 
 
-def _vector(what, v, n, dev):
-    """A float32 vector of n on the device (other float types and strides are converted)."""
-    if v is None:
-        return None
+def _vector(what, v, n):
+    """A contiguous float32 vector of n (other float types and strides are converted)."""
     if v.dim() != 1 or v.shape[0] != n or not v.dtype.is_floating_point:
         raise ValueError("%s: expected a floating vector of %d, got %s %s" % (what, n, v.dtype, tuple(v.shape)))
     return v if v.dtype == torch.float32 and v.is_contiguous() else v.to(torch.float32).contiguous()
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
 
 
 class BlockFP8(object):
@@ -103,7 +110,7 @@ class BlockFP8(object):
     Row slices (`x[10:20]`) share the memory.  `BlockFP8(data, exponent, cols)` takes existing tensors as they are.
     """
     BLOCK = 128
-    __slots__ = ("data", "exponent", "cols")
+    __slots__ = ("_data", "_exponent", "cols", "_ld", "_lde")
 
     def __init__(self, data, exponent, cols):
         cols = int(cols)
@@ -116,48 +123,61 @@ class BlockFP8(object):
                              % (cols, blocks * self.BLOCK, _up(blocks, 4), tuple(data.shape), tuple(exponent.shape)))
         if data.device != exponent.device:
             raise ValueError("BlockFP8: data on %s, exponent on %s" % (data.device, exponent.device))
-        if not (_plain(data) and _plain(exponent)) or _ld(data) % 16 or _ld(exponent) % 4 or data.data_ptr() % 16 or exponent.data_ptr() % 4:
+        if data.requires_grad:
+            raise ValueError("BlockFP8: no backward pass: detach the data")
+        ld, lde = _row_stride(data), _row_stride(exponent)
+        if ld is None or lde is None or ld % 16 or lde % 4 or data.data_ptr() % 16 or exponent.data_ptr() % 4:
             raise ValueError("BlockFP8: contiguous columns, data rows 16-byte aligned, exponent rows 4-byte aligned")
-        self.data, self.exponent, self.cols = data, exponent, cols
+        self._data, self._exponent, self.cols, self._ld, self._lde = data, exponent, cols, ld, lde
 
     @classmethod
     def empty(cls, rows, cols, device):
-        blocks = -(-int(cols) // cls.BLOCK)
         self = cls.__new__(cls)
-        self.data = torch.empty((rows, blocks * cls.BLOCK), dtype=torch.float8_e4m3fn, device=device)
-        self.exponent = torch.empty((rows, _up(blocks, 4)), dtype=torch.uint8, device=device)
-        self.cols = int(cols)
+        blocks = -(-int(cols) // cls.BLOCK)
+        self.cols, self._ld, self._lde = int(cols), blocks * cls.BLOCK, _up(blocks, 4)
+        self._data = torch.empty((rows, self._ld), dtype=torch.float8_e4m3fn, device=device)
+        self._exponent = torch.empty((rows, self._lde), dtype=torch.uint8, device=device)
         return self
 
     @property
+    def data(self):
+        return self._data
+
+    @property
+    def exponent(self):
+        return self._exponent
+
+    @property
     def rows(self):
-        return self.data.shape[0]
+        return self._data.shape[0]
 
     @property
     def shape(self):
-        return torch.Size((self.data.shape[0], self.cols))
+        return torch.Size((self._data.shape[0], self.cols))
 
     @property
     def device(self):
-        return self.data.device
+        return self._data.device
 
     def __getitem__(self, rows):
         if not isinstance(rows, slice) or rows.step not in (None, 1):
             raise ValueError("BlockFP8: only slices of consecutive rows")
-        return BlockFP8(self.data[rows], self.exponent[rows], self.cols)
+        return BlockFP8(self._data[rows], self._exponent[rows], self.cols)
 
     def dequantize(self, dtype=torch.float32, out=None):
         """The values, [rows, cols] float32 or bfloat16 (exact in both)."""
-        dev = _need_cuda(self.data, self.exponent)
+        data, exponent, cols = self._data, self._exponent, self.cols
+        dev = _same_device((data, exponent))
+        rows = data.shape[0]
         if out is None:
             if dtype not in _DT:
                 raise ValueError("dequantize: dtype %s not in %s" % (dtype, [str(d) for d in _DT]))
-            out = torch.empty((self.data.shape[0], self.cols), dtype=dtype, device=dev)
+            out, ld = torch.empty((rows, cols), dtype=dtype, device=dev), cols
         else:
-            _out("dequantize", out, self.shape, _DT, dev)
-        if out.shape[0]:
-            _call(dev, "sugar_fp8_dequant", self.data.data_ptr(), _ld(self.data), self.exponent.data_ptr(), _ld(self.exponent),
-                  out.shape[0], self.cols, out.data_ptr(), _ld(out), _DT[out.dtype])
+            ld = _out("dequantize", out, (rows, cols), _DT, dev)
+        if rows:
+            _call(dev, "sugar_fp8_dequant", data.data_ptr(), self._ld, exponent.data_ptr(), self._lde, rows, cols,
+                  out.data_ptr(), ld, _DT[out.dtype])
         return out
 
 
@@ -175,12 +195,13 @@ def quantize_block_fp8(x, out=None):
     keeps its largest finite magnitude within 448; values go to the nearest e4m3, ties to the even one.  Infinities and NaN
     become NaN and do not move the scale of their block.
     """
-    x = _rows("quantize_block_fp8", x)
-    dev = _need_cuda(x)
-    q = _fp8_out("quantize_block_fp8", out, x.shape[0], x.shape[1], dev)
-    if x.shape[0]:
-        _call(dev, "sugar_fp8_quant", x.data_ptr(), _ld(x), _DT[x.dtype], x.shape[0], x.shape[1], q.data.data_ptr(),
-              _ld(q.data), q.exponent.data_ptr(), _ld(q.exponent))
+    x, ld = _rows("quantize_block_fp8", x)
+    dev = _same_device((x,))
+    rows, cols = x.shape
+    q = _fp8_out("quantize_block_fp8", out, rows, cols, dev)
+    if rows:
+        _call(dev, "sugar_fp8_quant", x.data_ptr(), ld, _DT[x.dtype], rows, cols, q._data.data_ptr(), q._ld,
+              q._exponent.data_ptr(), q._lde)
     return q
 
 
@@ -188,33 +209,34 @@ def block_fp8_linear(a, w, scale=None, shift=None, relu=False, out_dtype=torch.b
     """
     relu(a @ w.T) * scale + shift for BlockFP8 a [rows, k] and w [n, k], rounded once to `out_dtype` (bfloat16 or float32).
     float32 outputs are float32 sums of exact products; bfloat16 outputs run twice as fast on the 8-bit matrix
-    instruction, whose sums are good to about 1.5e-5 (include/sugar_amd.h).  The order is that of the reference's layers, conv -> ReLU -> BatchNorm
-    (sugar/models/dynamictdnn.py:183); scale, shift: float vectors [n], either may be missing.
+    instruction, whose sums are good to about 1.5e-5 (include/sugar_amd.h).  The order is that of the reference's layers,
+    conv -> ReLU -> BatchNorm (sugar/models/dynamictdnn.py:183); scale, shift: float vectors [n], either may be missing.
     """
     if not isinstance(a, BlockFP8) or not isinstance(w, BlockFP8):
         raise ValueError("block_fp8_linear: operands must be BlockFP8 (quantize_block_fp8)")
-    rows, n, k = a.data.shape[0], w.data.shape[0], a.cols
+    rows, n, k = a._data.shape[0], w._data.shape[0], a.cols
     if k != w.cols:
         raise ValueError("block_fp8_linear: a has %d columns, w %d" % (k, w.cols))
     if n == 0:
         raise ValueError("block_fp8_linear: w has no rows")
-    dev = _need_cuda(a.data, a.exponent, w.data, w.exponent, *[v for v in (scale, shift) if v is not None])
-    scale, shift = _vector("scale", scale, n, dev), _vector("shift", shift, n, dev)
     flags = _lib.EPI_RELU if relu else 0
-    if scale is not None or shift is not None:
+    if scale is None and shift is None:
+        dev = _same_device((a._data, w._data))
+    else:
+        dev = _same_device([t for t in (a._data, w._data, scale, shift) if t is not None])
+        scale = torch.ones(n, device=dev) if scale is None else _vector("scale", scale, n)
+        shift = torch.zeros(n, device=dev) if shift is None else _vector("shift", shift, n)
         flags |= _lib.EPI_AFFINE
-        scale = torch.ones(n, device=dev) if scale is None else scale
-        shift = torch.zeros(n, device=dev) if shift is None else shift
     if out is None:
         if out_dtype not in _DT:
             raise ValueError("block_fp8_linear: out_dtype %s not in %s" % (out_dtype, [str(d) for d in _DT]))
-        out = torch.empty((rows, n), dtype=out_dtype, device=dev)
+        out, ld = torch.empty((rows, n), dtype=out_dtype, device=dev), n
     else:
-        _out("block_fp8_linear", out, (rows, n), _DT, dev)
+        ld = _out("block_fp8_linear", out, (rows, n), _DT, dev)
     if rows:
-        _call(dev, "sugar_fp8_linear", a.data.data_ptr(), _ld(a.data), a.exponent.data_ptr(), _ld(a.exponent), rows,
-              w.data.data_ptr(), _ld(w.data), w.exponent.data_ptr(), _ld(w.exponent), n, k, _ptr(scale), _ptr(shift), flags,
-              out.data_ptr(), _ld(out), _DT[out.dtype])
+        _call(dev, "sugar_fp8_linear", a._data.data_ptr(), a._ld, a._exponent.data_ptr(), a._lde, rows, w._data.data_ptr(), w._ld,
+              w._exponent.data_ptr(), w._lde, n, k, scale.data_ptr() if flags & _lib.EPI_AFFINE else None,
+              shift.data_ptr() if flags & _lib.EPI_AFFINE else None, flags, out.data_ptr(), ld, _DT[out.dtype])
     return out
 
 
@@ -241,8 +263,8 @@ def block_join(u, residual, post=None, gate=None, row_off=None, alpha=1.0, dense
     Outputs may be passed in; stream_out may be `residual` or `u` itself, normed_out `u` (in place).  With row_off, rows in
     front of the first and behind the last utterance are left as they are (in outputs allocated here: undefined).
     """
-    u = _rows("block_join: u", u)
-    residual = _rows("block_join: residual", residual)
+    u, ldu = _rows("block_join: u", u)
+    residual, ldr = _rows("block_join: residual", residual)
     rows, cols = u.shape
     if residual.shape != u.shape:
         raise ValueError("block_join: u %s, residual %s" % (tuple(u.shape), tuple(residual.shape)))
@@ -250,58 +272,69 @@ def block_join(u, residual, post=None, gate=None, row_off=None, alpha=1.0, dense
         raise ValueError("block_join: %d columns, at most %d" % (cols, MAX_JOIN_COLS))
     if u.dtype == torch.float32 and residual.dtype != torch.float32:
         raise ValueError("block_join: a float32 u needs a float32 residual")
-    vecs = [t for p in (post, pre) if p is not None for t in (p.weight, p.bias) if t is not None]
-    dev = _need_cuda(u, residual, *vecs, *[t for t in (gate, row_off) if t is not None])
-    d = _lib.SugarBlockJoin()
-    keep = []
-    for side, p in (("post", post), ("pre", pre)):
-        if p is None:
-            continue
-        if p.kind not in NORMS or p.kind is None or not p.eps >= 0:
-            raise ValueError("block_join: %s kind %r not in %s, or eps %r negative" % (side, p.kind, [k for k in NORMS if k], p.eps))
-        wt, bs = _vector(side + " weight", p.weight, cols, dev), _vector(side + " bias", p.bias, cols, dev)
-        keep += [wt, bs]
-        setattr(d, side + "_kind", NORMS[p.kind])
-        setattr(d, side + "_eps", p.eps)
-        setattr(d, "d_%s_w" % side, _ptr(wt))
-        setattr(d, "d_%s_b" % side, _ptr(bs))
+    inputs = [u, residual]
+    for p in (post, pre):
+        if p is not None:
+            inputs += [t for t in (p.weight, p.bias) if t is not None]
+    inputs += [t for t in (gate, row_off) if t is not None]
+    dev = _same_device(inputs)
+    (post_kind, post_eps, post_w, post_b), (pre_kind, pre_eps, pre_w, pre_b) = _norm("post", post, cols), _norm("pre", pre, cols)
+    utts = 0
     if row_off is not None:
         if row_off.dim() != 1 or row_off.shape[0] < 2 or row_off.dtype != torch.int32:
             raise ValueError("block_join: row_off must be int32 [B + 1], got %s %s" % (row_off.dtype, tuple(row_off.shape)))
         row_off = row_off.contiguous()
-        d.d_row_off, d.n_utts = row_off.data_ptr(), row_off.shape[0] - 1
+        utts = row_off.shape[0] - 1
+    gate_kind = ldg = 0
     if gate is not None:
         if gate.dim() == 1:
-            gate = _vector("gate", gate, cols, dev)
-            d.gate_kind, d.ldg = 1, cols
-        elif row_off is not None and tuple(gate.shape) == (d.n_utts, cols):
-            gate = _rows("block_join: gate", gate if gate.dtype == torch.float32 else gate.float())
-            d.gate_kind, d.ldg = 2, _ld(gate)
+            gate, gate_kind, ldg = _vector("gate", gate, cols), 1, cols
+        elif row_off is not None and tuple(gate.shape) == (utts, cols):
+            gate, ldg = _rows("block_join: gate", gate if gate.dtype == torch.float32 else gate.float())
+            gate_kind = 2
         elif row_off is None and gate.shape == u.shape and gate.dtype == u.dtype:
-            gate = _rows("block_join: gate", gate)
-            d.gate_kind, d.ldg = 3, _ld(gate)
+            gate, ldg = _rows("block_join: gate", gate)
+            gate_kind = 3
         else:
             raise ValueError("block_join: gate %s %s is neither [C], [B, C] with row_off, nor [rows, C] of u's dtype without it"
                              % (gate.dtype, tuple(gate.shape)))
-        d.d_gate = gate.data_ptr()
-    d.rows, d.cols, d.alpha, d.dense = rows, cols, alpha, int(bool(dense))
-    d.u_dtype, d.stream_dtype = _DT[u.dtype], _DT[residual.dtype]
-    stream = torch.empty((rows, cols), dtype=residual.dtype, device=dev) if stream_out is None else \
-        _out("block_join: stream_out", stream_out, (rows, cols), (residual.dtype,), dev)
-    d.d_u, d.ldu, d.d_residual, d.ldr = u.data_ptr(), _ld(u), residual.data_ptr(), _ld(residual)
-    d.d_stream, d.lds = stream.data_ptr(), _ld(stream)
+    if stream_out is None:
+        stream, lds = torch.empty((rows, cols), dtype=residual.dtype, device=dev), cols
+    else:
+        stream, lds = stream_out, _out("block_join: stream_out", stream_out, (rows, cols), (residual.dtype,), dev)
     z = q = None
-    if normed or normed_out is not None:
+    ldz = z_dtype = 0
+    if normed_out is not None:
+        z, ldz = normed_out, _out("block_join: normed_out", normed_out, (rows, cols), _DT, dev)
+    elif normed:
         out_dtype = u.dtype if out_dtype is None else out_dtype
         if out_dtype not in _DT:
             raise ValueError("block_join: out_dtype %s not in %s" % (out_dtype, [str(t) for t in _DT]))
-        z = torch.empty((rows, cols), dtype=out_dtype, device=dev) if normed_out is None else \
-            _out("block_join: normed_out", normed_out, (rows, cols), _DT, dev)
-        d.d_z, d.ldz, d.z_dtype = z.data_ptr(), _ld(z), _DT[z.dtype]
+        z, ldz = torch.empty((rows, cols), dtype=out_dtype, device=dev), cols
     if quantized or quantized_out is not None:
         q = _fp8_out("block_join: quantized_out", quantized_out, rows, cols, dev)
-        d.d_q, d.ldq, d.d_e, d.lde = q.data.data_ptr(), _ld(q.data), q.exponent.data_ptr(), _ld(q.exponent)
     if rows:
-        _call(dev, "sugar_block_join", C.byref(d))
-    del keep
+        p = torch.Tensor.data_ptr
+        _call(dev, "sugar_block_join", _JOIN.pack(
+            rows, cols, utts, _DT[u.dtype], _DT[residual.dtype], 0 if z is None else _DT[z.dtype], post_kind, pre_kind, gate_kind,
+            1 if dense else 0, alpha, post_eps, pre_eps, ldu, ldr, ldg, lds, ldz, 0 if q is None else q._ld, 0 if q is None else q._lde,
+            p(u), p(residual), 0 if post_w is None else p(post_w), 0 if post_b is None else p(post_b),
+            0 if pre_w is None else p(pre_w), 0 if pre_b is None else p(pre_b), 0 if gate is None else p(gate),
+            0 if row_off is None else p(row_off), p(stream), 0 if z is None else p(z),
+            0 if q is None else p(q._data), 0 if q is None else p(q._exponent)))
     return JoinResult(stream, z, q)
+
+
+# SugarBlockJoin of include/sugar_amd.h (_lib.SugarBlockJoin) as one packing: 30 attribute writes of a ctypes structure
+# cost 5 us a call
+_JOIN = struct.Struct("@q9i3f7q12P")
+
+
+def _norm(side, p, cols):
+    """(kind, eps, weight, bias) of a RowNorm or None; the vectors stay referenced until the call has been made."""
+    if p is None:
+        return 0, 0.0, None, None
+    if p.kind is None or p.kind not in NORMS or not p.eps >= 0:
+        raise ValueError("block_join: %s kind %r not in %s, or eps %r negative" % (side, p.kind, [k for k in NORMS if k], p.eps))
+    return (NORMS[p.kind], p.eps, None if p.weight is None else _vector(side + " weight", p.weight, cols),
+            None if p.bias is None else _vector(side + " bias", p.bias, cols))

@@ -127,29 +127,26 @@ __device__ __forceinline__ f32x4 mfma_fp8(i32x8 a, i32x8 b, f32x4 c, int ea, int
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, OPA, ea, OPB, eb);
 }
 
-// float32 outputs: the same block as four 16-bit products on the values converted to bf16 (every e4m3 value is one), whose
-// sums are good to f32 (4.6e-8 off on the same operands), at half the rate.  The block's sum is scaled afterwards.
+// float32 outputs: the same block as four 16-bit products on the values converted to bf16, block scale included (the
+// conversion instruction applies a power of two; an e4m3 value times one is a bf16 value down to the subnormals, byte 255
+// gives NaN), whose sums are good to f32 (4.6e-8 off on the same operands), at half the rate.  Conversions are one
+// instruction per two values and lie under the other wave's products.
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
-__device__ __forceinline__ void fp8_to_bf16(i32x8 q, bf16x8 (&h)[4]) {
+__device__ __forceinline__ void fp8_to_bf16(i32x8 q, int byte, bf16x8 (&h)[4]) {
+  const float sc = __uint_as_float((unsigned)(byte & 255) << 23);
 #pragma unroll
   for (int s = 0; s < 4; ++s)
 #pragma unroll
     for (int d = 0; d < 2; ++d) {
-      const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[2 * s + d], 1.0f, false);
-      const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[2 * s + d], 1.0f, true);
+      const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[2 * s + d], sc, false);
+      const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[2 * s + d], sc, true);
       h[s][4 * d] = lo[0]; h[s][4 * d + 1] = lo[1]; h[s][4 * d + 2] = hi[0]; h[s][4 * d + 3] = hi[1];
     }
 }
-__device__ __forceinline__ f32x4 mfma_wide(const bf16x8 (&a)[4], const bf16x8 (&b)[4]) {
-  f32x4 z = {0.f, 0.f, 0.f, 0.f};
+__device__ __forceinline__ f32x4 mfma_wide(const bf16x8 (&a)[4], const bf16x8 (&b)[4], f32x4 c) {
 #pragma unroll
-  for (int s = 0; s < 4; ++s) z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[s], b[s], z, 0, 0, 0);
-  return z;
-}
-// c + z 2^(ea + eb - 254), NaN when either byte is 255
-__device__ __forceinline__ float add_scaled(float c, float z, int ea, int eb) {
-  const float t = c + __builtin_amdgcn_ldexpf(z, ea + eb - 254);
-  return ea == 255 || eb == 255 ? __uint_as_float(0x7fc00000u) : t;
+  for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[s], b[s], c, 0, 0, 0);
+  return c;
 }
 
 struct Fp8Operand {        // [rows][ld] e4m3, [rows][lds] exponent bytes

@@ -96,15 +96,9 @@ __global__ __launch_bounds__(64 * NW) void fp8_linear_direct_kernel(LinearArgs p
     i32x8 wf;
     *(i32x4*)&wf = *(const i32x4*)(wp + kb * 128);
     *((i32x4*)&wf + 1) = *(const i32x4*)(wp + kb * 128 + 16);
+    const int ew = wep[kb];
     bf16x8 wh[4];
-    int ew[4];
-    if constexpr (WIDE) {
-      fp8_to_bf16(wf, wh);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ew[i] = p.we[(unsigned)min(co + 4 * fq + i, p.n - 1) * p.ldwe + kb];
-    } else {
-      ew[0] = wep[kb];
-    }
+    if constexpr (WIDE) fp8_to_bf16(wf, ew, wh);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int ar = min(r0 + t * 16 + fr, p.rows - 1);
@@ -115,12 +109,10 @@ __global__ __launch_bounds__(64 * NW) void fp8_linear_direct_kernel(LinearArgs p
       const int ea = p.ae[(unsigned)ar * p.ldae + kb];
       if constexpr (WIDE) {
         bf16x8 ah[4];
-        fp8_to_bf16(af, ah);
-        const f32x4 z = mfma_wide(wh, ah);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][i] = add_scaled(acc[t][i], z[i], ea, ew[i]);
+        fp8_to_bf16(af, ea, ah);
+        acc[t] = mfma_wide(wh, ah, acc[t]);
       } else {
-        acc[t] = mfma_fp8<0, 0>(wf, af, acc[t], ew[0], ea);
+        acc[t] = mfma_fp8<0, 0>(wf, af, acc[t], ew, ea);
       }
     }
   }
@@ -185,8 +177,7 @@ __device__ __forceinline__ void fp8_tile(const LinearArgs& p, const int co_base,
   for (int m = 0; m < MI; ++m)
 #pragma unroll
     for (int n = 0; n < NJ; ++n) acc[m][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  int ew[WIDE ? 4 * MI : MI], ex[NJ];
-  unsigned bad_w = 0, bad_x = 0;                                 // WIDE: bit per channel / row of this lane with a NaN exponent
+  int ew[MI], ex[NJ];
 
 #pragma unroll
   for (int t = 0; t < D; ++t)
@@ -204,37 +195,20 @@ __device__ __forceinline__ void fp8_tile(const LinearArgs& p, const int co_base,
     if ((kt & 3) == 0) {
       const unsigned* e = exps + ((kt >> 2) & 1) * (TM + TN);
 #pragma unroll
-      for (int m = 0; m < MI; ++m) {
-        if constexpr (WIDE) {
-          const i32x4 t = *(const i32x4*)(e + wm * CW + m * 16 + 4 * fq);    // the channels of this lane's results
-#pragma unroll
-          for (int i = 0; i < 4; ++i) ew[4 * m + i] = t[i];
-        } else {
-          ew[m] = e[wm * CW + m * 16 + fr];
-        }
-      }
+      for (int m = 0; m < MI; ++m) ew[m] = e[wm * CW + m * 16 + fr];
 #pragma unroll
       for (int n = 0; n < NJ; ++n) ex[n] = e[TM + wn * FW + n * 16 + fr];
     }
     if constexpr (WIDE) {
       bf16x8 xh[NJ][4];
 #pragma unroll
-      for (int n = 0; n < NJ; ++n) {
-        fp8_to_bf16(frag(xb, wn * FW + n * 16 + fr, fq), xh[n]);
-        bad_x |= (ex[n] & 255) == 255 ? 1u << n : 0u;
-      }
+      for (int n = 0; n < NJ; ++n) fp8_to_bf16(frag(xb, wn * FW + n * 16 + fr, fq), ex[n], xh[n]);
 #pragma unroll
       for (int m = 0; m < MI; ++m) {
         bf16x8 wh[4];
-        fp8_to_bf16(frag(wb, wm * CW + m * 16 + fr, fq), wh);
+        fp8_to_bf16(frag(wb, wm * CW + m * 16 + fr, fq), ew[m], wh);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) bad_w |= (ew[4 * m + i] & 255) == 255 ? 1u << (4 * m + i) : 0u;
-#pragma unroll
-        for (int n = 0; n < NJ; ++n) {
-          const f32x4 z = mfma_wide(wh, xh[n]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[m][n][i] += __builtin_amdgcn_ldexpf(z[i], (ew[4 * m + i] & 255) + (ex[n] & 255) - 254);
-        }
+        for (int n = 0; n < NJ; ++n) acc[m][n] = mfma_wide(wh, xh[n], acc[m][n]);
       }
     } else {
       i32x8 xf[NJ];
@@ -248,20 +222,11 @@ __device__ __forceinline__ void fp8_tile(const LinearArgs& p, const int co_base,
       }
     }
 #pragma unroll
-    for (int m = 0; m < (WIDE ? 4 * MI : MI); ++m) ew[m] = (int)((unsigned)ew[m] >> 8);
+    for (int m = 0; m < MI; ++m) ew[m] = (int)((unsigned)ew[m] >> 8);
 #pragma unroll
     for (int n = 0; n < NJ; ++n) ex[n] = (int)((unsigned)ex[n] >> 8);
     cur = cur + 1 == NS ? 0 : cur + 1;
     nxt = nxt + 1 == NS ? 0 : nxt + 1;
-  }
-  if constexpr (WIDE) {
-#pragma unroll
-    for (int m = 0; m < MI; ++m)
-#pragma unroll
-      for (int n = 0; n < NJ; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if ((bad_w >> (4 * m + i) | bad_x >> n) & 1) acc[m][n][i] = __uint_as_float(0x7fc00000u);
   }
 
   // ---- epilogue: accumulator tile (m, n): lane (fr, fq) holds row wn FW + n 16 + fr, channels wm CW + m 16 + 4 fq + 0..3
@@ -580,18 +545,33 @@ int launch_persist(LinearArgs p, int n_cu, hipStream_t s) {
 int launch_rows(const LinearArgs& p, hipStream_t s) {
   int n_cu = 0;
   if (int rc = device_cu_count(&n_cu)) return rc;
-  const int64_t t128 = ceil_div(p.n, 128) * ceil_div(p.rows, 128);
-  if (!p.out_f32 && p.vec && p.kb >= 2 && n_cu % 8 == 0 && ceil_div(p.n, 256) * ceil_div(p.rows, 256) >= n_cu)
+  // Measured, us (bf16 output unless said; direct | tile 64x64 | 64x128 | 128x128 | persist):
+  //   1 x 1536 -> 1536      3.5 | 5.7                      128 x 512 -> 512      3.2 | 3.8
+  //   256 x 1536 -> 192     4.1 | 5.8                      301 x 512 -> 512      4.1 | 3.8
+  //   301 x 1536 -> 1536    -   | 6.1 |  7.3 |  9.5        float32 output        -   | 9.0 | 11.0 | 16.5
+  //   1204 x 1536 -> 1536   -   | 7.9 |  7.7 | 10.0        float32 output        -   | 13.2 | 11.9 | 17.7
+  //   4816 x 1536 -> 1536   -   | 21.8 | 20.0 | 16.4       19264 x 528 -> 536    -   | 16.2 | 14.0 | 13.4
+  //   77056 x 512 -> 512    -   | 43  | 35   | 31.5 | 31.9   77056 x 768 -> 768      61.3 | 65.8 (the last two)
+  //   77056 x 1152 -> 1152  125.9 | 118.6                    77056 x 1536 -> 1536    231.9 | 180.8
+  // so: direct while its workgroups (each streams its 16 channels' weights once per 16 rows) are at most two a CU, the
+  // larger tile once it fills the CUs, the persistent kernel where k-loops are long enough to hide its epilogue and two
+  // rounds of tiles or more are there.
+  const bool f32 = p.out_f32;
+  if (ceil_div(p.n, 16) * ceil_div(p.rows, 16) <= 2ll * n_cu) {
+    constexpr int NT = 1, NW = 8;
+    const dim3 grid((unsigned)ceil_div(p.n, 16), (unsigned)ceil_div(p.rows, 16 * NT));
+    if (f32) hipLaunchKernelGGL((fp8_linear_direct_kernel<NT, NW, true>), grid, dim3(64 * NW), 0, s, p);
+    else hipLaunchKernelGGL((fp8_linear_direct_kernel<NT, NW, false>), grid, dim3(64 * NW), 0, s, p);
+    SUGAR_LAUNCH_CHECK();
+    return SUGAR_OK;
+  }
+  if (!f32 && p.vec && p.kb >= 8 && n_cu % 8 == 0 && ceil_div(p.n, 256) * ceil_div(p.rows, 256) >= 2 * n_cu)
     return launch_persist(p, n_cu, s);
-  if (t128 >= n_cu) return p.out_f32 ? launch_tile<128, 128, 2, true>(p, s) : launch_tile<128, 128, 2, false>(p, s);
-  if (p.rows > 64 && ceil_div(p.n, 64) * ceil_div(p.rows, 64) >= 64)
-    return p.out_f32 ? launch_tile<64, 64, 4, true>(p, s) : launch_tile<64, 64, 4, false>(p, s);
-  constexpr int NT = 2, NW = 4;
-  const dim3 grid((unsigned)ceil_div(p.n, 16), (unsigned)ceil_div(p.rows, 16 * NT));
-  if (p.out_f32) hipLaunchKernelGGL((fp8_linear_direct_kernel<NT, NW, true>), grid, dim3(64 * NW), 0, s, p);
-  else hipLaunchKernelGGL((fp8_linear_direct_kernel<NT, NW, false>), grid, dim3(64 * NW), 0, s, p);
-  SUGAR_LAUNCH_CHECK();
-  return SUGAR_OK;
+  if (ceil_div(p.n, 128) * ceil_div(p.rows, 128) >= n_cu)
+    return f32 ? launch_tile<128, 128, 2, true>(p, s) : launch_tile<128, 128, 2, false>(p, s);
+  if (4 * ceil_div(p.n, 64) * ceil_div(p.rows, 128) >= 3 * n_cu)
+    return f32 ? launch_tile<64, 128, 2, true>(p, s) : launch_tile<64, 128, 2, false>(p, s);
+  return f32 ? launch_tile<64, 64, 2, true>(p, s) : launch_tile<64, 64, 2, false>(p, s);
 }
 
 }  // namespace

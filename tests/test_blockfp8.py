@@ -244,7 +244,11 @@ def test_c_entries_check_their_arguments_before_any_launch():
 
 
 def test_join_struct_layout_matches_header():
-    assert C.sizeof(_lib.SugarBlockJoin) == 8 + 9 * 4 + 3 * 4 + 7 * 8 + 12 * 8
+    from sugar_amd import blockfp8
+    assert C.sizeof(_lib.SugarBlockJoin) == 8 + 9 * 4 + 3 * 4 + 7 * 8 + 12 * 8 == blockfp8._JOIN.size
+    values = tuple(range(1, 11)) + (0.5, 0.25, 0.125) + tuple(range(20, 39))
+    d = _lib.SugarBlockJoin.from_buffer_copy(blockfp8._JOIN.pack(*values))
+    assert tuple(getattr(d, name) for name, _ in d._fields_) == values
 
 
 # ------------------------------------------------------------------------------------------------ quantisation
