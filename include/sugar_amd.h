@@ -23,6 +23,9 @@
  *     reduction (instance norm, SE mean, attentive pooling) runs over each utterance's true frames.
  *   - dtype: SUGAR_F32 = exact-f32 MFMA path (parity >= 0.9999 cosine), SUGAR_BF16 = bf16 operands with f32
  *     accumulation (parity >= 0.999 cosine).  It selects the element type of feats / activations / weights.
+ *     SUGAR_FP8 is a subnet's precision, not a buffer's type: SUGAR_BF16 throughout, but block outputs, catconv's weights
+ *     and (385 .. 512 channels and multiples) the first convs' weights are held in 8 bits with block scales (parity >= 0.998
+ *     cosine).  Recalibration of such a subnet runs as that of a SUGAR_BF16 one.
  */
 #ifndef SUGAR_AMD_H
 #define SUGAR_AMD_H
@@ -35,6 +38,7 @@ extern "C" {
 
 #define SUGAR_F32 0
 #define SUGAR_BF16 1
+#define SUGAR_FP8 2         /* sugar_subnet_create only */
 
 #define SUGAR_OK 0
 #define SUGAR_EINVAL (-1)   /* bad argument (shape, alignment, NULL)            */

@@ -10,7 +10,8 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libsugar_amd.so")
 
-SUGAR_F32, SUGAR_BF16 = 0, 1
+SUGAR_F32, SUGAR_BF16, SUGAR_FP8 = 0, 1, 2
+PRECISIONS = {"bf16": SUGAR_BF16, "fp32": SUGAR_F32, "fp8": SUGAR_FP8}
 MAX_DEPTH, RES2_SCALE = 8, 8
 EPI_RELU, EPI_AFFINE, EPI_TANH = 1, 2, 4
 

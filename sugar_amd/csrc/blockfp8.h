@@ -155,10 +155,39 @@ struct Fp8Operand {        // [rows][ld] e4m3, [rows][lds] exponent bytes
   int64_t ldq = 0, lde = 0;
 };
 
+struct Fp8Weight {         // device-resident [n][k] operand of a layer (packed by pack_fp8)
+  uint8_t* q = nullptr;
+  uint8_t* e = nullptr;
+  int n = 0, k = 0;
+  Fp8Operand operand() const {
+    Fp8Operand o;
+    o.q = q; o.e = e; o.ldq = fp8_ldq(k); o.lde = fp8_lds(k);
+    return o;
+  }
+};
+// Reference-layout 1x1 conv weight [cout][cin] (host f32) -> [n][k] with out_map / in_map as pack_conv; the same values
+// sugar_fp8_quant gives
+int pack_fp8(Fp8Weight* w, const float* h_w, int cout, int cin, int n, const int* out_map, int k, const int* in_map);
+void free_fp8(Fp8Weight* w);
+
+struct Fp8Out {
+  void* y = nullptr;       // [rows][ldy] dtype
+  int64_t ldy = 0;
+  int dtype = SUGAR_BF16;
+  void* y2 = nullptr;      // optional second store (bf16 only) of columns >= y2_from, a multiple of 8 (pointer has NO column offset)
+  int64_t ldy2 = 0;
+  int y2_from = 0;
+};
+
 // y[r][o] = epilogue(sum_k a[r][k] w[o][k]), flags EPI_RELU | EPI_AFFINE (scale / shift [n], applied after the ReLU)
 int launch_fp8_linear(const Fp8Operand& a, int64_t rows, const Fp8Operand& w, int n, int k, const float* scale,
-                      const float* shift, int flags, void* d_y, int64_t ldy, int dtype, hipStream_t s);
+                      const float* shift, int flags, const Fp8Out& out, hipStream_t s);
 
-int launch_block_join(const SugarBlockJoin& j, hipStream_t s);
+// y [rows][ldy] dtype <- the first `cols` values of an operand (its exponent rows may begin anywhere)
+int launch_fp8_dequant(const Fp8Operand& a, int64_t rows, int cols, void* d_y, int64_t ldy, int dtype, hipStream_t s);
+
+// pad_exponents: also the padding bytes behind a row's last block (not where the 8-bit output is a column slice: the bytes
+// behind it belong to the next slice or row)
+int launch_block_join(const SugarBlockJoin& j, bool pad_exponents, hipStream_t s);
 
 }  // namespace sugar

@@ -1,5 +1,9 @@
 // Quantisation to 8-bit operands with block scales, their reading back, and the C entries (gfx950; product: fp8_gemm.hip).
 // The format is described in blockfp8.h.
+#include <math.h>
+
+#include <vector>
+
 #include "blockfp8.h"
 
 namespace sugar {
@@ -65,6 +69,73 @@ static int check_operand(const char* what, const uint8_t* q, int64_t ldq, const 
   return SUGAR_OK;
 }
 
+int launch_fp8_dequant(const Fp8Operand& a, int64_t rows, int cols, void* d_y, int64_t ldy, int dtype, hipStream_t s) {
+  const int64_t items = rows * fp8_blocks(cols);
+  const int vec = rows_vec(d_y, ldy, cols, dtype == SUGAR_F32 ? 4 : 2);
+  const unsigned grid = (unsigned)(ceil_div(items, 16) < 65536 ? ceil_div(items, 16) : 65536);
+  if (dtype == SUGAR_F32)
+    hipLaunchKernelGGL(fp8_dequant_kernel<float>, dim3(grid), dim3(256), 0, s, a.q, a.ldq, a.e, a.lde, items, cols,
+                       (int)fp8_blocks(cols), vec, (float*)d_y, ldy);
+  else
+    hipLaunchKernelGGL(fp8_dequant_kernel<bf16>, dim3(grid), dim3(256), 0, s, a.q, a.ldq, a.e, a.lde, items, cols,
+                       (int)fp8_blocks(cols), vec, (bf16*)d_y, ldy);
+  SUGAR_LAUNCH_CHECK();
+  return SUGAR_OK;
+}
+
+// host side of the quantiser: e4m3 bits of |v| <= 448, to nearest with ties to even (rint in the default mode)
+static uint8_t host_e4m3(float v) {
+  const uint8_t sign = signbit(v) ? 0x80 : 0;
+  const float a = fabsf(v);
+  if (!(a <= 448.f)) return sign | 0x7f;
+  if (a < 0.015625f) return sign | (uint8_t)rintf(a * 512.f);         // subnormals; 8 is the smallest normal's bits
+  int e;
+  (void)frexpf(a, &e);                                                // a = m 2^e, m in [0.5, 1)
+  int m = (int)rintf(ldexpf(a, 4 - e));                               // [8, 16]
+  if (m == 16) { m = 8; ++e; }
+  return sign | (uint8_t)((e + 6) << 3 | (m - 8));
+}
+
+int pack_fp8(Fp8Weight* w, const float* h_w, int cout, int cin, int n, const int* out_map, int k, const int* in_map) {
+  const int64_t ldq = fp8_ldq(k), lde = fp8_lds(k);
+  std::vector<uint8_t> q((size_t)(n * ldq), 0), e((size_t)(n * lde), 127);
+  std::vector<float> row((size_t)ldq);
+  for (int64_t r = 0; r < n; ++r)                                     // rows no channel maps to: zeros, exponent as of zeros
+    for (int64_t b = 0; b < fp8_blocks(k); ++b) e[(size_t)(r * lde + b)] = 0;
+  for (int o = 0; o < cout; ++o) {
+    const int64_t r = out_map ? out_map[o] : o;
+    row.assign(row.size(), 0.f);
+    for (int i = 0; i < cin; ++i) row[(size_t)(in_map ? in_map[i] : i)] = h_w[(size_t)o * cin + i];
+    for (int64_t b = 0; b < fp8_blocks(k); ++b) {
+      uint32_t big = 0;
+      for (int c = 0; c < FP8_BLOCK; ++c) {
+        uint32_t u;
+        memcpy(&u, &row[(size_t)(b * FP8_BLOCK + c)], 4);
+        u &= 0x7fffffffu;
+        if (u < 0x7f800000u && u > big) big = u;
+      }
+      int byte = (int)((big + 0x1fffffu) >> 23) - 8;                  // fp8_exponent
+      if (byte < 0) byte = 0;
+      e[(size_t)(r * lde + b)] = (uint8_t)byte;
+      for (int c = 0; c < FP8_BLOCK; ++c)
+        q[(size_t)(r * ldq + b * FP8_BLOCK + c)] = host_e4m3(ldexpf(row[(size_t)(b * FP8_BLOCK + c)], 127 - byte));
+    }
+  }
+  int rc;
+  if ((rc = dev_alloc(&w->q, q.size())) || (rc = dev_upload(w->q, q.data(), q.size())) || (rc = dev_alloc(&w->e, e.size())) ||
+      (rc = dev_upload(w->e, e.data(), e.size())))
+    return rc;
+  w->n = n;
+  w->k = k;
+  return SUGAR_OK;
+}
+
+void free_fp8(Fp8Weight* w) {
+  dev_free(w->q);
+  dev_free(w->e);
+  *w = Fp8Weight();
+}
+
 }  // namespace sugar
 
 using namespace sugar;
@@ -100,17 +171,9 @@ int sugar_fp8_dequant(const uint8_t* d_q, int64_t ldq, const uint8_t* d_e, int64
   if (rows == 0) return SUGAR_OK;
   const int esz = dtype == SUGAR_F32 ? 4 : 2;
   SUGAR_CHECK_ARG((uintptr_t)d_y % esz == 0, "fp8_dequant: unaligned output");
-  const int64_t items = rows * fp8_blocks(cols);
-  const int vec = rows_vec(d_y, ldy, cols, esz);
-  const unsigned grid = (unsigned)(ceil_div(items, 16) < 65536 ? ceil_div(items, 16) : 65536);
-  if (dtype == SUGAR_F32)
-    hipLaunchKernelGGL(fp8_dequant_kernel<float>, dim3(grid), dim3(256), 0, (hipStream_t)stream, d_q, ldq, d_e, lde, items,
-                       cols, (int)fp8_blocks(cols), vec, (float*)d_y, ldy);
-  else
-    hipLaunchKernelGGL(fp8_dequant_kernel<bf16>, dim3(grid), dim3(256), 0, (hipStream_t)stream, d_q, ldq, d_e, lde, items,
-                       cols, (int)fp8_blocks(cols), vec, (bf16*)d_y, ldy);
-  SUGAR_LAUNCH_CHECK();
-  return SUGAR_OK;
+  Fp8Operand a;
+  a.q = d_q; a.ldq = ldq; a.e = d_e; a.lde = lde;
+  return launch_fp8_dequant(a, rows, cols, d_y, ldy, dtype, (hipStream_t)stream);
 }
 
 int sugar_fp8_linear(const uint8_t* d_a, int64_t lda, const uint8_t* d_ae, int64_t ldae, int64_t rows, const uint8_t* d_w,
@@ -131,7 +194,9 @@ int sugar_fp8_linear(const uint8_t* d_a, int64_t lda, const uint8_t* d_ae, int64
   Fp8Operand a, w;
   a.q = d_a; a.ldq = lda; a.e = d_ae; a.lde = ldae;
   w.q = d_w; w.ldq = ldw; w.e = d_we; w.lde = ldwe;
-  return launch_fp8_linear(a, rows, w, n, k, d_scale, d_shift, flags, d_y, ldy, dtype, (hipStream_t)stream);
+  Fp8Out out;
+  out.y = d_y; out.ldy = ldy; out.dtype = dtype;
+  return launch_fp8_linear(a, rows, w, n, k, d_scale, d_shift, flags, out, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -23,6 +23,9 @@ struct LinearArgs {
   int rows, n, kb, flags, out_f32;
   int vec;                            // 16-byte stores: y aligned, n and ldy multiples of 16 bytes
   int n_co_tiles;
+  bf16* y2;                           // second store of columns >= y2_from (whole chunks of 8), or nullptr
+  int64_t ldy2;
+  int y2_from;
 };
 
 // ReLU in one instruction that hands NaN on (a maximum, not a maxNum)
@@ -74,7 +77,10 @@ __device__ __forceinline__ void store_out4(const LinearArgs& p, int64_t r, int c
     if (co + i >= p.n) break;
     const float t = p.flags & EPI_AFFINE ? fmaf(v[i], p.scale[co + i], p.shift[co + i]) : v[i];
     if (p.out_f32) ((float*)p.y)[r * p.ldy + co + i] = t;
-    else ((bf16*)p.y)[r * p.ldy + co + i] = (bf16)t;
+    else {
+      ((bf16*)p.y)[r * p.ldy + co + i] = (bf16)t;
+      if (p.y2 && co + i >= p.y2_from) p.y2[r * p.ldy2 + co + i] = (bf16)t;
+    }
   }
 }
 
@@ -265,7 +271,10 @@ __device__ __forceinline__ void fp8_tile(const LinearArgs& p, const int co_base,
       const int f = i * RPP + lane / CPR, ch = lane % CPR;
       const int r = r_base + wn * FW + n * 16 + f, co = co_base + wm * CW + ch * 8;
       const u32x4 v = *(const u32x4*)(ep + f * EPI_STRIDE + ch * 16);
-      if (r < p.rows && co < p.n) *(u32x4*)((bf16*)p.y + (int64_t)r * p.ldy + co) = v;
+      if (r < p.rows && co < p.n) {
+        *(u32x4*)((bf16*)p.y + (int64_t)r * p.ldy + co) = v;
+        if (p.y2 && co >= p.y2_from) *(u32x4*)(p.y2 + (int64_t)r * p.ldy2 + co) = v;
+      }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_wave_barrier();
@@ -565,7 +574,7 @@ int launch_rows(const LinearArgs& p, hipStream_t s) {
     SUGAR_LAUNCH_CHECK();
     return SUGAR_OK;
   }
-  if (!f32 && p.vec && p.kb >= 8 && n_cu % 8 == 0 && ceil_div(p.n, 256) * ceil_div(p.rows, 256) >= 2 * n_cu)
+  if (!f32 && p.vec && !p.y2 && p.kb >= 8 && n_cu % 8 == 0 && ceil_div(p.n, 256) * ceil_div(p.rows, 256) >= 2 * n_cu)
     return launch_persist(p, n_cu, s);
   if (ceil_div(p.n, 128) * ceil_div(p.rows, 128) >= n_cu)
     return f32 ? launch_tile<128, 128, 2, true>(p, s) : launch_tile<128, 128, 2, false>(p, s);
@@ -577,23 +586,26 @@ int launch_rows(const LinearArgs& p, hipStream_t s) {
 }  // namespace
 
 int launch_fp8_linear(const Fp8Operand& a, int64_t rows, const Fp8Operand& w, int n, int k, const float* scale,
-                      const float* shift, int flags, void* d_y, int64_t ldy, int dtype, hipStream_t s) {
+                      const float* shift, int flags, const Fp8Out& out, hipStream_t s) {
   // the kernels' row offsets are 32-bit: weights that do not fit are refused, rows beyond go to a launch of their own
   constexpr int64_t SPAN = (1ll << 32) - 4096;
   SUGAR_CHECK_ARG(n * w.ldq <= SPAN && n * w.lde <= SPAN, "fp8_linear: weights of %d rows with stride %lld are too large", n,
                   (long long)w.ldq);
   SUGAR_CHECK_ARG(a.ldq <= SPAN / 256 && a.lde <= SPAN / 256, "fp8_linear: row stride %lld too large", (long long)a.ldq);
   const int64_t per = SPAN / (a.ldq > a.lde ? a.ldq : a.lde) / 256 * 256;
-  const int esz = dtype == SUGAR_F32 ? 4 : 2;
+  const int esz = out.dtype == SUGAR_F32 ? 4 : 2;
   LinearArgs p;
   p.lda = (unsigned)a.ldq; p.ldae = (unsigned)a.lde;
   p.w = w.q; p.we = w.e; p.ldw = (unsigned)w.ldq; p.ldwe = (unsigned)w.lde;
-  p.ldy = ldy; p.scale = scale; p.shift = shift;
-  p.n = n; p.kb = (int)fp8_blocks(k); p.flags = flags; p.out_f32 = dtype == SUGAR_F32; p.n_co_tiles = 0;
-  p.vec = ((uintptr_t)d_y & 15) == 0 && (ldy * esz) % 16 == 0 && (n * esz) % 16 == 0;
+  p.ldy = out.ldy; p.scale = scale; p.shift = shift;
+  p.n = n; p.kb = (int)fp8_blocks(k); p.flags = flags; p.out_f32 = out.dtype == SUGAR_F32; p.n_co_tiles = 0;
+  p.ldy2 = out.ldy2; p.y2_from = out.y2_from;
+  p.vec = ((uintptr_t)out.y & 15) == 0 && (out.ldy * esz) % 16 == 0 && (n * esz) % 16 == 0 &&
+          ((uintptr_t)out.y2 & 15) == 0 && (out.ldy2 * esz) % 16 == 0;
   for (int64_t r0 = 0; r0 < rows; r0 += per) {
     p.a = a.q + r0 * a.ldq; p.ae = a.e + r0 * a.lde;
-    p.y = (char*)d_y + r0 * ldy * esz;
+    p.y = (char*)out.y + r0 * out.ldy * esz;
+    p.y2 = out.y2 ? (bf16*)out.y2 + r0 * out.ldy2 : nullptr;
     p.rows = (int)(rows - r0 < per ? rows - r0 : per);
     if (int rc = launch_rows(p, s)) return rc;
   }

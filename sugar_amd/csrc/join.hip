@@ -18,6 +18,7 @@ enum { NORM_NONE = SUGAR_NORM_NONE, NORM_AFFINE = SUGAR_NORM_AFFINE, NORM_RMS = 
 
 struct JoinArgs {
   SugarBlockJoin j;
+  int e_bytes;               // exponent bytes of a row that are written (the blocks, and padding where the row is an operand of its own)
 };
 
 // Sum over the 64 lanes, the same in every lane: within rows of 16 by DPP, across them by the row / half swaps (of a value
@@ -222,7 +223,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void block_join_kernel(Jo
           *(u32x2*)(j.d_q + r * j.ldq + c) = fp8_pack8(s[k], fp8_inverse(byte));
           const int l16 = lane & 15;
           if (l16 == 0) j.d_e[r * j.lde + kb] = (uint8_t)byte;
-          else if (kb == blocks - 1 && kb + l16 < ((blocks + 3) & ~3)) j.d_e[r * j.lde + kb + l16] = 127;   // padding bytes
+          else if (kb == blocks - 1 && kb + l16 < a.e_bytes) j.d_e[r * j.lde + kb + l16] = 127;   // padding bytes
         }
       }
     }
@@ -255,9 +256,10 @@ bool norm_ok(int kind) { return kind == NORM_NONE || kind == NORM_AFFINE || kind
 
 }  // namespace
 
-int launch_block_join(const SugarBlockJoin& j, hipStream_t s) {
+int launch_block_join(const SugarBlockJoin& j, bool pad_exponents, hipStream_t s) {
   JoinArgs a;
   a.j = j;
+  a.e_bytes = (int)(pad_exponents ? fp8_lds(j.cols) : fp8_blocks(j.cols));
   const int eu = j.u_dtype == SUGAR_F32 ? 4 : 2, es = j.stream_dtype == SUGAR_F32 ? 4 : 2, ez = j.z_dtype == SUGAR_F32 ? 4 : 2;
   const int eg = j.gate_kind == SUGAR_GATE_ROW ? eu : 4;
   // one path for rows that are all 16-byte aligned in whole chunks of 8 channels, one for everything else
@@ -301,5 +303,5 @@ extern "C" int sugar_block_join(const SugarBlockJoin* h, void* stream) {
     SUGAR_CHECK_ARG(j.d_e && !((uintptr_t)j.d_q & 15) && j.ldq % 16 == 0 && j.ldq >= fp8_ldq(j.cols) && j.lde >= fp8_lds(j.cols),
                     "block_join: bad 8-bit output");
   if (j.rows == 0) return SUGAR_OK;
-  return launch_block_join(j, (hipStream_t)stream);
+  return launch_block_join(j, true, (hipStream_t)stream);
 }

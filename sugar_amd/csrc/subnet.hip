@@ -13,7 +13,7 @@
 #include <mutex>
 #include <vector>
 
-#include "common.h"
+#include "blockfp8.h"
 
 namespace sugar {
 
@@ -113,6 +113,7 @@ int device_cu_count(int* n_cu) {
 
 struct Block {
   ConvLayer first, res[SUGAR_RES2_SCALE - 1], last;
+  Fp8Weight first8;                                            // SUGAR_FP8: first_conv on the previous block's 8-bit output
   SELayer se;
   BNState bn_first, bn_res[SUGAR_RES2_SCALE - 1], bn_last;   // raw BN parameters + running statistics (recalibration)
   int w = 0, wp = 0, midp = 0, kernel = 1;
@@ -123,6 +124,8 @@ struct Block {
 struct SugarSubnet {
   int dtype = SUGAR_BF16, device = 0;
   int in_feats = 80, embed = 192, depth = 0, c0 = 0, c0p = 0, ccat = 0, ccatp = 0, bott = 128, midp_max = 0;
+  bool fp8 = false;          // SUGAR_FP8: dtype is SUGAR_BF16, catconv and the first convs behind a block run in 8 bits
+  sugar::Fp8Weight catconv8;
   sugar::ConvLayer layer1, catconv, pool1;
   sugar::Block blocks[SUGAR_MAX_DEPTH];
   sugar::PoolLayer pool;
@@ -149,9 +152,11 @@ static void destroy(SugarSubnet* n) {
     free_conv(&n->layer1);
     free_conv(&n->catconv);
     free_conv(&n->pool1);
+    free_fp8(&n->catconv8);
     for (int i = 0; i < SUGAR_MAX_DEPTH; ++i) {
       Block& b = n->blocks[i];
       free_conv(&b.first);
+      free_fp8(&b.first8);
       free_conv(&b.last);
       for (auto& r : b.res) free_conv(&r);
       dev_free(b.se.w1t);
@@ -209,7 +214,12 @@ static int fold_tail(SugarSubnet* n, const float* const pool_bn[4], const float*
   return SUGAR_OK;
 }
 
+// SUGAR_FP8: columns a block's output takes in the 8-bit catconv input (whole scale blocks: no scale spans two outputs)
+static int cat8_slice(const SugarSubnet* n) { return (int)fp8_ldq(n->c0p); }
+
 static int create(const SugarSubnetDesc* d, int dtype, SugarSubnet* n) {
+  n->fp8 = dtype == SUGAR_FP8;
+  if (n->fp8) dtype = SUGAR_BF16;
   const int E = dtype == SUGAR_F32 ? 4 : 8;
   n->dtype = dtype;
   n->in_feats = d->in_feats;
@@ -248,6 +258,10 @@ static int create(const SugarSubnetDesc* d, int dtype, SugarSubnet* n) {
     if ((rc = pack_conv(&b.first, sb.first_w, &sb.first_bn, sb.mid_channels, d->c0, 1, 1, EPI_RELU, b.midp,
                         midmap.data(), n->c0p, nullptr, dtype)) ||
         (rc = bn_state_create(&b.bn_first, &sb.first_bn, sb.mid_channels, b.midp, midmap.data())))
+      return rc;
+    // exponent rows of a slice must begin on a dword to be an operand of their own: 4 blocks, i.e. 385 .. 512 channels etc.
+    if (n->fp8 && i > 0 && cat8_slice(n) % (4 * FP8_BLOCK) == 0 &&
+        (rc = pack_fp8(&b.first8, sb.first_w, sb.mid_channels, d->c0, b.midp, midmap.data(), n->c0p, nullptr)))
       return rc;
     for (int j = 0; j < SUGAR_RES2_SCALE - 1; ++j) {
       SUGAR_CHECK_ARG(sb.res_w[j] && bn_ok(sb.res_bn[j]), "block %d res2 conv %d: null tensor", i, j);
@@ -288,6 +302,13 @@ static int create(const SugarSubnetDesc* d, int dtype, SugarSubnet* n) {
     if ((rc = pack_conv(&n->catconv, d->catconv_w, nullptr, d->ccat, d->depth * d->c0, 1, 1, EPI_RELU, n->ccatp,
                         nullptr, d->depth * n->c0p, catmap.data(), dtype)))
       return rc;
+    if (n->fp8) {
+      const int slice = cat8_slice(n);
+      for (int blk = 0; blk < d->depth; ++blk)
+        for (int j = 0; j < d->c0; ++j) catmap[(size_t)blk * d->c0 + j] = blk * slice + j;
+      if ((rc = pack_fp8(&n->catconv8, d->catconv_w, d->ccat, d->depth * d->c0, n->ccatp, nullptr, d->depth * slice, catmap.data())))
+        return rc;
+    }
   }
   // pooling.linear1 (+tanh) as a conv; pooling.linear2 as the fused kernel's B operand  dynamictdnn.py:498-499
   if ((rc = pack_conv(&n->pool1, d->pool1_w, nullptr, d->bottleneck, d->ccat, 1, 1, EPI_TANH, d->bottleneck, nullptr,
@@ -338,6 +359,7 @@ struct Workspace {
   int2* rowseg;
   float* logmel;
   void *feats, *featp, *S, *cat, *mid1, *mid2, *ybuf, *hbuf, *abuf;
+  uint8_t *cat8, *cat8e;                 // SUGAR_FP8: catconv input in 8 bits and its exponents
   int32_t* orow;     // layer1 tap GEMM: output-row map of the padded row space
   float *separt, *sescale, *pooled, *poolpart, *tailpart;
   double* bnpart;    // recalibration: partial sums, batch (scale, shift), pre-BN embeddings
@@ -361,6 +383,8 @@ static Workspace plan(const SugarSubnet* n, int B, int64_t R, void* base) {
   w.orow = (int32_t*)take(gemm_taps_orow_ints(n->layer1, B, R) * 4);
   w.S = take(R * n->c0p * esz);
   w.cat = take(R * (int64_t)n->depth * n->c0p * esz);
+  w.cat8 = (uint8_t*)take(n->fp8 ? R * n->depth * cat8_slice(n) : 0);
+  w.cat8e = (uint8_t*)take(n->fp8 ? R * fp8_lds((int64_t)n->depth * cat8_slice(n)) : 0);
   w.mid1 = take(R * n->midp_max * esz);
   w.mid2 = take(R * n->midp_max * esz);
   w.ybuf = take(R * n->c0p * esz);
@@ -429,6 +453,15 @@ static int tdnn_forward(const SugarSubnet* n, const void* feats, const int32_t* 
   if ((rc = tapcopy(0, w.S, n->c0p, n->c0p))) return rc;
 
   const int ldcat = n->depth * n->c0p;
+  // SUGAR_FP8: block output i as an 8-bit operand, a column slice of the catconv input as `out` below
+  Fp8Operand cat8;
+  cat8.q = w.cat8; cat8.ldq = (int64_t)n->depth * cat8_slice(n); cat8.e = w.cat8e; cat8.lde = fp8_lds(cat8.ldq);
+  auto slice8 = [&](int i) {
+    Fp8Operand o = cat8;
+    o.q += (int64_t)i * cat8_slice(n);
+    o.e += (int64_t)i * cat8_slice(n) / FP8_BLOCK;
+    return o;
+  };
   for (int i = 0; i < n->depth; ++i) {
     const Block& b = n->blocks[i];
     // block input: layer1 output (still == S) for block 0, else the previous block's slice of the cat buffer
@@ -437,7 +470,17 @@ static int tdnn_forward(const SugarSubnet* n, const void* feats, const int32_t* 
     ConvIO f;
     f.x = xin; f.ldx = ldin; f.y = w.mid1; f.ldy = b.midp;
     f.y2 = w.mid2; f.ldy2 = b.midp; f.y2_from = (SUGAR_RES2_SCALE - 1) * b.wp;   // 8th split passes through (:300-301)
-    { Prof p(SUGAR_STAGE_FIRST, s); if ((rc = conv(b.first, f))) return rc; }
+    {
+      Prof p(SUGAR_STAGE_FIRST, s);
+      if (b.first8.q) {
+        Fp8Out o;
+        o.y = f.y; o.ldy = f.ldy; o.y2 = f.y2; o.ldy2 = f.ldy2; o.y2_from = f.y2_from;
+        rc = launch_fp8_linear(slice8(i - 1), R, b.first8.operand(), b.midp, n->c0p, b.first.scale, b.first.shift, b.first.flags, o, s);
+      } else {
+        rc = conv(b.first, f);
+      }
+      if (rc) return rc;
+    }
     if ((rc = tapcopy(1 + 4 * i, w.mid1, b.midp, b.midp))) return rc;
     {
     Prof p(SUGAR_STAGE_RES2, s);
@@ -461,15 +504,43 @@ static int tdnn_forward(const SugarSubnet* n, const void* feats, const int32_t* 
     void* out = col(w.cat, (int64_t)i * n->c0p);
     {
       Prof p(SUGAR_STAGE_SE_APPLY, s);
-      if ((rc = launch_se_apply(w.ybuf, n->c0p, w.sescale, n->c0p, w.S, n->c0p, out, ldcat, i + 1 < n->depth, row_off, B,
-                                t_max, dt, s)))
-        return rc;
+      if (n->fp8) {                                // out and S as below, out rounded to 8 bits (and to 16 where a bf16 conv reads it)
+        const bool last = i + 1 == n->depth;
+        SugarBlockJoin j = SugarBlockJoin();
+        j.rows = R; j.cols = n->c0p; j.n_utts = B;
+        j.u_dtype = j.stream_dtype = j.z_dtype = SUGAR_BF16;
+        j.gate_kind = SUGAR_GATE_UTTERANCE; j.dense = 1; j.alpha = 1.f;
+        j.d_u = w.ybuf; j.ldu = n->c0p; j.d_residual = w.S; j.ldr = n->c0p;
+        j.d_gate = w.sescale; j.ldg = n->c0p; j.d_row_off = row_off;
+        if (!last) { j.d_stream = w.S; j.lds = n->c0p; }
+        if (!last && !n->blocks[i + 1].first8.q) { j.d_z = out; j.ldz = ldcat; }
+        const Fp8Operand o = slice8(i);
+        j.d_q = const_cast<uint8_t*>(o.q); j.ldq = o.ldq; j.d_e = const_cast<uint8_t*>(o.e); j.lde = o.lde;
+        rc = launch_block_join(j, false, s);
+      } else {
+        rc = launch_se_apply(w.ybuf, n->c0p, w.sescale, n->c0p, w.S, n->c0p, out, ldcat, i + 1 < n->depth, row_off, B, t_max, dt, s);
+      }
+      if (rc) return rc;
     }
-    if ((rc = tapcopy(4 + 4 * i, out, ldcat, n->c0p))) return rc;
+    if (n->fp8 && tap == 4 + 4 * i && tap_out) {
+      if ((rc = launch_fp8_dequant(slice8(i), R, n->c0p, tap_out, n->c0p, SUGAR_F32, s))) return rc;
+    } else if ((rc = tapcopy(4 + 4 * i, out, ldcat, n->c0p))) {
+      return rc;
+    }
   }
   ConvIO c;
   c.x = w.cat; c.ldx = ldcat; c.y = w.hbuf; c.ldy = n->ccatp;
-  { Prof p(SUGAR_STAGE_CATCONV, s); if ((rc = conv(n->catconv, c))) return rc; }
+  {
+    Prof p(SUGAR_STAGE_CATCONV, s);
+    if (n->fp8) {
+      Fp8Out o;
+      o.y = w.hbuf; o.ldy = n->ccatp;
+      rc = launch_fp8_linear(cat8, R, n->catconv8.operand(), n->ccatp, n->catconv8.k, nullptr, nullptr, EPI_RELU, o, s);
+    } else {
+      rc = conv(n->catconv, c);
+    }
+    if (rc) return rc;
+  }
   if ((rc = tapcopy(100, w.hbuf, n->ccatp, n->ccatp))) return rc;
   ConvIO p1;
   p1.x = w.hbuf; p1.ldx = n->ccatp; p1.y = w.abuf; p1.ldy = n->bott;
@@ -635,7 +706,7 @@ const char* sugar_version(void) { return "sugar_amd 0.1 (gfx950)"; }
 
 int sugar_subnet_create(const SugarSubnetDesc* d, int dtype, int device, SugarSubnet** out) {
   SUGAR_CHECK_ARG(d && out, "subnet_create: null pointer");
-  SUGAR_CHECK_ARG(dtype == SUGAR_F32 || dtype == SUGAR_BF16, "subnet_create: bad dtype %d", dtype);
+  SUGAR_CHECK_ARG(dtype == SUGAR_F32 || dtype == SUGAR_BF16 || dtype == SUGAR_FP8, "subnet_create: bad dtype %d", dtype);
   SUGAR_CHECK_ARG(d->depth >= 1 && d->depth <= SUGAR_MAX_DEPTH, "subnet_create: depth %d out of range", d->depth);
   SUGAR_CHECK_ARG(d->in_feats == SUGAR_N_MELS, "subnet_create: in_feats %d (only 80 supported)", d->in_feats);
   SUGAR_CHECK_ARG(d->c0 > 0 && d->ccat > 0 && d->embed_dim > 0 && d->bottleneck == 128,

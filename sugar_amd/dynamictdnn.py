@@ -199,8 +199,8 @@ class TDNNSubnet(nn.Module):
         return self._device
 
     def set_precision(self, precision):
-        if precision not in ("bf16", "fp32"):
-            raise ValueError("precision %r not in ['bf16', 'fp32']" % (precision,))
+        if precision not in _lib.PRECISIONS:
+            raise ValueError("precision %r not in %s" % (precision, sorted(_lib.PRECISIONS)))
         if precision != self.precision:
             self._generation += 1
         self.precision = precision
@@ -234,7 +234,12 @@ class TDNNSubnet(nn.Module):
 
     @property
     def dtype_id(self):
-        return _lib.SUGAR_BF16 if self.precision == "bf16" else _lib.SUGAR_F32
+        return _lib.PRECISIONS[self.precision]
+
+    @property
+    def feature_dtype(self):
+        """Type of the front-end's features and of the 16-bit / 32-bit activations ("fp8" subnets: bfloat16)."""
+        return torch.float32 if self.precision == "fp32" else torch.bfloat16
 
     # ---- packing -----------------------------------------------------------------------------------------
     def handle(self, device=None):
@@ -308,7 +313,7 @@ class TDNNSubnet(nn.Module):
         if not x.is_cuda:
             raise _lib.SugarError("sugar_amd runs on an MI355X only: features must be CUDA tensors (no CPU fallback)")
         B, _, T = x.shape
-        dt = torch.bfloat16 if self.precision == "bf16" else torch.float32
+        dt = self.feature_dtype
         feats = x.transpose(1, 2).to(dt).contiguous().view(B * T, self.in_feats)   # channels-last packed rows
         row_off = torch.arange(0, (B + 1) * T, T, dtype=torch.int32, device=x.device)
         return self.forward_rows(feats, row_off, B, B * T, T)

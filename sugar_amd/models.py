@@ -9,7 +9,7 @@ Differences, all forced by the environment or by the scope of this build:
   * there is no network: ``supernet_filename`` / ``subnet_filename`` are LOCAL paths (``repo_id`` is a local
     directory they are resolved against, or "" / None); file formats are the reference's
     (``{'state_dict': {'module.__S__.*': ...}}`` and ``{'subnet': config, 'bn': {...}}``);
-  * ``precision`` ("bf16" default, "fp32") selects the MFMA path;
+  * ``precision`` ("bf16" default, "fp32", "fp8") selects the MFMA path;
   * ``forward`` also accepts a list of 1-D waveforms of different lengths (the reference runs those at batch 1);
   * the loss head (``__L__``) is not on the inference path: ``label`` must be None.
 """
@@ -130,7 +130,7 @@ class WrappedModel(nn.Module):
         returned `info` keys are the reference's (sugar/models/__init__.py:129-165), the files are local."""
         front_end = _choice("feat_type", feat_type, _FRONT_ENDS)
         backbone = _choice("model_type", model_type, _BACKBONES)
-        _choice("precision", precision, {"bf16": None, "fp32": None})
+        _choice("precision", precision, _lib.PRECISIONS)
         info = {"supernet_file": _local_file(repo_id, supernet_filename), "subnet_file": None, "subnet": None}
         info["supernet"] = torch.load(info["supernet_file"], map_location="cpu", weights_only=True)["state_dict"]
         transform = front_end(n_mels=feat_dim)

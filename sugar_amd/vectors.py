@@ -231,7 +231,7 @@ def _packed_features(packed, spk, sub):
     from .transforms import LogMelFbanks
     if not packed.cache_features or sub.training or not isinstance(getattr(spk, "__T__", None), LogMelFbanks):
         return None
-    return packed.features(spk.__T__, torch.bfloat16 if sub.precision == "bf16" else torch.float32)
+    return packed.features(spk.__T__, sub.feature_dtype)
 
 
 def _walk(datalst, n_jobs):

@@ -572,3 +572,54 @@ def test_results_do_not_depend_on_the_other_rows():
     j = block_join(u, res, pre=norm_of("rms", 512, 5))
     k = block_join(u[7:9], res[7:9], pre=norm_of("rms", 512, 5))
     assert torch.equal(j.normed[7:9], k.normed)
+
+
+@gpu
+@pytest.mark.parametrize("r,n,k", [(23000, 1536, 1152), (44000, 776, 1400), (100001, 264, 1024), (35000, 1024, 2100)])
+def test_linear_persistent_tiles(r, n, k):
+    """Products of two rounds of 256 x 256 tiles and more: odd numbers of k-tiles, channels and rows that end inside a tile,
+    one tile of channels, tails; with and without the affine vectors, and rows around the output left alone."""
+    a, w = operands(r, r, n, k)
+    s, t = rows_of(8, 1, n)[0].cuda(), rows_of(9, 1, n)[0].cuda()
+    out = torch.full((r + 2, n + 8), 7.0, dtype=torch.bfloat16, device="cuda")
+    for scale, shift, relu in ((s, t, True), (None, None, False)):
+        got = block_fp8_linear(a, w, scale=scale, shift=shift, relu=relu, out=out[1:r + 1, :n])
+        wide = block_fp8_linear(a, w, scale=scale, shift=shift, relu=relu, out_dtype=torch.float32)
+        for lo in (0, 200, r // 2, r - 333):
+            rows = slice(lo, lo + 333)
+            y, mag = linear64(a[rows], w, scale, shift, relu)
+            assert ((wide[rows].cpu().double() - y).abs() <= (k + 4) * U32 * mag).all()
+            f = 1.0 if scale is None else scale.cpu().double().abs()
+            tol = ((k + 4) * U32 * mag + cut64(a[rows], w) * f) * (1 + 2.0 ** -8) + 2.0 ** -8 * y.abs()
+            assert ((got[rows].cpu().double() - y).abs() <= tol).all()
+        # everywhere, against the float32 output: cut-offs and roundings of both
+        top = a.data.float().abs().amax(1)
+        assert torch.isfinite(top).all()
+        assert ((got.float() - wide).norm() / wide.norm()).item() <= 2.0 ** -8
+        worst = (got.float() - wide).abs().amax(1) / wide.abs().amax(1).clamp(min=1e-30)
+        assert (worst <= 2.0 ** -7).all()
+    assert (out[0] == 7).all() and (out[-1] == 7).all() and (out[:, n:] == 7).all()
+
+
+@gpu
+def test_linear_huge_operand_offsets():
+    """Rows whose byte offsets pass 32 bits: the left operand is cut into launches."""
+    r, k, n = 2_200_000, 2048, 8
+    a = BlockFP8.empty(r, k, "cuda")
+    a.data.view(torch.uint8).fill_(0x38)                                # 1.0
+    a.exponent.fill_(127)
+    w = quantize_block_fp8(rows_of(1, n, k).cuda())
+    probe = [0, 1, 2_000_000, 2_097_000, 2_097_151, 2_097_152, 2_100_000, r - 1]
+    x = rows_of(2, len(probe), k, spread=0.2).cuda()
+    q = quantize_block_fp8(x)
+    for i, row in enumerate(probe):
+        a.data[row:row + 1].view(torch.uint8).copy_(q.data[i:i + 1].view(torch.uint8))
+        a.exponent[row:row + 1].copy_(q.exponent[i:i + 1])
+    y = block_fp8_linear(a, w, out_dtype=torch.float32)
+    want, mag = linear64(q, w, None, None, False)
+    assert ((y[probe].cpu().double() - want).abs() <= (k + 4) * U32 * mag).all()
+    ones, mag = values64(w).sum(1), values64(w).abs().sum(1)
+    keep = torch.ones(r, dtype=torch.bool, device="cuda")
+    keep[probe] = False
+    bad = ((y.double() - ones.cuda()).abs() > ((k + 4) * U32 * mag).cuda()).any(1) & keep
+    assert not bad.any()

@@ -1,0 +1,157 @@
+"""
+Precision "fp8" of the embedding path: block outputs, catconv's and the first convs' weights in 8 bits with block scales,
+everything else as in "bf16".
+
+Bars.  Rounding to e4m3 is off by at most 2^-4 of a value, evenly spread at worst: 2^-4 / sqrt(3) = 0.036 in the mean
+square.  A product has two rounded factors, so sums of products are off by at most 0.036 sqrt(2) = 0.051 of their norm (the
+errors of the terms are independent, and the terms add like them).  One such layer is followed by others that see a relative
+error of their input: an embedding off by 0.051 of its norm has a cosine of 1 - 0.051^2 / 2 = 0.9987 with the exact one;
+the bar for whole embeddings is 0.998.
+"""
+import ctypes as C
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+import sugar_amd
+from oracle import ref_cpu
+from sugar_amd import _lib, layout, synth
+from sugar_amd.graphs import GraphedEmbedder
+
+gpu = pytest.mark.gpu
+DEV = "cuda:0"
+CONFIGS = {
+    "base": layout.BASE,                                              # first convs in 8 bits (512 channels = 4 blocks)
+    "largest": layout.LARGEST,
+    "smallest": layout.SMALLEST,                                      # 128 channels: one block a slice, 16-bit first convs
+    "three_blocks": (3, [384, 256, 384, 176], [3, 1, 3, 5], 768),     # a slice of three blocks: exponents off the dword
+    "odd": (4, [176, 136, 256, 176, 200], [5, 3, 1, 5, 3], 536),      # a slice that ends inside its second block
+}
+
+
+def model_of(supernet, cfg, precision):
+    sub = supernet.clone(cfg).set_precision(precision)
+    supernet.config = None
+    return sugar_amd.WrappedModel(sugar_amd.SpeakerModel(sub, transform=sugar_amd.LogMelFbanks())).to(DEV).eval()
+
+
+def test_precision_names(supernet):
+    sub = supernet.clone(layout.SMALLEST)
+    supernet.config = None
+    g = sub.generation
+    assert sub.set_precision("fp8") is sub and sub.dtype_id == _lib.SUGAR_FP8 and sub.feature_dtype == torch.bfloat16
+    assert sub.generation == g + 1
+    assert sub.set_precision("fp32").feature_dtype == torch.float32 and sub.set_precision("bf16").feature_dtype == torch.bfloat16
+    with pytest.raises(ValueError):
+        sub.set_precision("fp16")
+    assert _lib.lib().sugar_subnet_create(C.byref(_lib.SugarSubnetDesc()), 3, 0, C.byref(C.c_void_p())) == -1
+
+
+@gpu
+@pytest.mark.parametrize("name", sorted(CONFIGS))
+def test_embeddings_match_the_oracle(name, supernet, sup_state):
+    cfg = CONFIGS[name]
+    wav = synth.waveforms(6, 20000, seed=3)
+    want = ref_cpu.embed(ref_cpu.clone_state(sup_state, cfg), cfg[0], wav)
+    model = model_of(supernet, cfg, "fp8")
+    emb = model(wav.to(DEV)).cpu()
+    cos = F.cosine_similarity(emb.double(), want.double(), dim=1)
+    print(name, "cosine to the f32 oracle: min %.6f" % cos.min().item())
+    assert cos.min() >= 0.998
+    assert torch.equal(model(wav.to(DEV)).cpu(), emb)                   # repeats bit for bit
+
+
+@gpu
+def test_full_batch_and_ragged_lists(supernet, sup_state):
+    """256 x 3 s (the persistent product, the 128 x 128 tiles) and utterances of unlike lengths in one call, against the
+    same model's bf16 embeddings (cosine >= 0.999 to the oracle themselves)."""
+    fp8, b16 = model_of(supernet, layout.BASE, "fp8"), model_of(supernet, layout.BASE, "bf16")
+    g = torch.Generator(device=DEV).manual_seed(5)
+    wav = torch.randn(256, 48000, device=DEV, generator=g)
+    cos = F.cosine_similarity(fp8(wav).double(), b16(wav).double(), dim=1)
+    print("256 x 3 s: cosine to bf16 min %.6f" % cos.min().item())
+    assert cos.min() >= 0.998
+    lens = [10000, 48000, 16000, 100000, 32001, 9999]
+    wavs = [w.to(DEV) for w in synth.ragged_waveforms(lens, seed=2)]
+    cos = F.cosine_similarity(fp8(wavs).double(), b16(wavs).double(), dim=1)
+    assert cos.min() >= 0.998
+    want = ref_cpu.embed_ragged(ref_cpu.clone_state(sup_state, layout.BASE), 3, [w.cpu() for w in wavs])
+    assert F.cosine_similarity(fp8(wavs).cpu().double(), want.double(), dim=1).min() >= 0.998
+
+
+@gpu
+@pytest.mark.parametrize("name", ["base", "odd", "three_blocks"])
+def test_stage_taps(name, supernet):
+    """Every stage against the bf16 path: identical up to the first 8-bit rounding (block 0's end), relative errors within
+    the bars above behind it (0.051 a layer of products in 8 bits)."""
+    cfg = CONFIGS[name]
+    T = 120
+    feats = torch.randn(2 * T, 80, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(DEV)
+    row_off = torch.tensor([0, T, 2 * T], dtype=torch.int32, device=DEV)
+    subs = [supernet.clone(cfg).set_precision(p) for p in ("bf16", "fp8")]
+    supernet.config = None
+    rel = lambda a, b: ((a.double() - b.double()).norm() / b.double().norm()).item()
+    taps = [0] + [1 + k for k in range(4 * cfg[0])] + [100, 102]
+    for what in taps:
+        want, got = [s.tap(feats, row_off, 2, 2 * T, T, what)[0] for s in subs]
+        err = rel(got, want)
+        if what <= 3:
+            assert torch.equal(got, want), what
+        elif what == 4:
+            assert 0 < err <= 0.036                                     # one rounding
+        else:
+            assert err <= 0.051 * (1 + (what - 4) // 4 if what < 100 else cfg[0] + 1), (what, err)
+    for s in subs:
+        s.release()
+
+
+@gpu
+def test_graph_recalibration_and_precision_changes(supernet, sup_state):
+    """A captured forward replays bit for bit; recalibration of an fp8 subnet moves the statistics as a bf16 one's and its
+    eval path (first convs' affine included) uses them; precisions can be switched to and fro."""
+    model = model_of(supernet, layout.BASE, "fp8")
+    g = GraphedEmbedder(model, synth.waveforms(3, 32000, seed=1).to(DEV), normalize=True)
+    for seed in (2, 3, 4):
+        wav = synth.waveforms(3, 32000, seed=seed).to(DEV)
+        got = g(wav).clone()
+        ref = model(wav, normalize=True)
+        torch.cuda.synchronize()
+        assert torch.equal(got, ref)
+    wav = synth.waveforms(8, 24000, seed=9).to(DEV)
+    before = model(wav)
+    sub = model.module.__S__
+    sub.set_precision("bf16")
+    other = model(wav)
+    sub.set_precision("fp8")
+    assert torch.equal(model(wav), before) and not torch.equal(other, before)
+    pair = [model_of(supernet, layout.BASE, p) for p in ("fp8", "bf16")]
+    for m in pair:
+        m.train()
+        for seed in (11, 12):
+            m(synth.waveforms(8, 24000, seed=seed).to(DEV))
+        m.eval()
+    states = [m.module.__S__.state_dict() for m in pair]
+    assert all(torch.equal(states[0][k], states[1][k]) for k in states[0])
+    embs = [m(wav) for m in pair]
+    assert F.cosine_similarity(embs[0].double(), embs[1].double(), dim=1).min() >= 0.998
+    assert not torch.equal(embs[0], before)
+
+
+@gpu
+def test_host_packed_weights_are_the_quantisers(supernet):
+    """catconv from its own tap: the block outputs in 8 bits times the weights as sugar_fp8_quant would give them."""
+    cfg = CONFIGS["smallest"]
+    sub = supernet.clone(cfg).set_precision("fp8")
+    supernet.config = None
+    T = 90
+    feats = torch.randn(T, 80, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(DEV)
+    row_off = torch.tensor([0, T], dtype=torch.int32, device=DEV)
+    outs = torch.cat([sub.tap(feats, row_off, 1, T, T, 4 + 4 * i)[0] for i in range(cfg[0])], 1)
+    w = dict(sub.named_parameters())["catconv.weight"].detach()[:, :, 0].to(DEV)
+    want = torch.relu(outs.double() @ sugar_amd.quantize_block_fp8(w.contiguous()).dequantize().double().t())
+    got = sub.tap(feats, row_off, 1, T, T, 100)[0].double()
+    # outs are the 8-bit values themselves; what differs is the product's float32 rounding (2^-13 cuts) and bf16's
+    mag = outs.double().abs() @ w.double().abs().t()
+    assert ((got - want).abs() <= 2.0 ** -8 * want + 2.0 ** -10 * mag).all()
+    sub.release()
