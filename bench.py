@@ -47,7 +47,8 @@ PREHEAT_STEPS = 30   # untimed passes at set-up, before the W warm-up steps: the
                      # work to ramp, longer than W = 5 steps (measured: 1.351 ms/step timed after 5 steps from idle,
                      # 1.324 after 60, 1.328 over 100 timed steps); reported in config.preheat_steps
 PEAK = {"bf16": (2500.0, "dense bf16 MFMA peak, MI355X_MICROARCH.md chip table"),
-        "fp32": (157.3, "f32 matrix peak, MI355X_MICROARCH.md chip table")}
+        "fp32": (157.3, "f32 matrix peak, MI355X_MICROARCH.md chip table"),
+        "fp8": (5000.0, "dense 8-bit MFMA peak, twice the bf16 one")}
 
 
 def cpu_baseline(config, shapes, seconds=10.0):
@@ -77,7 +78,7 @@ def stage_roofline(stages_ms, config, B, L, R, precision):
     """Per stage: algorithmic GFLOP and MB per step, the roofline that bounds it and the fraction
     of that roofline the measured time reaches.  Bytes count each activation tensor once in and once out."""
     depth, ch, ks, ccat = config
-    esz = 2 if precision == "bf16" else 4
+    esz = 4 if precision == "fp32" else 2        # ("fp8": block outputs are one byte, the rest of the path two)
     c0 = ch[0]
     w = [ch[i + 1] // 8 for i in range(depth)]
     mid = [8 * x for x in w]
@@ -93,12 +94,13 @@ def stage_roofline(stages_ms, config, B, L, R, precision):
         "pool_linear1": (2.0 * R * ccat * 128, (ccat + 128.0) * R * esz),
         "pool_stats": (2.0 * R * 128 * ccat, (ccat + 128.0) * R * esz),
     }
-    peak_tf = PEAK[precision][0]
     out = {}
     for name, (flops, nbytes) in work.items():
         ms = stages_ms.get(name)
         if not ms:
             continue
+        # "fp8": catconv in 8 bits (and most first convs; priced at the 16-bit peak here), every other product in 16
+        peak_tf = PEAK["bf16" if precision == "fp8" and name != "catconv" else precision][0]
         t_mfma, t_hbm = flops / (peak_tf * 1e12), nbytes / (HBM_PEAK_GBS * 1e9)
         bound = "mfma" if t_mfma > t_hbm else "hbm"
         out[name] = {"ms": ms, "gflop": round(flops / 1e9, 2), "mbytes": round(nbytes / 1e6, 1), "bound": bound,
@@ -113,7 +115,7 @@ def main():
     ap.add_argument("--steps", type=int, default=20)
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--workload", default="base256", choices=sorted(WORKLOADS))
-    ap.add_argument("--precision", default="bf16", choices=["bf16", "fp32"])
+    ap.add_argument("--precision", default="bf16", choices=["bf16", "fp32", "fp8"])
     ap.add_argument("--global-batch", type=int, default=None,
                     help="strong scaling: ONE batch of this many utterances split evenly over the ranks (per-GPU batch = "
                          "G / N); default for --workload largest / base: 512 / 256.  Without it the per-GPU batch is "
@@ -339,6 +341,7 @@ def main():
                        "weights": "deterministic synthetic (sugar_amd/synth.py)"},
             "roofline": {"kernel": "%s catconv launch [%d frames x K %d -> %d]"
                                    % ("gemm1x1_persist_kernel (256x256x64 LDS-DMA MFMA GEMM, quadrant ping-pong schedule, persistent split-tail grid)" if args.precision == "bf16"
+                                      else "fp8_linear_persist_kernel (256x256x128 block-scaled 8-bit product, persistent)" if args.precision == "fp8"
                                       else "conv_gemm_kernel<float,128,128>", R, depth * ch[0], ccat),
                          "bound": "mfma", "achieved": round(achieved, 2) if achieved else None, "peak": peak,
                          "unit": "TFLOP/s", "frac": round(achieved / peak, 4) if achieved else None,

@@ -18,6 +18,7 @@ enum { NORM_NONE = SUGAR_NORM_NONE, NORM_AFFINE = SUGAR_NORM_AFFINE, NORM_RMS = 
 
 struct JoinArgs {
   SugarBlockJoin j;
+  int run;                   // consecutive rows a wave (WPR = 1) or workgroup takes
   int e_bytes;               // exponent bytes of a row that are written (the blocks, and padding where the row is an operand of its own)
 };
 
@@ -83,24 +84,25 @@ struct Raw8 {
 
 // weight and bias of a norm for this lane's channels: 1 and 0 where there is no vector, 0 past the row (so that what a
 // norm leaves there is 0)
-template <int NCH, int WPR>
+template <int NCH, int WPR, bool VEC>
 struct NormVec {
   float w[NCH][8], b[NCH][8];
   __device__ __forceinline__ void load(const float* __restrict__ pw, const float* __restrict__ pb, int cw, int C) {
 #pragma unroll
-    for (int k = 0; k < NCH; ++k)
+    for (int k = 0; k < NCH; ++k) {
+      const int c = cw + k * (512 * WPR);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int c = cw + k * (512 * WPR) + i, cc = c < C ? c : C - 1;
-        w[k][i] = c < C ? (pw ? pw[cc] : 1.f) : 0.f;
-        b[k][i] = c < C && pb ? pb[cc] : 0.f;
-      }
+      for (int i = 0; i < 8; ++i) { w[k][i] = c + i < C ? 1.f : 0.f; b[k][i] = 0.f; }
+      Raw8<float, VEC> t;
+      if (pw) { t.load(pw, c, C); t.get(w[k], c, C); }
+      if (pb) { t.load(pb, c, C); t.get(b[k], c, C); }
+    }
   }
 };
 
 // x <- norm(x) over the row's C channels; lanes past the row hold zeros before and after.
 template <int NCH, int WPR, bool VEC>
-__device__ __forceinline__ void row_norm(float (&x)[NCH][8], int kind, const NormVec<NCH, WPR>& p, float eps, int C, float inv_c, int cw,
+__device__ __forceinline__ void row_norm(float (&x)[NCH][8], int kind, const NormVec<NCH, WPR, VEC>& p, float eps, int C, float inv_c, int cw,
                                          float* red, int wv) {
   if (kind == NORM_NONE) return;
   float mean = 0.f, mul = 1.f;
@@ -134,7 +136,7 @@ __device__ __forceinline__ void row_norm(float (&x)[NCH][8], int kind, const Nor
 }
 
 // NCH x 8 channels a lane, WPR waves a row.  Each wave (WPR = 1; else each workgroup) takes a run of consecutive rows.
-template <typename TU, typename TS, int NCH, int WPR, bool VEC>
+template <typename TU, typename TS, int NCH, int WPR, bool VEC, bool NORMS>
 __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void block_join_kernel(JoinArgs a) {
   __shared__ float red[WPR > 1 ? WPR : 1];
   const SugarBlockJoin& j = a.j;
@@ -142,25 +144,25 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void block_join_kernel(Jo
   const int C = j.cols;
   const int cw = (WPR > 1 ? wv * 512 : 0) + lane * 8;          // first channel of this lane's chunk 0
   const float inv_c = 1.0f / (float)C;
-  constexpr int RPB = WPR > 1 ? 1 : 4;                         // rows a workgroup holds
-  const int64_t per = (j.rows + (int64_t)gridDim.x * RPB - 1) / ((int64_t)gridDim.x * RPB);
-  const int64_t first = ((int64_t)blockIdx.x * RPB + (WPR > 1 ? 0 : __builtin_amdgcn_readfirstlane(wv))) * per;
-  const int64_t last = first + per < j.rows ? first + per : j.rows;
+  constexpr int RPB = WPR > 1 ? 1 : 4;                         // runs of rows a workgroup takes
+  const int64_t first = ((int64_t)blockIdx.x * RPB + (WPR > 1 ? 0 : __builtin_amdgcn_readfirstlane(wv))) * a.run;
+  const int64_t last = first + a.run < j.rows ? first + a.run : j.rows;
   if (first >= last) return;
   int b = 0, b_end = 0, begin = 0;
-  if (j.d_row_off) {                                           // last utterance that begins at or before the first row
-    int lo = 0, hi = j.n_utts;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (j.d_row_off[mid] <= first) lo = mid; else hi = mid;
+  if (j.d_row_off) {                                           // last utterance that begins at or before the first row: 64-ary search
+    for (int n = j.n_utts; n > 1;) {
+      const int step = (n + 63) >> 6, i = lane * step;
+      const bool le = i < n && j.d_row_off[b + i] <= first;
+      const int k = max((int)__popcll(__ballot(le)) - 1, 0) * step;
+      b += k;
+      n = min(step, n - k);
     }
-    b = lo;
     b_end = j.d_row_off[b + 1];
     begin = j.d_row_off[0];
   }
-  NormVec<NCH, WPR> post, pre;                                 // in registers over the rows
-  if (j.post_kind) post.load(j.d_post_w, j.d_post_b, cw, C);
-  if (j.pre_kind) pre.load(j.d_pre_w, j.d_pre_b, cw, C);
+  NormVec<NCH, WPR, VEC> post, pre;                                 // in registers over the rows
+  if (NORMS && j.post_kind) post.load(j.d_post_w, j.d_post_b, cw, C);
+  if (NORMS && j.pre_kind) pre.load(j.d_pre_w, j.d_pre_b, cw, C);
   for (int64_t r = first; r < last; ++r) {
     if (j.d_row_off) {
       while (r >= b_end && b + 1 < j.n_utts) { ++b; b_end = j.d_row_off[b + 1]; }
@@ -184,7 +186,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void block_join_kernel(Jo
     float v[NCH][8], s[NCH][8];
 #pragma unroll
     for (int k = 0; k < NCH; ++k) ru[k].get(v[k], cw + k * (512 * WPR), C);
-    row_norm<NCH, WPR, VEC>(v, j.post_kind, post, j.post_eps, C, inv_c, cw, red, wv);
+    if (NORMS) row_norm<NCH, WPR, VEC>(v, j.post_kind, post, j.post_eps, C, inv_c, cw, red, wv);
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       const int c = cw + k * (512 * WPR);
@@ -206,7 +208,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void block_join_kernel(Jo
       if (j.d_stream) store8((TS*)j.d_stream + r * j.lds, c, C, VEC, st);
     }
     if (!j.d_z && !j.d_q) continue;
-    row_norm<NCH, WPR, VEC>(s, j.pre_kind, pre, j.pre_eps, C, inv_c, cw, red, wv);
+    if (NORMS) row_norm<NCH, WPR, VEC>(s, j.pre_kind, pre, j.pre_eps, C, inv_c, cw, red, wv);
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       const int c = cw + k * (512 * WPR);
@@ -231,12 +233,19 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void block_join_kernel(Jo
 }
 
 template <typename TU, typename TS, int NCH, int WPR>
-int launch_join(const JoinArgs& a, bool vec, int n_cu, hipStream_t s) {
+int launch_join(JoinArgs a, bool vec, int n_cu, hipStream_t s) {
   constexpr int threads = WPR > 4 ? 64 * WPR : 256;
-  const int64_t want = ceil_div(a.j.rows, WPR > 1 ? 1 : 4), most = 2048ll / threads * n_cu;
-  const unsigned grid = (unsigned)(want < most ? want : most);
-  if (vec) hipLaunchKernelGGL((block_join_kernel<TU, TS, NCH, WPR, true>), dim3(grid), dim3(threads), 0, s, a);
-  else hipLaunchKernelGGL((block_join_kernel<TU, TS, NCH, WPR, false>), dim3(grid), dim3(threads), 0, s, a);
+  // Rows a wave (workgroup) takes one after the other.  Many rows: without norms 2 (77 056 x 512 with 8-bit output: 56 / 50 /
+  // 52 / 55 us for 1 / 2 / 4 / 8), with norms enough to share the fetch of their vectors (92 / 70 / 60 / 61 us; 48 611 x
+  // 1024 layer / layer into a 32-bit stream 128 / 118 / 123 / 124; 40 000 x 2048, a workgroup a row, 180 / 143 / 130 / 126).
+  // Few rows: spread over the chip first (301 x 512 4.0 / 4.8 / 6.8 us, 1204 x 1024 by workgroups 8.5 / 8.1 / 10.7).
+  const bool norms = a.j.post_kind || a.j.pre_kind;
+  const int64_t most = WPR > 1 ? 8 : !norms || NCH > 1 || sizeof(TU) == 4 ? 2 : 4, share = a.j.rows / (8ll * n_cu * (WPR > 1 ? 1 : 4));
+  a.run = (int)(share < 1 ? 1 : share < most ? share : most);
+  const dim3 grid((unsigned)ceil_div(a.j.rows, (int64_t)a.run * (WPR > 1 ? 1 : 4)));
+  if (vec && norms) hipLaunchKernelGGL((block_join_kernel<TU, TS, NCH, WPR, true, true>), grid, dim3(threads), 0, s, a);
+  else if (vec) hipLaunchKernelGGL((block_join_kernel<TU, TS, NCH, WPR, true, false>), grid, dim3(threads), 0, s, a);
+  else hipLaunchKernelGGL((block_join_kernel<TU, TS, NCH, WPR, false, true>), grid, dim3(threads), 0, s, a);
   SUGAR_LAUNCH_CHECK();
   return SUGAR_OK;
 }
@@ -265,6 +274,7 @@ int launch_block_join(const SugarBlockJoin& j, bool pad_exponents, hipStream_t s
   // one path for rows that are all 16-byte aligned in whole chunks of 8 channels, one for everything else
   const bool vec = rows_vec(j.d_u, j.ldu, j.cols, eu) && rows_vec(j.d_residual, j.ldr, j.cols, es) &&
                    (!j.d_stream || rows_vec(j.d_stream, j.lds, j.cols, es)) && (!j.d_z || rows_vec(j.d_z, j.ldz, j.cols, ez)) &&
+                   !(((uintptr_t)j.d_post_w | (uintptr_t)j.d_post_b | (uintptr_t)j.d_pre_w | (uintptr_t)j.d_pre_b) & 15) &&
                    (!j.d_gate || rows_vec(j.d_gate, j.gate_kind == SUGAR_GATE_CHANNEL ? j.cols : j.ldg, j.cols, eg));
   if (j.u_dtype == SUGAR_F32) return launch_join_t<float, float>(a, vec, s);
   return j.stream_dtype == SUGAR_F32 ? launch_join_t<bf16, float>(a, vec, s) : launch_join_t<bf16, bf16>(a, vec, s);
