@@ -299,6 +299,164 @@ int launch_tile(LinearArgs p, hipStream_t s) {
   return SUGAR_OK;
 }
 
+// ------------------------------------------------------------------------------------------ weights in registers, many rows
+// A tile kernel stages both operands of every tile (77 056 x 512 x 512 in 128 x 128 tiles: 315 MB through LDS for 118 MB of
+// tensors), and at K <= 512 that DMA bounds it.  Here the WEIGHTS stay: a workgroup owns a slab of 256 channels, each of its
+// 8 waves the fragments of 32 of them for the whole of K in registers (16 KB a lane), and walks a run of rows in tiles of
+// 64.  Only rows move, once per slab, through a ring of LDS stages ([64 rows][128 bytes] per block) that runs on across
+// tiles; one barrier a tile.  Row i of a wave's 16-channel tile m is channel 8 (i / 4) + 4 m + i % 4 of its 32 (wreg_row), so
+// that a lane's 8 results of a row are neighbours: one 16-byte store straight from the accumulators.
+// 77 056 x 512 -> 512: 30 us (3.9 TB/s; 128 x 128 tiles 33), of which the rows beyond the first take 0.27 ns each (5.7 TB/s)
+// and the launch, the weights' way into registers and the first tile 9 us.  Longer K the same way (4 waves of up to 64
+// channels with 512 registers each) was built and dropped: 77 056 x 1536 -> 1536 271 us against 178 of the persistent kernel;
+// a lone wave per SIMD does not hide the moves between its two register halves.
+struct RowRun { int begin, end, slab; };                          // rows of a workgroup
+
+// Workgroups b and b + 8 (one XCD) take the slabs of one run of rows: all but the first read of a row hit L2.  Runs in units
+// of 16 rows, as even as they go; a run's last tile may be partly the next run's (or nobody's) rows.
+__device__ __forceinline__ RowRun row_run(int rows, int n_slabs, int runs) {
+  const int b = blockIdx.x, xcd = b & 7, jj = b >> 3, run = xcd + 8 * (jj / n_slabs);
+  const int units = (rows + 15) >> 4, q = units / runs, rem = units % runs;
+  RowRun r;
+  r.slab = jj % n_slabs;
+  r.begin = 16 * (run * q + min(run, rem));
+  r.end = min(rows, r.begin + 16 * (q + (run < rem)));
+  return r;
+}
+
+template <int KB>
+struct Short {
+  static constexpr int SLAB = 256, NS = KB == 4 ? 4 : KB == 3 ? 5 : KB == 2 ? 6 : 8, STAGE = KB * 8192;
+  static constexpr int LDS = NS * (STAGE + 256);
+};
+
+template <int KB>
+__global__ __launch_bounds__(512, 2) void fp8_linear_short_kernel(LinearArgs p, int n_slabs, int runs) {
+  typedef Short<KB> C;
+  constexpr int NS = C::NS, D = NS - 1, NST = 4;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  unsigned* exps = (unsigned*)(smem + NS * C::STAGE);             // [NS][64]
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fq = lane >> 4;
+  const RowRun run = row_run(p.rows, n_slabs, runs);
+  const int nt = (run.end - run.begin + 63) >> 6;
+  if (nt <= 0) return;                                            // (whole workgroups: no barrier is missed)
+  const int co = run.slab * C::SLAB + wv * 32;
+
+  const int row = wv * 8 + (lane >> 3);                           // DMA: wave wv fills rows 8 wv .. 8 wv + 7 of each block
+  const unsigned coff = ((lane & 7) ^ ((row >> 1) & 7)) << 4;
+  auto stage = [&](int t) {
+    const int slot = t % NS, base = run.begin + t * 64;
+    if (wv == 0) dma<4>(p.ae, (unsigned)min(base + lane, p.rows - 1) * p.ldae, (unsigned char*)(exps + slot * 64));
+    const unsigned off = (unsigned)min(base + row, p.rows - 1) * p.lda + coff;
+#pragma unroll
+    for (int k = 0; k < KB; ++k) dma<16>(p.a + k * 128, off, smem + slot * C::STAGE + k * 8192 + wv * 1024);
+  };
+#pragma unroll
+  for (int t = 0; t < D; ++t)
+    if (t < nt) stage(t);
+
+  i32x8 wf[KB][2];
+  int ew[2];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const unsigned wr = (unsigned)min(co + wreg_row(m, fr), p.n - 1);
+    ew[m] = *(const int*)(p.we + wr * p.ldwe);
+#pragma unroll
+    for (int k = 0; k < KB; ++k) {
+      const uint8_t* src = p.w + wr * p.ldw + k * 128 + fq * 16;
+      *(i32x4*)&wf[k][m] = *(const i32x4*)src;
+      *((i32x4*)&wf[k][m] + 1) = *(const i32x4*)(src + 64);
+    }
+  }
+  const bool relu = p.flags & EPI_RELU, affine = p.flags & EPI_AFFINE;
+  const int cl = co + 8 * fq;
+  float sc[8], sh[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) { sc[i] = 1.f; sh[i] = 0.f; }
+  if (affine) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      sc[i] = p.scale[min(cl + i, p.n - 1)];
+      sh[i] = p.shift[min(cl + i, p.n - 1)];
+    }
+  }
+  // Every tile but a run's last stores all its rows; where this wave's channels are all inside too, D tiles' stores (and KB
+  // x (D - 1) rows' DMA) are younger than the DMA that is waited for.
+  const bool counted = co + 32 <= p.n && !p.y2;
+  for (int t = 0; t < nt; ++t) {
+    if (t + D - 1 < nt) {
+      if (counted && t >= D) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * KB + D * NST) : "memory");
+      else asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * KB) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // tile t is there, tile t - 1 has been read
+    if (t + D < nt) stage(t + D);
+    const unsigned char* xb = smem + (t % NS) * C::STAGE;
+    int ex[4];
+    f32x4 acc[2][4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      ex[n] = exps[(t % NS) * 64 + n * 16 + fr];
+      acc[0][n] = acc[1][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int k = 0; k < KB; ++k) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const i32x8 xf = frag(xb + k * 8192, n * 16 + fr, fq);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          if (k == 0) acc[m][n] = mfma_fp8<0, 0>(wf[k][m], xf, acc[m][n], ew[m], ex[n]);
+          if (k == 1) acc[m][n] = mfma_fp8<1, 1>(wf[k][m], xf, acc[m][n], ew[m], ex[n]);
+          if (k == 2) acc[m][n] = mfma_fp8<2, 2>(wf[k][m], xf, acc[m][n], ew[m], ex[n]);
+          if (k == 3) acc[m][n] = mfma_fp8<3, 3>(wf[k][m], xf, acc[m][n], ew[m], ex[n]);
+        }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = acc[i >> 2][n][i & 3];
+        if (relu) v[i] = relu_nan(v[i]);
+        if (affine) v[i] = fmaf(v[i], sc[i], sh[i]);
+      }
+      const int r = run.begin + t * 64 + n * 16 + fr;
+      if (r < run.end && cl < p.n) {
+        bf16x8 o;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = (bf16)v[i];
+        *(bf16x8*)((bf16*)p.y + (int64_t)r * p.ldy + cl) = o;
+        if (p.y2 && cl >= p.y2_from) *(bf16x8*)(p.y2 + (int64_t)r * p.ldy2 + cl) = o;
+      }
+    }
+  }
+}
+
+template <int KB>
+int launch_short(const LinearArgs& p, int n_cu, hipStream_t s) {
+  typedef Short<KB> C;
+  static OptInMask opted{0};
+  if (int rc = lds_opt_in((const void*)fp8_linear_short_kernel<KB>, C::LDS, &opted)) return rc;
+  const int n_slabs = (int)ceil_div(p.n, C::SLAB);
+  int runs = n_cu / n_slabs / 8 * 8;
+  if (runs < 8) runs = 8;
+  hipLaunchKernelGGL(fp8_linear_short_kernel<KB>, dim3((unsigned)(n_slabs * runs)), dim3(512), C::LDS, s, p, n_slabs, runs);
+  SUGAR_LAUNCH_CHECK();
+  return SUGAR_OK;
+}
+
+int launch_short(const LinearArgs& p, int n_cu, hipStream_t s) {
+  switch (p.kb) {
+    case 1: return launch_short<1>(p, n_cu, s);
+    case 2: return launch_short<2>(p, n_cu, s);
+    case 3: return launch_short<3>(p, n_cu, s);
+    default: return launch_short<4>(p, n_cu, s);
+  }
+}
+
 // ------------------------------------------------------------------------------------------ persistent 256 x 256 tiles
 // One workgroup per CU walks its tiles; the schedule is that of gemm_tiles_persist (conv1x1.hip, two phases a k-tile):
 //   phase 1   reads b0, a0, b1 | barrier | a0 x b0, a0 x b1      DMA: weights of the next k-tile
@@ -562,8 +720,11 @@ int launch_rows(const LinearArgs& p, hipStream_t s) {
   //   4816 x 1536 -> 1536   -   | 21.8 | 20.0 | 16.4       19264 x 528 -> 536    -   | 16.2 | 14.0 | 13.4
   //   77056 x 512 -> 512    -   | 43  | 35   | 31.5 | 31.9   77056 x 768 -> 768      61.3 | 65.8 (the last two)
   //   77056 x 1152 -> 1152  125.9 | 118.6                    77056 x 1536 -> 1536    231.9 | 180.8
+  // weights in registers | 128 x 128:  77056 x 512 -> 512 29.9 | 33.9, -> 1024 49.4 | 59.1, -> 256 21.3 | 20.2;
+  //   77056 x 384 -> 384 24.9 | 22.8;  77056 x 128 -> 512 18.3 | 19.6;  38528 x 512 -> 512 19.8 | 19.3
   // so: direct while its workgroups (each streams its 16 channels' weights once per 16 rows) are at most two a CU, the
-  // larger tile once it fills the CUs, the persistent kernel where k-loops are long enough to hide its epilogue and two
+  // larger tile once it fills the CUs, weights in registers for K <= 512 where two slabs or more are three quarters full and
+  // walk rows enough to pay for their fetch, the persistent kernel where k-loops are long enough to hide its epilogue and two
   // rounds of tiles or more are there.
   const bool f32 = p.out_f32;
   if (ceil_div(p.n, 16) * ceil_div(p.rows, 16) <= 2ll * n_cu) {
@@ -574,6 +735,9 @@ int launch_rows(const LinearArgs& p, hipStream_t s) {
     SUGAR_LAUNCH_CHECK();
     return SUGAR_OK;
   }
+  const int64_t slabs = ceil_div(p.n, 256);
+  if (!f32 && p.vec && p.kb <= 4 && n_cu % 8 == 0 && slabs >= 2 && 4ll * p.n >= 3 * 256 * slabs && p.rows * slabs >= 400ll * n_cu)
+    return launch_short(p, n_cu, s);
   if (!f32 && p.vec && !p.y2 && p.kb >= 8 && n_cu % 8 == 0 && ceil_div(p.n, 256) * ceil_div(p.rows, 256) >= 2 * n_cu)
     return launch_persist(p, n_cu, s);
   if (ceil_div(p.n, 128) * ceil_div(p.rows, 128) >= n_cu)

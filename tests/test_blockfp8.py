@@ -579,6 +579,17 @@ def test_results_do_not_depend_on_the_other_rows():
 def test_linear_persistent_tiles(r, n, k):
     """Products of two rounds of 256 x 256 tiles and more: odd numbers of k-tiles, channels and rows that end inside a tile,
     one tile of channels, tails; with and without the affine vectors, and rows around the output left alone."""
+    check_many_rows(r, n, k)
+
+
+@gpu
+@pytest.mark.parametrize("r,n,k", [(60000, 512, 512), (35001, 776, 384), (52007, 456, 100), (52016, 1000, 200)])
+def test_linear_weights_in_registers(r, n, k):
+    """Products of up to 4 blocks over many rows: every number of blocks, slabs that are not full, runs of uneven length."""
+    check_many_rows(r, n, k)
+
+
+def check_many_rows(r, n, k):
     a, w = operands(r, r, n, k)
     s, t = rows_of(8, 1, n)[0].cuda(), rows_of(9, 1, n)[0].cuda()
     out = torch.full((r + 2, n + 8), 7.0, dtype=torch.bfloat16, device="cuda")
