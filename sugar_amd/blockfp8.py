@@ -20,7 +20,7 @@ import torch
 from . import _lib
 
 _DT = {torch.float32: _lib.SUGAR_F32, torch.bfloat16: _lib.SUGAR_BF16}
-NORMS = {None: 0, "affine": 1, "rms": 2, "layer": 3}
+NORMS = {"affine": 1, "rms": 2, "layer": 3}
 MAX_JOIN_COLS = 8192
 _raw_stream = torch._C._cuda_getCurrentRawStream       # (torch.cuda.current_stream builds an object, 1 us of a 10 us call)
 _FN = {}
@@ -30,18 +30,21 @@ def _up(v, m):
     return (v + m - 1) // m * m
 
 
-def _same_device(tensors):
-    """The device all of them are on (a GPU), none of them part of a recorded gradient."""
-    dev = tensors[0].device
+def _gpu(dev):
+    if dev.type != "cuda":
+        raise _lib.SugarError("sugar_amd runs on an MI355X only: tensors must be CUDA tensors (no CPU fallback)")
+    return dev
+
+
+def _same_device(dev, tensors):
+    """All on `dev` (a GPU), none of them part of a recorded gradient."""
+    _gpu(dev)
     grad = torch.is_grad_enabled()
     for t in tensors:
-        if not t.is_cuda:
-            raise _lib.SugarError("sugar_amd runs on an MI355X only: tensors must be CUDA tensors (no CPU fallback)")
         if t.device != dev:
             raise ValueError("tensors on %s and %s" % (dev, t.device))
         if grad and t.requires_grad:
             raise ValueError("no backward pass: call under torch.no_grad() or detach the inputs")
-    return dev
 
 
 def _call(dev, name, *args):
@@ -95,6 +98,31 @@ def _out(what, out, shape, dtypes, dev):
     return ld
 
 
+def _memory(t, ld=None):
+    """(first byte, bytes of a row, bytes from row to row, rows) of a matrix, vector or BlockFP8 part."""
+    if t.dim() == 1:
+        return t.data_ptr(), t.shape[0] * t.element_size(), 0, 1
+    size = t.element_size()
+    return t.data_ptr(), t.shape[1] * size, (_row_stride(t) if ld is None else ld) * size, t.shape[0]
+
+
+def _apart(what, out, others, same=()):
+    """An output passed in must not share memory with what a call reads or writes besides it, except be one of `same`
+    itself (same first element and strides).  Column slices of one buffer are apart."""
+    p, width, step, rows = _memory(out)
+    for t in others:
+        q, w, st, r = _memory(t)
+        if not rows or not r or p >= q + (r - 1) * st + w or q >= p + (rows - 1) * step + width:
+            continue
+        if st == step and step:
+            off = (q - p) % step
+            if off >= width and off + w <= step:
+                continue
+        if any(t is x for x in same) and p == q and step == st and t.dtype == out.dtype:
+            continue
+        raise ValueError("%s: the output shares memory with another operand" % what)
+
+
 def _vector(what, v, n):
     """A contiguous float32 vector of n (other float types and strides are converted)."""
     if v.dim() != 1 or v.shape[0] != n or not v.dtype.is_floating_point:
@@ -110,7 +138,7 @@ class BlockFP8(object):
     Row slices (`x[10:20]`) share the memory.  `BlockFP8(data, exponent, cols)` takes existing tensors as they are.
     """
     BLOCK = 128
-    __slots__ = ("_data", "_exponent", "cols", "_ld", "_lde")
+    __slots__ = ("_data", "_exponent", "_buf", "rows", "cols", "_ld", "_lde")
 
     def __init__(self, data, exponent, cols):
         cols = int(cols)
@@ -128,56 +156,69 @@ class BlockFP8(object):
         ld, lde = _row_stride(data), _row_stride(exponent)
         if ld is None or lde is None or ld % 16 or lde % 4 or data.data_ptr() % 16 or exponent.data_ptr() % 4:
             raise ValueError("BlockFP8: contiguous columns, data rows 16-byte aligned, exponent rows 4-byte aligned")
-        self._data, self._exponent, self.cols, self._ld, self._lde = data, exponent, cols, ld, lde
+        self._data, self._exponent, self._buf = data, exponent, None
+        self.rows, self.cols, self._ld, self._lde = data.shape[0], cols, ld, lde
 
     @classmethod
     def empty(cls, rows, cols, device):
+        """An operand to be written into: one allocation, values and exponents one behind the other."""
         self = cls.__new__(cls)
         blocks = -(-int(cols) // cls.BLOCK)
-        self.cols, self._ld, self._lde = int(cols), blocks * cls.BLOCK, _up(blocks, 4)
-        self._data = torch.empty((rows, self._ld), dtype=torch.float8_e4m3fn, device=device)
-        self._exponent = torch.empty((rows, self._lde), dtype=torch.uint8, device=device)
+        self.rows, self.cols, self._ld, self._lde = int(rows), int(cols), blocks * cls.BLOCK, _up(blocks, 4)
+        self._buf = torch.empty(self.rows * (self._ld + self._lde), dtype=torch.uint8, device=device)
+        self._data = self._exponent = None
         return self
+
+    def _pointers(self):
+        if self._buf is None:
+            return self._data.data_ptr(), self._exponent.data_ptr()
+        p = self._buf.data_ptr()
+        return p, p + self.rows * self._ld
+
+    def _split(self):
+        n = self.rows * self._ld
+        self._data = self._buf[:n].view(torch.float8_e4m3fn).view(self.rows, self._ld)
+        self._exponent = self._buf[n:].view(self.rows, self._lde)
 
     @property
     def data(self):
+        if self._data is None:
+            self._split()
         return self._data
 
     @property
     def exponent(self):
+        if self._exponent is None:
+            self._split()
         return self._exponent
 
     @property
-    def rows(self):
-        return self._data.shape[0]
+    def device(self):
+        return (self._data if self._buf is None else self._buf).device
 
     @property
     def shape(self):
-        return torch.Size((self._data.shape[0], self.cols))
-
-    @property
-    def device(self):
-        return self._data.device
+        return torch.Size((self.rows, self.cols))
 
     def __getitem__(self, rows):
         if not isinstance(rows, slice) or rows.step not in (None, 1):
             raise ValueError("BlockFP8: only slices of consecutive rows")
-        return BlockFP8(self._data[rows], self._exponent[rows], self.cols)
+        return BlockFP8(self.data[rows], self.exponent[rows], self.cols)
 
     def dequantize(self, dtype=torch.float32, out=None):
         """The values, [rows, cols] float32 or bfloat16 (exact in both)."""
-        data, exponent, cols = self._data, self._exponent, self.cols
-        dev = _same_device((data, exponent))
-        rows = data.shape[0]
+        rows, cols = self.rows, self.cols
+        dev = _gpu(self.device)
         if out is None:
             if dtype not in _DT:
                 raise ValueError("dequantize: dtype %s not in %s" % (dtype, [str(d) for d in _DT]))
             out, ld = torch.empty((rows, cols), dtype=dtype, device=dev), cols
         else:
             ld = _out("dequantize", out, (rows, cols), _DT, dev)
+            _apart("dequantize", out, (self.data, self.exponent))
         if rows:
-            _call(dev, "sugar_fp8_dequant", data.data_ptr(), self._ld, exponent.data_ptr(), self._lde, rows, cols,
-                  out.data_ptr(), ld, _DT[out.dtype])
+            d, e = self._pointers()
+            _call(dev, "sugar_fp8_dequant", d, self._ld, e, self._lde, rows, cols, out.data_ptr(), ld, _DT[out.dtype])
         return out
 
 
@@ -196,12 +237,15 @@ def quantize_block_fp8(x, out=None):
     become NaN and do not move the scale of their block.
     """
     x, ld = _rows("quantize_block_fp8", x)
-    dev = _same_device((x,))
+    dev = x.device
+    _same_device(dev, (x,))
     rows, cols = x.shape
     q = _fp8_out("quantize_block_fp8", out, rows, cols, dev)
+    if out is not None:
+        _apart("quantize_block_fp8", x, (q.data, q.exponent))
     if rows:
-        _call(dev, "sugar_fp8_quant", x.data_ptr(), ld, _DT[x.dtype], rows, cols, q._data.data_ptr(), q._ld,
-              q._exponent.data_ptr(), q._lde)
+        d, e = q._pointers()
+        _call(dev, "sugar_fp8_quant", x.data_ptr(), ld, _DT[x.dtype], rows, cols, d, q._ld, e, q._lde)
     return q
 
 
@@ -214,36 +258,58 @@ def block_fp8_linear(a, w, scale=None, shift=None, relu=False, out_dtype=torch.b
     """
     if not isinstance(a, BlockFP8) or not isinstance(w, BlockFP8):
         raise ValueError("block_fp8_linear: operands must be BlockFP8 (quantize_block_fp8)")
-    rows, n, k = a._data.shape[0], w._data.shape[0], a.cols
+    rows, n, k = a.rows, w.rows, a.cols
     if k != w.cols:
         raise ValueError("block_fp8_linear: a has %d columns, w %d" % (k, w.cols))
     if n == 0:
         raise ValueError("block_fp8_linear: w has no rows")
-    flags = _lib.EPI_RELU if relu else 0
-    if scale is None and shift is None:
-        dev = _same_device((a._data, w._data))
-    else:
-        dev = _same_device([t for t in (a._data, w._data, scale, shift) if t is not None])
+    dev = a.device
+    if w.device != dev:
+        raise ValueError("tensors on %s and %s" % (dev, w.device))
+    _gpu(dev)
+    flags, sp, tp = _lib.EPI_RELU if relu else 0, None, None
+    if scale is not None or shift is not None:
+        _same_device(dev, [t for t in (scale, shift) if t is not None])
         scale = torch.ones(n, device=dev) if scale is None else _vector("scale", scale, n)
         shift = torch.zeros(n, device=dev) if shift is None else _vector("shift", shift, n)
-        flags |= _lib.EPI_AFFINE
+        flags, sp, tp = flags | _lib.EPI_AFFINE, scale.data_ptr(), shift.data_ptr()
     if out is None:
         if out_dtype not in _DT:
             raise ValueError("block_fp8_linear: out_dtype %s not in %s" % (out_dtype, [str(d) for d in _DT]))
         out, ld = torch.empty((rows, n), dtype=out_dtype, device=dev), n
     else:
         ld = _out("block_fp8_linear", out, (rows, n), _DT, dev)
+        _apart("block_fp8_linear", out, [t for t in (a.data, a.exponent, w.data, w.exponent, scale, shift) if t is not None])
     if rows:
-        _call(dev, "sugar_fp8_linear", a._data.data_ptr(), a._ld, a._exponent.data_ptr(), a._lde, rows, w._data.data_ptr(), w._ld,
-              w._exponent.data_ptr(), w._lde, n, k, scale.data_ptr() if flags & _lib.EPI_AFFINE else None,
-              shift.data_ptr() if flags & _lib.EPI_AFFINE else None, flags, out.data_ptr(), ld, _DT[out.dtype])
+        (ap, aep), (wp, wep) = a._pointers(), w._pointers()
+        _call(dev, "sugar_fp8_linear", ap, a._ld, aep, a._lde, rows, wp, w._ld, wep, w._lde, n, k, sp, tp, flags,
+              out.data_ptr(), ld, _DT[out.dtype])
     return out
 
 
-RowNorm = collections.namedtuple("RowNorm", "kind weight bias eps")
-RowNorm.__new__.__defaults__ = (None, None, 1e-5)
-RowNorm.__doc__ = """A norm over the channels of a row: kind "rms" (x / sqrt(mean x^2 + eps)), "layer" ((x - mean) /
-sqrt(var + eps)) or "affine" (x itself: a folded BatchNorm); times `weight`, plus `bias` (float vectors, or None)."""
+class RowNorm(object):
+    """
+    A norm over the channels of a row: kind "rms" (x / sqrt(mean x^2 + eps)), "layer" ((x - mean) / sqrt(var + eps)) or
+    "affine" (x itself: a folded BatchNorm), times `weight`, plus `bias` (float vectors, or None).  The vectors are used as
+    they are where they are contiguous float32 (later changes in place count), else converted once, here.
+    """
+    __slots__ = ("kind", "weight", "bias", "eps", "code", "cols")
+
+    def __init__(self, kind, weight=None, bias=None, eps=1e-5):
+        if kind not in NORMS:
+            raise ValueError("RowNorm: kind %r not in %s" % (kind, sorted(NORMS)))
+        if not eps >= 0:
+            raise ValueError("RowNorm: negative eps %r" % (eps,))
+        self.kind, self.eps, self.code, self.cols = kind, float(eps), NORMS[kind], None
+        for v in (weight, bias):
+            if v is not None:
+                if v.dim() != 1 or self.cols not in (None, v.shape[0]):
+                    raise ValueError("RowNorm: weight and bias must be vectors of one length, got %s"
+                                     % [None if t is None else tuple(t.shape) for t in (weight, bias)])
+                self.cols = v.shape[0]
+        self.weight = None if weight is None else _vector("RowNorm: weight", weight, self.cols)
+        self.bias = None if bias is None else _vector("RowNorm: bias", bias, self.cols)
+
 
 JoinResult = collections.namedtuple("JoinResult", "stream normed quantized")
 
@@ -260,7 +326,8 @@ def block_join(u, residual, post=None, gate=None, row_off=None, alpha=1.0, dense
     sugar/models/dynamictdnn.py:94-100), or [rows, C] in u's dtype.  Arithmetic is float32, each output is rounded once.
     `dense` is the running sum of DynamicTDNN.forward (:657-660).  Returns (stream, normed, quantized): stream in
     residual's dtype, normed = z in out_dtype (default u's) unless normed=False, quantized = z as BlockFP8 if asked for.
-    Outputs may be passed in; stream_out may be `residual` or `u` itself, normed_out `u` (in place).  With row_off, rows in
+    Outputs may be passed in; stream_out may be `residual` or `u` itself, normed_out `u` (in place), any other shared memory
+    is refused.  With row_off, rows in
     front of the first and behind the last utterance are left as they are (in outputs allocated here: undefined).
     """
     u, ldu = _rows("block_join: u", u)
@@ -272,13 +339,19 @@ def block_join(u, residual, post=None, gate=None, row_off=None, alpha=1.0, dense
         raise ValueError("block_join: %d columns, at most %d" % (cols, MAX_JOIN_COLS))
     if u.dtype == torch.float32 and residual.dtype != torch.float32:
         raise ValueError("block_join: a float32 u needs a float32 residual")
-    inputs = [u, residual]
-    for p in (post, pre):
-        if p is not None:
-            inputs += [t for t in (p.weight, p.bias) if t is not None]
-    inputs += [t for t in (gate, row_off) if t is not None]
-    dev = _same_device(inputs)
-    (post_kind, post_eps, post_w, post_b), (pre_kind, pre_eps, pre_w, pre_b) = _norm("post", post, cols), _norm("pre", pre, cols)
+    dev = u.device
+    inputs = [residual, u]
+    post_kind = pre_kind = post_w = post_b = pre_w = pre_b = 0
+    post_eps = pre_eps = 0.0
+    if post is not None:
+        post_kind, post_eps, post_w, post_b = _norm("post", post, cols, inputs)
+    if pre is not None:
+        pre_kind, pre_eps, pre_w, pre_b = _norm("pre", pre, cols, inputs)
+    if gate is not None:
+        inputs.append(gate)
+    if row_off is not None:
+        inputs.append(row_off)
+    _same_device(dev, inputs)
     utts = 0
     if row_off is not None:
         if row_off.dim() != 1 or row_off.shape[0] < 2 or row_off.dtype != torch.int32:
@@ -299,7 +372,7 @@ def block_join(u, residual, post=None, gate=None, row_off=None, alpha=1.0, dense
             raise ValueError("block_join: gate %s %s is neither [C], [B, C] with row_off, nor [rows, C] of u's dtype without it"
                              % (gate.dtype, tuple(gate.shape)))
     if stream_out is None:
-        stream, lds = torch.empty((rows, cols), dtype=residual.dtype, device=dev), cols
+        stream, lds = _like(residual, residual.dtype, rows, cols, dev), cols
     else:
         stream, lds = stream_out, _out("block_join: stream_out", stream_out, (rows, cols), (residual.dtype,), dev)
     z = q = None
@@ -310,18 +383,24 @@ def block_join(u, residual, post=None, gate=None, row_off=None, alpha=1.0, dense
         out_dtype = u.dtype if out_dtype is None else out_dtype
         if out_dtype not in _DT:
             raise ValueError("block_join: out_dtype %s not in %s" % (out_dtype, [str(t) for t in _DT]))
-        z, ldz = torch.empty((rows, cols), dtype=out_dtype, device=dev), cols
+        z, ldz = _like(u, out_dtype, rows, cols, dev), cols
     if quantized or quantized_out is not None:
         q = _fp8_out("block_join: quantized_out", quantized_out, rows, cols, dev)
+    if stream_out is not None or normed_out is not None or quantized_out is not None:
+        others = [t for t in [u, residual, gate, row_off] + inputs[2:] if t is not None]
+        parts = [] if q is None else [q.data, q.exponent]
+        _apart("block_join: stream_out", stream, others + parts, (residual, u))
+        if z is not None:
+            _apart("block_join: normed_out", z, others + parts + [stream], (u,))
+        for t in parts:
+            _apart("block_join: quantized_out", t, others)
     if rows:
-        p = torch.Tensor.data_ptr
+        q_ptr, e_ptr = (0, 0) if q is None else q._pointers()
         _call(dev, "sugar_block_join", _JOIN.pack(
             rows, cols, utts, _DT[u.dtype], _DT[residual.dtype], 0 if z is None else _DT[z.dtype], post_kind, pre_kind, gate_kind,
             1 if dense else 0, alpha, post_eps, pre_eps, ldu, ldr, ldg, lds, ldz, 0 if q is None else q._ld, 0 if q is None else q._lde,
-            p(u), p(residual), 0 if post_w is None else p(post_w), 0 if post_b is None else p(post_b),
-            0 if pre_w is None else p(pre_w), 0 if pre_b is None else p(pre_b), 0 if gate is None else p(gate),
-            0 if row_off is None else p(row_off), p(stream), 0 if z is None else p(z),
-            0 if q is None else p(q._data), 0 if q is None else p(q._exponent)))
+            u.data_ptr(), residual.data_ptr(), post_w, post_b, pre_w, pre_b, 0 if gate is None else gate.data_ptr(),
+            0 if row_off is None else row_off.data_ptr(), stream.data_ptr(), 0 if z is None else z.data_ptr(), q_ptr, e_ptr))
     return JoinResult(stream, z, q)
 
 
@@ -330,11 +409,20 @@ def block_join(u, residual, post=None, gate=None, row_off=None, alpha=1.0, dense
 _JOIN = struct.Struct("@q9i3f7q12P")
 
 
-def _norm(side, p, cols):
-    """(kind, eps, weight, bias) of a RowNorm or None; the vectors stay referenced until the call has been made."""
-    if p is None:
-        return 0, 0.0, None, None
-    if p.kind is None or p.kind not in NORMS or not p.eps >= 0:
-        raise ValueError("block_join: %s kind %r not in %s, or eps %r negative" % (side, p.kind, [k for k in NORMS if k], p.eps))
-    return (NORMS[p.kind], p.eps, None if p.weight is None else _vector(side + " weight", p.weight, cols),
-            None if p.bias is None else _vector(side + " bias", p.bias, cols))
+def _norm(side, p, cols, inputs):
+    """(kind, eps, weight pointer, bias pointer) of a RowNorm, whose vectors join the inputs to be checked."""
+    if not isinstance(p, RowNorm):
+        raise ValueError("block_join: %s must be a RowNorm, got %r" % (side, p))
+    if p.cols is not None and p.cols != cols:
+        raise ValueError("block_join: the vectors of %s have %d entries, rows %d" % (side, p.cols, cols))
+    w, b = p.weight, p.bias
+    if w is not None:
+        inputs.append(w)
+    if b is not None:
+        inputs.append(b)
+    return p.code, p.eps, 0 if w is None else w.data_ptr(), 0 if b is None else b.data_ptr()
+
+
+def _like(x, dtype, rows, cols, dev):
+    """A new contiguous [rows, cols] (empty_like is the cheaper call)."""
+    return torch.empty_like(x) if x.dtype == dtype and x.is_contiguous() else torch.empty((rows, cols), dtype=dtype, device=dev)

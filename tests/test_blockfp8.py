@@ -482,11 +482,33 @@ def test_join_in_place_strides_and_single_outputs():
     assert torch.equal(got.stream, want.stream) and torch.equal(u2, want.normed)
     assert torch.equal(r2[:, 0], big_r[:, 0]) and torch.equal(r2[:, 201:], big_r[:, 201:])
     for bad in (lambda: block_join(u, res, gate=torch.rand(7, c).cuda()), lambda: block_join(u, res, gate=torch.rand(r, c).cuda()),
-                lambda: block_join(u, res, post=RowNorm("batch")), lambda: block_join(u, res, post=RowNorm("rms", torch.ones(3).cuda())),
+                lambda: block_join(u, res, post=RowNorm("batch")), lambda: block_join(u, res, post="rms"), lambda: block_join(u, res, post=RowNorm("rms", torch.ones(3).cuda())),
                 lambda: block_join(u, res, pre=RowNorm("rms", None, None, -1.0)), lambda: block_join(u, res, out_dtype=torch.float16),
                 lambda: block_join(u, res, row_off=torch.zeros(3).cuda()), lambda: block_join(u, res, stream_out=u2[:5]),
                 lambda: block_join(u, res, gate=torch.rand(c)), lambda: block_join(u, res, quantized_out=stream_like(u2))):
         with pytest.raises((ValueError, _lib.SugarError)):
+            bad()
+
+
+@gpu
+def test_outputs_that_share_memory_are_refused():
+    c, r = 128, 16
+    big = rows_of(1, r, 3 * c, torch.bfloat16).cuda()
+    u, res, out = big[:, :c], big[:, c:2 * c], big[:, 2 * c:]            # columns of one buffer are apart
+    want = block_join(u, res)
+    got = block_join(u, res, stream_out=out)
+    assert torch.equal(got.stream, want.stream) and torch.equal(got.normed, want.normed)
+    flat = torch.zeros(r * c + 8, dtype=torch.bfloat16, device="cuda")
+    x, y = flat[:r * c].view(r, c), flat[8:].view(r, c)
+    q = quantize_block_fp8(x)
+    raw = q.data.view(torch.uint8).view(-1)[:r * 64].view(torch.bfloat16).view(r, 32)
+    for bad in (lambda: block_join(x, x.clone(), stream_out=y), lambda: block_join(x.clone(), x, normed_out=y),
+                lambda: block_join(x.clone(), x, normed_out=x), lambda: block_join(u, res, stream_out=x, normed_out=x),
+                lambda: block_join(x.clone(), x.clone(), stream_out=x, normed_out=y),
+                lambda: block_join(big[:, :c], big[:, c:2 * c], stream_out=big[:, 8:c + 8]),
+                lambda: block_fp8_linear(q, q[:16], out=q.data.view(torch.uint8).view(torch.bfloat16)[:, :16]),
+                lambda: quantize_block_fp8(raw, out=BlockFP8(q.data, q.exponent, 32))):
+        with pytest.raises(ValueError, match="shares memory"):
             bad()
 
 
