@@ -64,44 +64,42 @@ __device__ __forceinline__ u32x2 fp8_pack8(const float* v, float inv) {
   return (u32x2){(unsigned)lo, (unsigned)hi};
 }
 
-// Eight consecutive elements from channel c on; those past `n` (the row's channels) read as 0.  vec: the row is 16-byte
-// aligned and n a multiple of 8, so the eight are all inside or all outside.
+// 16 bytes at the alignment of their elements: rows of odd widths and strides begin anywhere, and the hardware's global
+// loads and stores take any address (one instruction either way).
+typedef bf16x8 bf16x8_u __attribute__((aligned(2)));
+typedef f32x4 f32x4_u __attribute__((aligned(4)));
+typedef u32x4 u32x4_u __attribute__((aligned(2)));
+
+// Eight consecutive elements from channel c on; those past `n` (the row's channels) read as 0.
 template <typename T>
-__device__ __forceinline__ void load8(const T* __restrict__ p, int c, int n, bool vec, float* v) {
+__device__ __forceinline__ void load8(const T* __restrict__ p, int c, int n, float* v) {
+  if (c + 8 <= n) {
+    if constexpr (sizeof(T) == 2) {
+      const bf16x8 t = *(const bf16x8_u*)(p + c);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = 0.f;
-  if (vec) {
-    if (c < n) {
-      if constexpr (sizeof(T) == 2) {
-        const bf16x8 t = *(const bf16x8*)(p + c);
+      for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
+    } else {
+      const f32x4 t0 = *(const f32x4_u*)(p + c), t1 = *(const f32x4_u*)(p + c + 4);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
-      } else {
-        const f32x4 t0 = *(const f32x4*)(p + c), t1 = *(const f32x4*)(p + c + 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { v[i] = t0[i]; v[4 + i] = t1[i]; }
-      }
+      for (int i = 0; i < 4; ++i) { v[i] = t0[i]; v[4 + i] = t1[i]; }
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c + i < n) v[i] = to_f32(p[c + i]);
+    for (int i = 0; i < 8; ++i) v[i] = c + i < n ? to_f32(p[c + i]) : 0.f;
   }
 }
 
 template <typename T>
-__device__ __forceinline__ void store8(T* __restrict__ p, int c, int n, bool vec, const float* v) {
-  if (vec) {
-    if (c < n) {
-      if constexpr (sizeof(T) == 2) {
-        bf16x8 t;
+__device__ __forceinline__ void store8(T* __restrict__ p, int c, int n, const float* v) {
+  if (c + 8 <= n) {
+    if constexpr (sizeof(T) == 2) {
+      bf16x8 t;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) t[i] = (bf16)v[i];
-        *(bf16x8*)(p + c) = t;
-      } else {
-        *(f32x4*)(p + c) = (f32x4){v[0], v[1], v[2], v[3]};
-        *(f32x4*)(p + c + 4) = (f32x4){v[4], v[5], v[6], v[7]};
-      }
+      for (int i = 0; i < 8; ++i) t[i] = (bf16)v[i];
+      *(bf16x8_u*)(p + c) = t;
+    } else {
+      *(f32x4_u*)(p + c) = (f32x4){v[0], v[1], v[2], v[3]};
+      *(f32x4_u*)(p + c + 4) = (f32x4){v[4], v[5], v[6], v[7]};
     }
   } else {
 #pragma unroll
@@ -110,9 +108,15 @@ __device__ __forceinline__ void store8(T* __restrict__ p, int c, int n, bool vec
   }
 }
 
-// rows that load8 / store8 may take 16 bytes at a time
-static inline bool rows_vec(const void* p, int64_t ld, int64_t cols, int esz) {
-  return ((uintptr_t)p & 15) == 0 && (ld * esz) % 16 == 0 && cols % 8 == 0;
+// eight bf16 of a row of n channels from channel c on, as they lie in memory
+__device__ __forceinline__ void store_bf16x8(bf16* __restrict__ y, int c, int n, bf16x8 o) {
+  if (c + 8 <= n) {
+    *(bf16x8_u*)(y + c) = o;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < n) y[c + i] = o[i];
+  }
 }
 
 // ---- products -------------------------------------------------------------------------------------------------------

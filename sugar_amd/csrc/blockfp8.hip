@@ -14,7 +14,7 @@ namespace {
 // 16 lanes own one block of 128 columns, 8 values each: the block's largest magnitude is four DPP steps, no LDS.
 template <typename T>
 __global__ __launch_bounds__(256) void fp8_quant_kernel(const T* __restrict__ x, int64_t ldx, int64_t items, int cols,
-                                                        int blocks, int vec, uint8_t* __restrict__ q, int64_t ldq,
+                                                        int blocks, uint8_t* __restrict__ q, int64_t ldq,
                                                         uint8_t* __restrict__ e, int64_t lde) {
   const int l16 = threadIdx.x & 15;
   const int64_t stride = (int64_t)gridDim.x * 16;
@@ -22,7 +22,7 @@ __global__ __launch_bounds__(256) void fp8_quant_kernel(const T* __restrict__ x,
     const int64_t row = it / blocks;
     const int kb = (int)(it - row * blocks), c = kb * FP8_BLOCK + l16 * 8;
     float v[8];
-    load8(x + row * ldx, c, cols, vec, v);
+    load8(x + row * ldx, c, cols, v);
     unsigned big = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) { const unsigned u = fp8_finite_bits(v[i]); big = u > big ? u : big; }
@@ -36,7 +36,7 @@ __global__ __launch_bounds__(256) void fp8_quant_kernel(const T* __restrict__ x,
 template <typename T>
 __global__ __launch_bounds__(256) void fp8_dequant_kernel(const uint8_t* __restrict__ q, int64_t ldq,
                                                           const uint8_t* __restrict__ e, int64_t lde, int64_t items, int cols,
-                                                          int blocks, int vec, T* __restrict__ y, int64_t ldy) {
+                                                          int blocks, T* __restrict__ y, int64_t ldy) {
   const int l16 = threadIdx.x & 15;
   const int64_t stride = (int64_t)gridDim.x * 16;
   for (int64_t it = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); it < items; it += stride) {
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(256) void fp8_dequant_kernel(const uint8_t* __restr
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = byte == 255 ? __uint_as_float(0x7fc00000u) : __builtin_amdgcn_ldexpf(v[i], byte - 127);
-    store8(y + row * ldy, c, cols, vec, v);
+    store8(y + row * ldy, c, cols, v);
   }
 }
 
@@ -71,14 +71,13 @@ static int check_operand(const char* what, const uint8_t* q, int64_t ldq, const 
 
 int launch_fp8_dequant(const Fp8Operand& a, int64_t rows, int cols, void* d_y, int64_t ldy, int dtype, hipStream_t s) {
   const int64_t items = rows * fp8_blocks(cols);
-  const int vec = rows_vec(d_y, ldy, cols, dtype == SUGAR_F32 ? 4 : 2);
   const unsigned grid = (unsigned)(ceil_div(items, 16) < 65536 ? ceil_div(items, 16) : 65536);
   if (dtype == SUGAR_F32)
     hipLaunchKernelGGL(fp8_dequant_kernel<float>, dim3(grid), dim3(256), 0, s, a.q, a.ldq, a.e, a.lde, items, cols,
-                       (int)fp8_blocks(cols), vec, (float*)d_y, ldy);
+                       (int)fp8_blocks(cols), (float*)d_y, ldy);
   else
     hipLaunchKernelGGL(fp8_dequant_kernel<bf16>, dim3(grid), dim3(256), 0, s, a.q, a.ldq, a.e, a.lde, items, cols,
-                       (int)fp8_blocks(cols), vec, (bf16*)d_y, ldy);
+                       (int)fp8_blocks(cols), (bf16*)d_y, ldy);
   SUGAR_LAUNCH_CHECK();
   return SUGAR_OK;
 }
@@ -151,14 +150,13 @@ int sugar_fp8_quant(const void* d_x, int64_t ldx, int dtype, int64_t rows, int c
   const int esz = dtype == SUGAR_F32 ? 4 : 2;
   SUGAR_CHECK_ARG((uintptr_t)d_x % esz == 0, "fp8_quant: unaligned input");
   const int64_t items = rows * fp8_blocks(cols);
-  const int vec = rows_vec(d_x, ldx, cols, esz);
   const unsigned grid = (unsigned)(ceil_div(items, 16) < 65536 ? ceil_div(items, 16) : 65536);
   if (dtype == SUGAR_F32)
     hipLaunchKernelGGL(fp8_quant_kernel<float>, dim3(grid), dim3(256), 0, (hipStream_t)stream, (const float*)d_x, ldx, items,
-                       cols, (int)fp8_blocks(cols), vec, d_q, ldq, d_e, lde);
+                       cols, (int)fp8_blocks(cols), d_q, ldq, d_e, lde);
   else
     hipLaunchKernelGGL(fp8_quant_kernel<bf16>, dim3(grid), dim3(256), 0, (hipStream_t)stream, (const bf16*)d_x, ldx, items,
-                       cols, (int)fp8_blocks(cols), vec, d_q, ldq, d_e, lde);
+                       cols, (int)fp8_blocks(cols), d_q, ldq, d_e, lde);
   SUGAR_LAUNCH_CHECK();
   return SUGAR_OK;
 }

@@ -21,7 +21,6 @@ struct LinearArgs {
   void* y;
   const float *scale, *shift;
   int rows, n, kb, flags, out_f32;
-  int vec;                            // 16-byte stores: y aligned, n and ldy multiples of 16 bytes
   int n_co_tiles;
   bf16* y2;                           // second store of columns >= y2_from (whole chunks of 8), or nullptr
   int64_t ldy2;
@@ -63,13 +62,13 @@ __device__ __forceinline__ void store_out4(const LinearArgs& p, int64_t r, int c
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = relu_nan(v[i]);
   }
-  if (p.vec && p.out_f32) {
-    if (co >= p.n) return;
+  if (p.out_f32 && co + 4 <= p.n) {
     if (p.flags & EPI_AFFINE) {
+      const f32x4 sc = *(const f32x4_u*)(p.scale + co), sh = *(const f32x4_u*)(p.shift + co);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = fmaf(v[i], p.scale[co + i], p.shift[co + i]);
+      for (int i = 0; i < 4; ++i) v[i] = fmaf(v[i], sc[i], sh[i]);
     }
-    *(f32x4*)((float*)p.y + r * p.ldy + co) = v;
+    *(f32x4_u*)((float*)p.y + r * p.ldy + co) = v;
     return;
   }
 #pragma unroll
@@ -236,7 +235,7 @@ __device__ __forceinline__ void fp8_tile(const LinearArgs& p, const int co_base,
   }
 
   // ---- epilogue: accumulator tile (m, n): lane (fr, fq) holds row wn FW + n 16 + fr, channels wm CW + m 16 + 4 fq + 0..3
-  if (p.out_f32 || !p.vec) {                                     // 16 bytes a lane, 64 in a row (or odd widths)
+  if (p.out_f32) {                                               // 16 bytes a lane, 64 in a row
 #pragma unroll
     for (int n = 0; n < NJ; ++n) {
       const int r = r_base + wn * FW + n * 16 + fr;
@@ -246,7 +245,7 @@ __device__ __forceinline__ void fp8_tile(const LinearArgs& p, const int co_base,
     }
   }
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // stage memory free: epilogue staging, or the caller's next tile
-  if (p.out_f32 || !p.vec) return;
+  if (p.out_f32) return;
   constexpr int EPI_STRIDE = CW * 2 + 16, CPR = CW / 8, RPP = 64 / CPR;
   static_assert(8 * 16 * EPI_STRIDE <= NS * STAGE_BYTES, "epilogue staging fits the stages");
   unsigned char* ep = smem + wv * (16 * EPI_STRIDE);             // this wave's [16 rows][CW channels]
@@ -270,10 +269,10 @@ __device__ __forceinline__ void fp8_tile(const LinearArgs& p, const int co_base,
     for (int i = 0; i < 16 / RPP; ++i) {
       const int f = i * RPP + lane / CPR, ch = lane % CPR;
       const int r = r_base + wn * FW + n * 16 + f, co = co_base + wm * CW + ch * 8;
-      const u32x4 v = *(const u32x4*)(ep + f * EPI_STRIDE + ch * 16);
+      const bf16x8 v = *(const bf16x8*)(ep + f * EPI_STRIDE + ch * 16);
       if (r < p.rows && co < p.n) {
-        *(u32x4*)((bf16*)p.y + (int64_t)r * p.ldy + co) = v;
-        if (p.y2 && co >= p.y2_from) *(u32x4*)(p.y2 + (int64_t)r * p.ldy2 + co) = v;
+        store_bf16x8((bf16*)p.y + (int64_t)r * p.ldy, co, p.n, v);
+        if (p.y2 && co >= p.y2_from) store_bf16x8(p.y2 + (int64_t)r * p.ldy2, co, p.n, v);
       }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -428,8 +427,8 @@ __global__ __launch_bounds__(512, 2) void fp8_linear_short_kernel(LinearArgs p, 
         bf16x8 o;
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[i] = (bf16)v[i];
-        *(bf16x8*)((bf16*)p.y + (int64_t)r * p.ldy + cl) = o;
-        if (p.y2 && cl >= p.y2_from) *(bf16x8*)(p.y2 + (int64_t)r * p.ldy2 + cl) = o;
+        store_bf16x8((bf16*)p.y + (int64_t)r * p.ldy, cl, p.n, o);
+        if (p.y2 && cl >= p.y2_from) store_bf16x8(p.y2 + (int64_t)r * p.ldy2, cl, p.n, o);
       }
     }
   }
@@ -667,8 +666,8 @@ __device__ __forceinline__ void fp8_tiles_persist(const LinearArgs& p, const int
       for (int i = 0; i < 16 * HN / RPP; ++i) {
         const int f = i * RPP + lane / CPR, ch = lane % CPR;
         const int rr = r_cur + wn * FW + pass * (16 * HN) + f, co = co_cur + wm * CW + ch * 8;
-        const u32x4 v = *(const u32x4*)(ep + f * EPI_STRIDE + ch * 16);
-        if (rr < p.rows && co < p.n) *(u32x4*)((bf16*)p.y + (int64_t)rr * p.ldy + co) = v;
+        const bf16x8 v = *(const bf16x8*)(ep + f * EPI_STRIDE + ch * 16);
+        if (rr < p.rows && co < p.n) store_bf16x8((bf16*)p.y + (int64_t)rr * p.ldy, co, p.n, v);
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_wave_barrier();
@@ -736,9 +735,9 @@ int launch_rows(const LinearArgs& p, hipStream_t s) {
     return SUGAR_OK;
   }
   const int64_t slabs = ceil_div(p.n, 256);
-  if (!f32 && p.vec && p.kb <= 4 && n_cu % 8 == 0 && slabs >= 2 && 4ll * p.n >= 3 * 256 * slabs && p.rows * slabs >= 400ll * n_cu)
+  if (!f32 && p.kb <= 4 && n_cu % 8 == 0 && slabs >= 2 && 4ll * p.n >= 3 * 256 * slabs && p.rows * slabs >= 400ll * n_cu)
     return launch_short(p, n_cu, s);
-  if (!f32 && p.vec && !p.y2 && p.kb >= 8 && n_cu % 8 == 0 && ceil_div(p.n, 256) * ceil_div(p.rows, 256) >= 2 * n_cu)
+  if (!f32 && !p.y2 && p.kb >= 8 && n_cu % 8 == 0 && ceil_div(p.n, 256) * ceil_div(p.rows, 256) >= 2 * n_cu)
     return launch_persist(p, n_cu, s);
   if (ceil_div(p.n, 128) * ceil_div(p.rows, 128) >= n_cu)
     return f32 ? launch_tile<128, 128, 2, true>(p, s) : launch_tile<128, 128, 2, false>(p, s);
@@ -764,8 +763,6 @@ int launch_fp8_linear(const Fp8Operand& a, int64_t rows, const Fp8Operand& w, in
   p.ldy = out.ldy; p.scale = scale; p.shift = shift;
   p.n = n; p.kb = (int)fp8_blocks(k); p.flags = flags; p.out_f32 = out.dtype == SUGAR_F32; p.n_co_tiles = 0;
   p.ldy2 = out.ldy2; p.y2_from = out.y2_from;
-  p.vec = ((uintptr_t)out.y & 15) == 0 && (out.ldy * esz) % 16 == 0 && (n * esz) % 16 == 0 &&
-          ((uintptr_t)out.y2 & 15) == 0 && (out.ldy2 * esz) % 16 == 0;
   for (int64_t r0 = 0; r0 < rows; r0 += per) {
     p.a = a.q + r0 * a.ldq; p.ae = a.e + r0 * a.lde;
     p.y = (char*)out.y + r0 * out.ldy * esz;

@@ -8,6 +8,8 @@
 // Everything between the loads and the stores is f32 in registers: a wave (or four, for wide or few rows) holds its row,
 // so a norm's mean and its sum of squares about that mean are two exact passes over registers, not over memory, and z
 // comes from the unrounded s.  Bound: HBM (u and residual in, stream and z out).
+#include <type_traits>
+
 #include "blockfp8.h"
 
 namespace sugar {
@@ -50,41 +52,41 @@ __device__ __forceinline__ float row_total(float v, float* red, int wv) {
 }
 
 // Eight channels as they lie in memory, fetched without a branch and without touching the values, so that every load of a
-// row is on its way before the first is used.  VEC: 16-byte loads; a lane past the row reads the row's beginning.
-template <typename T, bool VEC>
+// row is on its way before the first is used: 16-byte loads, a lane that is not whole inside the row reads the row's
+// beginning.  The lane with the last n % 8 channels fetches them one by one when it is asked for the values.
+// WIDE: rows of 8 channels and more; shorter ones are read one by one altogether.
+template <typename T, bool WIDE>
 struct Raw8 {
-  u32x4 q[sizeof(T) / 2];
-  float f[VEC ? 1 : 8];
+  typedef typename std::conditional<sizeof(T) == 2, bf16x8_u, f32x4_u>::type Chunk;
+  Chunk q[sizeof(T) / 2];
   __device__ __forceinline__ void load(const T* __restrict__ p, int c, int n) {
-    if constexpr (VEC) {
-      const u32x4* s = (const u32x4*)(p + (c < n ? c : 0));
+    if constexpr (WIDE) {
+      const Chunk* s = (const Chunk*)(p + (c + 8 <= n ? c : 0));
 #pragma unroll
       for (int i = 0; i < (int)sizeof(T) / 2; ++i) q[i] = s[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = c + i < n ? to_f32(p[c + i]) : 0.f;
     }
   }
-  __device__ __forceinline__ void get(float* v, int c, int n) const {
-    if constexpr (VEC) {
-      const bool in = c < n;
+  __device__ __forceinline__ void get(const T* __restrict__ p, float* v, int c, int n) const {
+    if constexpr (WIDE) {
+      const bool in = c + 8 <= n;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float t;
-        if constexpr (sizeof(T) == 2) t = __uint_as_float(i & 1 ? q[0][i / 2] & 0xffff0000u : q[0][i / 2] << 16);
-        else t = __uint_as_float(q[i / 4][i % 4]);
-        v[i] = in ? t : 0.f;
+      for (int i = 0; i < 8; ++i) v[i] = in ? to_f32(q[i * sizeof(T) / 16][i % (16 / sizeof(T))]) : 0.f;
+    }
+    if (!WIDE || (n & 7)) {
+      if (c < n && c + 8 > n) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < n ? to_f32(p[c + i]) : 0.f;
+      } else if (!WIDE) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.f;
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = f[i];
     }
   }
 };
 
 // weight and bias of a norm for this lane's channels: 1 and 0 where there is no vector, 0 past the row (so that what a
 // norm leaves there is 0)
-template <int NCH, int WPR, bool VEC>
+template <int NCH, int WPR, bool WIDE>
 struct NormVec {
   float w[NCH][8], b[NCH][8];
   __device__ __forceinline__ void load(const float* __restrict__ pw, const float* __restrict__ pb, int cw, int C) {
@@ -93,16 +95,16 @@ struct NormVec {
       const int c = cw + k * (512 * WPR);
 #pragma unroll
       for (int i = 0; i < 8; ++i) { w[k][i] = c + i < C ? 1.f : 0.f; b[k][i] = 0.f; }
-      Raw8<float, VEC> t;
-      if (pw) { t.load(pw, c, C); t.get(w[k], c, C); }
-      if (pb) { t.load(pb, c, C); t.get(b[k], c, C); }
+      Raw8<float, WIDE> t;
+      if (pw) { t.load(pw, c, C); t.get(pw, w[k], c, C); }
+      if (pb) { t.load(pb, c, C); t.get(pb, b[k], c, C); }
     }
   }
 };
 
 // x <- norm(x) over the row's C channels; lanes past the row hold zeros before and after.
-template <int NCH, int WPR, bool VEC>
-__device__ __forceinline__ void row_norm(float (&x)[NCH][8], int kind, const NormVec<NCH, WPR, VEC>& p, float eps, int C, float inv_c, int cw,
+template <int NCH, int WPR, bool WIDE>
+__device__ __forceinline__ void row_norm(float (&x)[NCH][8], int kind, const NormVec<NCH, WPR, WIDE>& p, float eps, int C, float inv_c, int cw,
                                          float* red, int wv) {
   if (kind == NORM_NONE) return;
   float mean = 0.f, mul = 1.f;
@@ -120,10 +122,18 @@ __device__ __forceinline__ void row_norm(float (&x)[NCH][8], int kind, const Nor
     for (int k = 0; k < NCH; ++k) {
       const int c = cw + k * (512 * WPR);
       float tk = 0.f;
+      if (C & 7) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = VEC || c + i < C ? x[k][i] - mean : 0.f;
-        tk = fmaf(d, d, tk);
+        for (int i = 0; i < 8; ++i) {
+          const float d = c + i < C ? x[k][i] - mean : 0.f;
+          tk = fmaf(d, d, tk);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float d = x[k][i] - mean;
+          tk = fmaf(d, d, tk);
+        }
       }
       t += c < C ? tk : 0.f;
     }
@@ -136,7 +146,7 @@ __device__ __forceinline__ void row_norm(float (&x)[NCH][8], int kind, const Nor
 }
 
 // NCH x 8 channels a lane, WPR waves a row.  Each wave (WPR = 1; else each workgroup) takes a run of consecutive rows.
-template <typename TU, typename TS, int NCH, int WPR, bool VEC, bool NORMS>
+template <typename TU, typename TS, int NCH, int WPR, bool WIDE, bool NORMS>
 __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void block_join_kernel(JoinArgs a) {
   __shared__ float red[WPR > 1 ? WPR : 1];
   const SugarBlockJoin& j = a.j;
@@ -160,7 +170,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void block_join_kernel(Jo
     b_end = j.d_row_off[b + 1];
     begin = j.d_row_off[0];
   }
-  NormVec<NCH, WPR, VEC> post, pre;                                 // in registers over the rows
+  NormVec<NCH, WPR, WIDE> post, pre;                                 // in registers over the rows
   if (NORMS && j.post_kind) post.load(j.d_post_w, j.d_post_b, cw, C);
   if (NORMS && j.pre_kind) pre.load(j.d_pre_w, j.d_pre_b, cw, C);
   for (int64_t r = first; r < last; ++r) {
@@ -168,36 +178,40 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void block_join_kernel(Jo
       while (r >= b_end && b + 1 < j.n_utts) { ++b; b_end = j.d_row_off[b + 1]; }
       if (r >= b_end || r < begin) continue;                   // a row of no utterance: left as it is
     }
-    Raw8<TU, VEC> ru[NCH], rgu[NCH];
-    Raw8<TS, VEC> rs[NCH];
-    Raw8<float, VEC> rg[NCH];
+    const TU* up = (const TU*)j.d_u + r * j.ldu;
+    const TS* rp = (const TS*)j.d_residual + r * j.ldr;
+    const void* gp = j.gate_kind == SUGAR_GATE_ROW ? (const void*)((const TU*)j.d_gate + r * j.ldg)
+                                                   : (const void*)((const float*)j.d_gate + (j.gate_kind == SUGAR_GATE_UTTERANCE ? b * j.ldg : 0));
+    Raw8<TU, WIDE> ru[NCH], rgu[NCH];
+    Raw8<TS, WIDE> rs[NCH];
+    Raw8<float, WIDE> rg[NCH];
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) ru[k].load((const TU*)j.d_u + r * j.ldu, cw + k * (512 * WPR), C);
+    for (int k = 0; k < NCH; ++k) ru[k].load(up, cw + k * (512 * WPR), C);
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) rs[k].load((const TS*)j.d_residual + r * j.ldr, cw + k * (512 * WPR), C);
+    for (int k = 0; k < NCH; ++k) rs[k].load(rp, cw + k * (512 * WPR), C);
     if (j.gate_kind == SUGAR_GATE_ROW) {
 #pragma unroll
-      for (int k = 0; k < NCH; ++k) rgu[k].load((const TU*)j.d_gate + r * j.ldg, cw + k * (512 * WPR), C);
+      for (int k = 0; k < NCH; ++k) rgu[k].load((const TU*)gp, cw + k * (512 * WPR), C);
     } else if (j.gate_kind) {
 #pragma unroll
       for (int k = 0; k < NCH; ++k)
-        rg[k].load((const float*)j.d_gate + (j.gate_kind == SUGAR_GATE_UTTERANCE ? b * j.ldg : 0), cw + k * (512 * WPR), C);
+        rg[k].load((const float*)gp, cw + k * (512 * WPR), C);
     }
     float v[NCH][8], s[NCH][8];
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) ru[k].get(v[k], cw + k * (512 * WPR), C);
-    if (NORMS) row_norm<NCH, WPR, VEC>(v, j.post_kind, post, j.post_eps, C, inv_c, cw, red, wv);
+    for (int k = 0; k < NCH; ++k) ru[k].get(up, v[k], cw + k * (512 * WPR), C);
+    if (NORMS) row_norm<NCH, WPR, WIDE>(v, j.post_kind, post, j.post_eps, C, inv_c, cw, red, wv);
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       const int c = cw + k * (512 * WPR);
       float g[8];
-      if (j.gate_kind == SUGAR_GATE_ROW) rgu[k].get(g, c, C);
-      else if (j.gate_kind) rg[k].get(g, c, C);
+      if (j.gate_kind == SUGAR_GATE_ROW) rgu[k].get((const TU*)gp, g, c, C);
+      else if (j.gate_kind) rg[k].get((const float*)gp, g, c, C);
       else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) g[i] = 1.f;
       }
-      rs[k].get(s[k], c, C);
+      rs[k].get(rp, s[k], c, C);
       float st[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -205,16 +219,16 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void block_join_kernel(Jo
         s[k][i] = fmaf(j.alpha * g[i], v[k][i], res);
         st[i] = j.dense ? res + s[k][i] : s[k][i];
       }
-      if (j.d_stream) store8((TS*)j.d_stream + r * j.lds, c, C, VEC, st);
+      if (j.d_stream) store8((TS*)j.d_stream + r * j.lds, c, C, st);
     }
     if (!j.d_z && !j.d_q) continue;
-    if (NORMS) row_norm<NCH, WPR, VEC>(s, j.pre_kind, pre, j.pre_eps, C, inv_c, cw, red, wv);
+    if (NORMS) row_norm<NCH, WPR, WIDE>(s, j.pre_kind, pre, j.pre_eps, C, inv_c, cw, red, wv);
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       const int c = cw + k * (512 * WPR);
       if (j.d_z) {
-        if (j.z_dtype == SUGAR_F32) store8((float*)j.d_z + r * j.ldz, c, C, VEC, s[k]);
-        else store8((bf16*)j.d_z + r * j.ldz, c, C, VEC, s[k]);
+        if (j.z_dtype == SUGAR_F32) store8((float*)j.d_z + r * j.ldz, c, C, s[k]);
+        else store8((bf16*)j.d_z + r * j.ldz, c, C, s[k]);
       }
       if (j.d_q) {                                             // (past the row s is 0: the operand's padding columns)
         unsigned big = 0;
@@ -233,7 +247,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void block_join_kernel(Jo
 }
 
 template <typename TU, typename TS, int NCH, int WPR>
-int launch_join(JoinArgs a, bool vec, int n_cu, hipStream_t s) {
+int launch_join(JoinArgs a, int n_cu, hipStream_t s) {
   constexpr int threads = WPR > 4 ? 64 * WPR : 256;
   // Rows a wave (workgroup) takes one after the other.  Many rows: without norms 2 (77 056 x 512 with 8-bit output: 56 / 50 /
   // 52 / 55 us for 1 / 2 / 4 / 8), with norms enough to share the fetch of their vectors (92 / 70 / 60 / 61 us; 48 611 x
@@ -243,22 +257,23 @@ int launch_join(JoinArgs a, bool vec, int n_cu, hipStream_t s) {
   const int64_t most = WPR > 1 ? 8 : !norms || NCH > 1 || sizeof(TU) == 4 ? 2 : 4, share = a.j.rows / (8ll * n_cu * (WPR > 1 ? 1 : 4));
   a.run = (int)(share < 1 ? 1 : share < most ? share : most);
   const dim3 grid((unsigned)ceil_div(a.j.rows, (int64_t)a.run * (WPR > 1 ? 1 : 4)));
-  if (vec && norms) hipLaunchKernelGGL((block_join_kernel<TU, TS, NCH, WPR, true, true>), grid, dim3(threads), 0, s, a);
-  else if (vec) hipLaunchKernelGGL((block_join_kernel<TU, TS, NCH, WPR, true, false>), grid, dim3(threads), 0, s, a);
+  const bool wide = a.j.cols >= 8;
+  if (wide && norms) hipLaunchKernelGGL((block_join_kernel<TU, TS, NCH, WPR, true, true>), grid, dim3(threads), 0, s, a);
+  else if (wide) hipLaunchKernelGGL((block_join_kernel<TU, TS, NCH, WPR, true, false>), grid, dim3(threads), 0, s, a);
   else hipLaunchKernelGGL((block_join_kernel<TU, TS, NCH, WPR, false, true>), grid, dim3(threads), 0, s, a);
   SUGAR_LAUNCH_CHECK();
   return SUGAR_OK;
 }
 
 template <typename TU, typename TS>
-int launch_join_t(const JoinArgs& a, bool vec, hipStream_t s) {
+int launch_join_t(const JoinArgs& a, hipStream_t s) {
   int n_cu = 0;
   if (int rc = device_cu_count(&n_cu)) return rc;
   const int C = a.j.cols;
-  if (C <= 512) return launch_join<TU, TS, 1, 1>(a, vec, n_cu, s);
-  if (C <= 1024 && a.j.rows >= 16ll * n_cu) return launch_join<TU, TS, 2, 1>(a, vec, n_cu, s);
-  if (C <= 2048) return launch_join<TU, TS, 1, 4>(a, vec, n_cu, s);
-  return launch_join<TU, TS, 1, 16>(a, vec, n_cu, s);
+  if (C <= 512) return launch_join<TU, TS, 1, 1>(a, n_cu, s);
+  if (C <= 1024 && a.j.rows >= 16ll * n_cu) return launch_join<TU, TS, 2, 1>(a, n_cu, s);
+  if (C <= 2048) return launch_join<TU, TS, 1, 4>(a, n_cu, s);
+  return launch_join<TU, TS, 1, 16>(a, n_cu, s);
 }
 
 bool norm_ok(int kind) { return kind == NORM_NONE || kind == NORM_AFFINE || kind == NORM_RMS || kind == NORM_LAYER; }
@@ -269,15 +284,8 @@ int launch_block_join(const SugarBlockJoin& j, bool pad_exponents, hipStream_t s
   JoinArgs a;
   a.j = j;
   a.e_bytes = (int)(pad_exponents ? fp8_lds(j.cols) : fp8_blocks(j.cols));
-  const int eu = j.u_dtype == SUGAR_F32 ? 4 : 2, es = j.stream_dtype == SUGAR_F32 ? 4 : 2, ez = j.z_dtype == SUGAR_F32 ? 4 : 2;
-  const int eg = j.gate_kind == SUGAR_GATE_ROW ? eu : 4;
-  // one path for rows that are all 16-byte aligned in whole chunks of 8 channels, one for everything else
-  const bool vec = rows_vec(j.d_u, j.ldu, j.cols, eu) && rows_vec(j.d_residual, j.ldr, j.cols, es) &&
-                   (!j.d_stream || rows_vec(j.d_stream, j.lds, j.cols, es)) && (!j.d_z || rows_vec(j.d_z, j.ldz, j.cols, ez)) &&
-                   !(((uintptr_t)j.d_post_w | (uintptr_t)j.d_post_b | (uintptr_t)j.d_pre_w | (uintptr_t)j.d_pre_b) & 15) &&
-                   (!j.d_gate || rows_vec(j.d_gate, j.gate_kind == SUGAR_GATE_CHANNEL ? j.cols : j.ldg, j.cols, eg));
-  if (j.u_dtype == SUGAR_F32) return launch_join_t<float, float>(a, vec, s);
-  return j.stream_dtype == SUGAR_F32 ? launch_join_t<bf16, float>(a, vec, s) : launch_join_t<bf16, bf16>(a, vec, s);
+  if (j.u_dtype == SUGAR_F32) return launch_join_t<float, float>(a, s);
+  return j.stream_dtype == SUGAR_F32 ? launch_join_t<bf16, float>(a, s) : launch_join_t<bf16, bf16>(a, s);
 }
 
 }  // namespace sugar
