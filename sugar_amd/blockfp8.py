@@ -125,9 +125,11 @@ def _apart(what, out, others, same=()):
 
 def _vector(what, v, n):
     """A contiguous float32 vector of n (other float types and strides are converted)."""
+    if v.dtype is torch.float32 and v.shape == (n,) and v.is_contiguous():
+        return v
     if v.dim() != 1 or v.shape[0] != n or not v.dtype.is_floating_point:
         raise ValueError("%s: expected a floating vector of %d, got %s %s" % (what, n, v.dtype, tuple(v.shape)))
-    return v if v.dtype == torch.float32 and v.is_contiguous() else v.to(torch.float32).contiguous()
+    return v.to(torch.float32).contiguous()
 
 
 class BlockFP8(object):

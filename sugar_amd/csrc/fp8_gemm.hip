@@ -56,30 +56,36 @@ __device__ __forceinline__ i32x8 frag(const unsigned char* base, int row, int fq
   return f;
 }
 
-// Epilogue and store of four consecutive channels of one row, straight from the accumulators.
-__device__ __forceinline__ void store_out4(const LinearArgs& p, int64_t r, int co, f32x4 v) {
-  if (p.flags & EPI_RELU) {
+__device__ __forceinline__ f32x4 epilogue4(f32x4 v, bool relu, bool affine, f32x4 sc, f32x4 sh) {
+  if (relu) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = relu_nan(v[i]);
   }
-  if (p.out_f32 && co + 4 <= p.n) {
-    if (p.flags & EPI_AFFINE) {
-      const f32x4 sc = *(const f32x4_u*)(p.scale + co), sh = *(const f32x4_u*)(p.shift + co);
+  if (affine) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = fmaf(v[i], sc[i], sh[i]);
+    for (int i = 0; i < 4; ++i) v[i] = fmaf(v[i], sc[i], sh[i]);
+  }
+  return v;
+}
+
+// Four consecutive results of one row, from channel co on.
+__device__ __forceinline__ void store_out4(const LinearArgs& p, int64_t r, int co, f32x4 v) {
+  if (p.out_f32) {
+    float* y = (float*)p.y + r * p.ldy + co;
+    if (co + 4 <= p.n) {
+      *(f32x4_u*)y = v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (co + i < p.n) y[i] = v[i];
     }
-    *(f32x4_u*)((float*)p.y + r * p.ldy + co) = v;
     return;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (co + i >= p.n) break;
-    const float t = p.flags & EPI_AFFINE ? fmaf(v[i], p.scale[co + i], p.shift[co + i]) : v[i];
-    if (p.out_f32) ((float*)p.y)[r * p.ldy + co + i] = t;
-    else {
-      ((bf16*)p.y)[r * p.ldy + co + i] = (bf16)t;
-      if (p.y2 && co + i >= p.y2_from) p.y2[r * p.ldy2 + co + i] = (bf16)t;
-    }
+    ((bf16*)p.y)[r * p.ldy + co + i] = (bf16)v[i];
+    if (p.y2 && co + i >= p.y2_from) p.y2[r * p.ldy2 + co + i] = (bf16)v[i];
   }
 }
 
@@ -129,6 +135,15 @@ __global__ __launch_bounds__(64 * NW) void fp8_linear_direct_kernel(LinearArgs p
 #pragma unroll
     for (int k = 1; k < NW; ++k) v += part[k][t][lane];
     const int r = r0 + t * 16 + fr;
+    f32x4 sc = {1.f, 1.f, 1.f, 1.f}, sh = {0.f, 0.f, 0.f, 0.f};
+    if (p.flags & EPI_AFFINE) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sc[i] = p.scale[min(co + 4 * fq + i, p.n - 1)];
+        sh[i] = p.shift[min(co + 4 * fq + i, p.n - 1)];
+      }
+    }
+    v = epilogue4(v, p.flags & EPI_RELU, p.flags & EPI_AFFINE, sc, sh);
     if (r < p.rows) store_out4(p, r, co + 4 * fq, v);
   }
 }
@@ -138,7 +153,7 @@ __global__ __launch_bounds__(64 * NW) void fp8_linear_direct_kernel(LinearArgs p
 // share of k-tile t, barrier, issue the DMA of k-tile t + NS - 1 into the buffer k-tile t - 1 was read from, compute.
 // Exponents travel as one dword per row and four k-tiles, staged with the first of the four (double buffer) and shifted
 // down a byte per k-tile.
-constexpr int linear_tile_lds(int TM, int TN, int NS) { return (TM + TN) * (NS * 128 + 8); }
+constexpr int linear_tile_lds(int TM, int TN, int NS) { return (TM + TN) * (NS * 128 + 8) + 8 * TM; }
 
 template <int TM, int TN, int NS, bool WIDE>
 __device__ __forceinline__ void fp8_tile(const LinearArgs& p, const int co_base, const int r_base) {
@@ -150,7 +165,14 @@ __device__ __forceinline__ void fp8_tile(const LinearArgs& p, const int co_base,
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wv >> 2, wn = wv & 3, fr = lane & 15, fq = lane >> 4;
   unsigned* exps = (unsigned*)(smem + NS * STAGE_BYTES);         // [2][TM + TN]
+  float* aff = (float*)(exps + 2 * (TM + TN));                   // [scale | shift][TM], fetched with the first k-tile
   const int nk = p.kb;
+  const bool relu = p.flags & EPI_RELU, affine = p.flags & EPI_AFFINE;
+  if (affine && wv < TM / 32) {
+    const int c = (wv % (TM / 64)) * 64;
+    dma<4>((const uint8_t*)(wv < TM / 64 ? p.scale : p.shift), 4 * min(co_base + c + lane, p.n - 1),
+           (unsigned char*)(aff + (wv < TM / 64 ? 0 : TM) + c));
+  }
 
   unsigned woff[WI], xoff[XI];
 #pragma unroll
@@ -235,17 +257,31 @@ __device__ __forceinline__ void fp8_tile(const LinearArgs& p, const int co_base,
   }
 
   // ---- epilogue: accumulator tile (m, n): lane (fr, fq) holds row wn FW + n 16 + fr, channels wm CW + m 16 + 4 fq + 0..3
-  if (p.out_f32) {                                               // 16 bytes a lane, 64 in a row
+  f32x4 sc[MI], sh[MI];
+#pragma unroll
+  for (int m = 0; m < MI; ++m) {
+    sc[m] = (f32x4){1.f, 1.f, 1.f, 1.f};
+    sh[m] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  }
+  if (affine) {
+#pragma unroll
+    for (int m = 0; m < MI; ++m) {
+      sc[m] = *(const f32x4*)(aff + wm * CW + m * 16 + 4 * fq);
+      sh[m] = *(const f32x4*)(aff + TM + wm * CW + m * 16 + 4 * fq);
+    }
+  }
+  if constexpr (WIDE) {                                          // float32 outputs: 16 bytes a lane, 64 in a row
 #pragma unroll
     for (int n = 0; n < NJ; ++n) {
       const int r = r_base + wn * FW + n * 16 + fr;
       if (r >= p.rows) continue;
 #pragma unroll
-      for (int m = 0; m < MI; ++m) store_out4(p, r, co_base + wm * CW + m * 16 + 4 * fq, acc[m][n]);
+      for (int m = 0; m < MI; ++m)
+        store_out4(p, r, co_base + wm * CW + m * 16 + 4 * fq, epilogue4(acc[m][n], relu, affine, sc[m], sh[m]));
     }
+    return;
   }
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // stage memory free: epilogue staging, or the caller's next tile
-  if (p.out_f32) return;
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // stage memory becomes the epilogue staging
   constexpr int EPI_STRIDE = CW * 2 + 16, CPR = CW / 8, RPP = 64 / CPR;
   static_assert(8 * 16 * EPI_STRIDE <= NS * STAGE_BYTES, "epilogue staging fits the stages");
   unsigned char* ep = smem + wv * (16 * EPI_STRIDE);             // this wave's [16 rows][CW channels]
@@ -253,15 +289,8 @@ __device__ __forceinline__ void fp8_tile(const LinearArgs& p, const int co_base,
   for (int n = 0; n < NJ; ++n) {
 #pragma unroll
     for (int m = 0; m < MI; ++m) {
-      const int col = m * 16 + 4 * fq, co = co_base + wm * CW + col;
-      f32x4 v = acc[m][n];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (p.flags & EPI_RELU) v[i] = relu_nan(v[i]);
-        if (p.flags & EPI_AFFINE) v[i] = fmaf(v[i], p.scale[min(co + i, p.n - 1)], p.shift[min(co + i, p.n - 1)]);
-      }
-      const bf16x4 o = {(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
-      *(bf16x4*)(ep + fr * EPI_STRIDE + col * 2) = o;
+      const f32x4 v = epilogue4(acc[m][n], relu, affine, sc[m], sh[m]);
+      *(bf16x4*)(ep + fr * EPI_STRIDE + (m * 16 + 4 * fq) * 2) = (bf16x4){(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // the staging is the wave's own: no workgroup barrier
     __builtin_amdgcn_wave_barrier();
@@ -329,7 +358,8 @@ struct Short {
   static constexpr int LDS = NS * (STAGE + 256);
 };
 
-template <int KB>
+// RAGGED: n is no multiple of 8 (the store of a row's last channels one by one, in the loop of every product, cost 8 %)
+template <int KB, bool RAGGED>
 __global__ __launch_bounds__(512, 2) void fp8_linear_short_kernel(LinearArgs p, int n_slabs, int runs) {
   typedef Short<KB> C;
   constexpr int NS = C::NS, D = NS - 1, NST = 4;
@@ -427,32 +457,34 @@ __global__ __launch_bounds__(512, 2) void fp8_linear_short_kernel(LinearArgs p, 
         bf16x8 o;
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[i] = (bf16)v[i];
-        store_bf16x8((bf16*)p.y + (int64_t)r * p.ldy, cl, p.n, o);
-        if (p.y2 && cl >= p.y2_from) store_bf16x8(p.y2 + (int64_t)r * p.ldy2, cl, p.n, o);
+        if constexpr (RAGGED) store_bf16x8((bf16*)p.y + (int64_t)r * p.ldy, cl, p.n, o);
+        else *(bf16x8_u*)((bf16*)p.y + (int64_t)r * p.ldy + cl) = o;
+        if (p.y2 && cl >= p.y2_from) *(bf16x8_u*)(p.y2 + (int64_t)r * p.ldy2 + cl) = o;
       }
     }
   }
 }
 
-template <int KB>
+template <int KB, bool RAGGED>
 int launch_short(const LinearArgs& p, int n_cu, hipStream_t s) {
   typedef Short<KB> C;
   static OptInMask opted{0};
-  if (int rc = lds_opt_in((const void*)fp8_linear_short_kernel<KB>, C::LDS, &opted)) return rc;
+  if (int rc = lds_opt_in((const void*)fp8_linear_short_kernel<KB, RAGGED>, C::LDS, &opted)) return rc;
   const int n_slabs = (int)ceil_div(p.n, C::SLAB);
   int runs = n_cu / n_slabs / 8 * 8;
   if (runs < 8) runs = 8;
-  hipLaunchKernelGGL(fp8_linear_short_kernel<KB>, dim3((unsigned)(n_slabs * runs)), dim3(512), C::LDS, s, p, n_slabs, runs);
+  hipLaunchKernelGGL((fp8_linear_short_kernel<KB, RAGGED>), dim3((unsigned)(n_slabs * runs)), dim3(512), C::LDS, s, p, n_slabs, runs);
   SUGAR_LAUNCH_CHECK();
   return SUGAR_OK;
 }
 
 int launch_short(const LinearArgs& p, int n_cu, hipStream_t s) {
+  const bool ragged = p.n % 8 != 0;
   switch (p.kb) {
-    case 1: return launch_short<1>(p, n_cu, s);
-    case 2: return launch_short<2>(p, n_cu, s);
-    case 3: return launch_short<3>(p, n_cu, s);
-    default: return launch_short<4>(p, n_cu, s);
+    case 1: return ragged ? launch_short<1, true>(p, n_cu, s) : launch_short<1, false>(p, n_cu, s);
+    case 2: return ragged ? launch_short<2, true>(p, n_cu, s) : launch_short<2, false>(p, n_cu, s);
+    case 3: return ragged ? launch_short<3, true>(p, n_cu, s) : launch_short<3, false>(p, n_cu, s);
+    default: return ragged ? launch_short<4, true>(p, n_cu, s) : launch_short<4, false>(p, n_cu, s);
   }
 }
 
@@ -755,6 +787,7 @@ int launch_fp8_linear(const Fp8Operand& a, int64_t rows, const Fp8Operand& w, in
   SUGAR_CHECK_ARG(n * w.ldq <= SPAN && n * w.lde <= SPAN, "fp8_linear: weights of %d rows with stride %lld are too large", n,
                   (long long)w.ldq);
   SUGAR_CHECK_ARG(a.ldq <= SPAN / 256 && a.lde <= SPAN / 256, "fp8_linear: row stride %lld too large", (long long)a.ldq);
+  SUGAR_CHECK_ARG(!out.y2 || (n % 8 == 0 && out.y2_from % 8 == 0 && out.dtype == SUGAR_BF16), "fp8_linear: second output of ragged chunks");
   const int64_t per = SPAN / (a.ldq > a.lde ? a.ldq : a.lde) / 256 * 256;
   const int esz = out.dtype == SUGAR_F32 ? 4 : 2;
   LinearArgs p;
