@@ -2,6 +2,7 @@
 // The format is described in blockfp8.h.
 #include <math.h>
 
+#include <new>
 #include <vector>
 
 #include "blockfp8.h"
@@ -95,7 +96,7 @@ static uint8_t host_e4m3(float v) {
   return sign | (uint8_t)((e + 6) << 3 | (m - 8));
 }
 
-int pack_fp8(Fp8Weight* w, const float* h_w, int cout, int cin, int n, const int* out_map, int k, const int* in_map) {
+static int pack_fp8_rows(Fp8Weight* w, const float* h_w, int cout, int cin, int n, const int* out_map, int k, const int* in_map) {
   const int64_t ldq = fp8_ldq(k), lde = fp8_lds(k);
   std::vector<uint8_t> q((size_t)(n * ldq), 0), e((size_t)(n * lde), 127);
   std::vector<float> row((size_t)ldq);
@@ -127,6 +128,15 @@ int pack_fp8(Fp8Weight* w, const float* h_w, int cout, int cin, int n, const int
   w->n = n;
   w->k = k;
   return SUGAR_OK;
+}
+
+int pack_fp8(Fp8Weight* w, const float* h_w, int cout, int cin, int n, const int* out_map, int k, const int* in_map) {
+  try {                                                               // (called below a C entry)
+    return pack_fp8_rows(w, h_w, cout, cin, n, out_map, k, in_map);
+  } catch (const std::bad_alloc&) {
+    set_error("pack_fp8: host alloc");
+    return SUGAR_ENOMEM;
+  }
 }
 
 void free_fp8(Fp8Weight* w) {

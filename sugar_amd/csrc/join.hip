@@ -295,7 +295,7 @@ using namespace sugar;
 extern "C" int sugar_block_join(const SugarBlockJoin* h, void* stream) {
   SUGAR_CHECK_ARG(h, "block_join: null descriptor");
   const SugarBlockJoin& j = *h;
-  SUGAR_CHECK_ARG(j.rows >= 0 && j.rows < (1ll << 40) && j.cols > 0 && j.cols <= SUGAR_JOIN_MAX_COLS,
+  SUGAR_CHECK_ARG(j.rows >= 0 && j.rows < (1ll << 33) && j.cols > 0 && j.cols <= SUGAR_JOIN_MAX_COLS,
                   "block_join: rows %lld, columns %d out of range (1..%d)", (long long)j.rows, j.cols, SUGAR_JOIN_MAX_COLS);
   SUGAR_CHECK_ARG((j.u_dtype == SUGAR_F32 || j.u_dtype == SUGAR_BF16) && (j.stream_dtype == SUGAR_F32 || j.stream_dtype == SUGAR_BF16) &&
                       (j.z_dtype == SUGAR_F32 || j.z_dtype == SUGAR_BF16),

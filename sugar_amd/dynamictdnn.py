@@ -147,6 +147,8 @@ class TDNNSubnet(nn.Module):
         depth, ch, ks, ccat = config
         self.subnet_config = (int(depth), list(ch[:depth + 1]), list(ks[:depth + 1]), int(ccat))
         self.in_feats, self.out_embeds = in_feats, out_embeds
+        if precision not in _lib.PRECISIONS:
+            raise ValueError("precision %r not in %s" % (precision, sorted(_lib.PRECISIONS)))
         self.precision = precision
         shapes = layout.subnet_shapes(self.subnet_config, in_feats, out_embeds)
         _build_tree(self, shapes, _default_init if state is None else

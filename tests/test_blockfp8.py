@@ -234,7 +234,7 @@ def test_c_entries_check_their_arguments_before_any_launch():
         for k, v in kw.items():
             setattr(d, k, v)
         return lib.sugar_block_join(C.byref(d), None)
-    for kw in (dict(rows=-1), dict(cols=0), dict(cols=8193), dict(u_dtype=2), dict(u_dtype=0), dict(d_u=None), dict(d_stream=None),
+    for kw in (dict(rows=-1), dict(rows=1 << 33), dict(cols=0), dict(cols=8193), dict(u_dtype=2), dict(u_dtype=0), dict(d_u=None), dict(d_stream=None),
                dict(post_kind=4), dict(pre_kind=-1), dict(post_eps=-1.0), dict(gate_kind=1), dict(d_gate=p), dict(gate_kind=4, d_gate=p),
                dict(gate_kind=2, d_gate=p, ldg=8), dict(d_row_off=p), dict(ldu=7), dict(ldr=4), dict(d_z=p, ldz=7), dict(d_u=p + 1),
                dict(d_q=p, ldq=128, lde=4), dict(d_q=p, d_e=p, ldq=64, lde=4), dict(d_q=p, d_e=p, ldq=128, lde=1),

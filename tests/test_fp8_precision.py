@@ -45,6 +45,8 @@ def test_precision_names(supernet):
     assert sub.set_precision("fp32").feature_dtype == torch.float32 and sub.set_precision("bf16").feature_dtype == torch.bfloat16
     with pytest.raises(ValueError):
         sub.set_precision("fp16")
+    with pytest.raises(ValueError):
+        sugar_amd.TDNNSubnet(layout.SMALLEST, precision="fp16")
     assert _lib.lib().sugar_subnet_create(C.byref(_lib.SugarSubnetDesc()), 3, 0, C.byref(C.c_void_p())) == -1
 
 
