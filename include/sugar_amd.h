@@ -289,7 +289,7 @@ int sugar_snorm_trials(const float* d_scores, const int32_t* d_enroll, const int
  * sugar_fp8_dequant: d_y [rows][ldy] dtype <- the values (exact in either dtype within its normal range; a float32
  *   magnitude that rounded up to 2^128 reads back as infinity).
  * sugar_fp8_linear: d_y[r][o] = epilogue(sum_k a[r][k] w[o][k]), f32 accumulation.  SUGAR_F32 outputs: exact
- *   products, float32 sums.  SUGAR_BF16 outputs: the 8-bit matrix instruction, which aligns 8 neighbouring products to the
+ *   products of the values as bfloat16 numbers (which they are from 2^-133 up to 2^128), float32 sums.  SUGAR_BF16 outputs: the 8-bit matrix instruction, which aligns 8 neighbouring products to the
  *   largest and cuts them 2^-13 below its leading bit (1.5e-5 of the result on random operands; bf16 rounds by 1.7e-3).
  *   flags bit0 ReLU, bit1 * d_scale[o] + d_shift[o] after it (float32 [n]); d_y [rows][ldy] dtype.  The left operand is
  *   rows x k, the weights n x k; a call allocates nothing and needs no workspace. */

@@ -22,6 +22,8 @@ from . import _lib
 _DT = {torch.float32: _lib.SUGAR_F32, torch.bfloat16: _lib.SUGAR_BF16}
 NORMS = {"affine": 1, "rms": 2, "layer": 3}
 MAX_JOIN_COLS = 8192
+MAX_COLS = 1 << 24                                     # channels of an operand, outputs of a product (32-bit integers at the C ABI)
+F32_MAX, INF = torch.finfo(torch.float32).max, float("inf")
 _raw_stream = torch._C._cuda_getCurrentRawStream       # (torch.cuda.current_stream builds an object, 1 us of a 10 us call)
 _FN = {}
 
@@ -68,6 +70,8 @@ def _rows(what, x):
         raise ValueError("%s: expected [rows, columns], got %s" % (what, tuple(x.shape)))
     if x.dtype not in _DT:
         raise ValueError("%s: dtype %s not in %s" % (what, x.dtype, [str(d) for d in _DT]))
+    if x.shape[1] >= MAX_COLS:
+        raise ValueError("%s: %d columns, fewer than %d are taken" % (what, x.shape[1], MAX_COLS))
     ld = _row_stride(x)
     if ld is None:
         x = x.contiguous()
@@ -89,6 +93,8 @@ def _row_stride(x):
 
 def _out(what, out, shape, dtypes, dev):
     """Row stride of a tensor to write into."""
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("%s: an output that requires a gradient" % what)
     if tuple(out.shape) != tuple(shape) or out.dtype not in dtypes or out.device != dev:
         raise ValueError("%s: expected %s %s on %s, got %s %s on %s" % (what, tuple(shape), "/".join(str(d) for d in dtypes), dev,
                                                                         tuple(out.shape), out.dtype, out.device))
@@ -148,7 +154,7 @@ class BlockFP8(object):
         if data.dim() != 2 or data.dtype != torch.float8_e4m3fn or exponent.dim() != 2 or exponent.dtype != torch.uint8:
             raise ValueError("BlockFP8: data float8_e4m3fn [rows, n], exponent uint8 [rows, n]; got %s %s, %s %s"
                              % (data.dtype, tuple(data.shape), exponent.dtype, tuple(exponent.shape)))
-        if cols < 1 or data.shape[1] < blocks * self.BLOCK or exponent.shape[1] < _up(blocks, 4) or data.shape[0] != exponent.shape[0]:
+        if not 1 <= cols < MAX_COLS or data.shape[1] < blocks * self.BLOCK or exponent.shape[1] < _up(blocks, 4) or data.shape[0] != exponent.shape[0]:
             raise ValueError("BlockFP8: %d columns need data [rows, >= %d] and exponent [rows, >= %d], got %s and %s"
                              % (cols, blocks * self.BLOCK, _up(blocks, 4), tuple(data.shape), tuple(exponent.shape)))
         if data.device != exponent.device:
@@ -208,7 +214,7 @@ class BlockFP8(object):
         return BlockFP8(self.data[rows], self.exponent[rows], self.cols)
 
     def dequantize(self, dtype=torch.float32, out=None):
-        """The values, [rows, cols] float32 or bfloat16 (exact in both)."""
+        """The values, [rows, cols] float32 or bfloat16 (exact in both down to the type's subnormals: an e4m3 value has 4 bits)."""
         rows, cols = self.rows, self.cols
         dev = _gpu(self.device)
         if out is None:
@@ -229,6 +235,7 @@ def _fp8_out(what, out, rows, cols, dev):
         return BlockFP8.empty(rows, cols, dev)
     if not isinstance(out, BlockFP8) or out.rows != rows or out.cols != cols or out.device != dev:
         raise ValueError("%s: expected a BlockFP8 of [%d, %d] on %s" % (what, rows, cols, dev))
+    _apart(what, out.data, (out.exponent,))
     return out
 
 
@@ -263,8 +270,8 @@ def block_fp8_linear(a, w, scale=None, shift=None, relu=False, out_dtype=torch.b
     rows, n, k = a.rows, w.rows, a.cols
     if k != w.cols:
         raise ValueError("block_fp8_linear: a has %d columns, w %d" % (k, w.cols))
-    if n == 0:
-        raise ValueError("block_fp8_linear: w has no rows")
+    if not 0 < n < MAX_COLS:
+        raise ValueError("block_fp8_linear: w has %d rows, 1 .. %d are taken" % (n, MAX_COLS - 1))
     dev = a.device
     if w.device != dev:
         raise ValueError("tensors on %s and %s" % (dev, w.device))
@@ -300,8 +307,8 @@ class RowNorm(object):
     def __init__(self, kind, weight=None, bias=None, eps=1e-5):
         if kind not in NORMS:
             raise ValueError("RowNorm: kind %r not in %s" % (kind, sorted(NORMS)))
-        if not eps >= 0:
-            raise ValueError("RowNorm: negative eps %r" % (eps,))
+        if not 0 <= eps <= F32_MAX:
+            raise ValueError("RowNorm: eps %r is no finite float32 >= 0" % (eps,))
         self.kind, self.eps, self.code, self.cols = kind, float(eps), NORMS[kind], None
         for v in (weight, bias):
             if v is not None:
@@ -329,8 +336,8 @@ def block_join(u, residual, post=None, gate=None, row_off=None, alpha=1.0, dense
     `dense` is the running sum of DynamicTDNN.forward (:657-660).  Returns (stream, normed, quantized): stream in
     residual's dtype, normed = z in out_dtype (default u's) unless normed=False, quantized = z as BlockFP8 if asked for.
     Outputs may be passed in; stream_out may be `residual` or `u` itself, normed_out `u` (in place), any other shared memory
-    is refused.  With row_off, rows in
-    front of the first and behind the last utterance are left as they are (in outputs allocated here: undefined).
+    is refused.  With row_off, rows in front of the first and behind the last utterance are left as they are (in outputs
+    allocated here: undefined).  alpha is a number of the host, passed by value (a captured graph keeps it).
     """
     u, ldu = _rows("block_join: u", u)
     residual, ldr = _rows("block_join: residual", residual)
@@ -341,14 +348,17 @@ def block_join(u, residual, post=None, gate=None, row_off=None, alpha=1.0, dense
         raise ValueError("block_join: %d columns, at most %d" % (cols, MAX_JOIN_COLS))
     if u.dtype == torch.float32 and residual.dtype != torch.float32:
         raise ValueError("block_join: a float32 u needs a float32 residual")
+    if isinstance(alpha, torch.Tensor) or (abs(alpha) > F32_MAX and abs(alpha) != INF):
+        raise ValueError("block_join: alpha %r is no float32 number" % (alpha,))
     dev = u.device
-    inputs = [residual, u]
+    inputs = [residual, u]                             # and the norms' vectors, then what else comes in
     post_kind = pre_kind = post_w = post_b = pre_w = pre_b = 0
     post_eps = pre_eps = 0.0
     if post is not None:
         post_kind, post_eps, post_w, post_b = _norm("post", post, cols, inputs)
     if pre is not None:
         pre_kind, pre_eps, pre_w, pre_b = _norm("pre", pre, cols, inputs)
+    vectors = inputs[2:]
     if gate is not None:
         inputs.append(gate)
     if row_off is not None:
@@ -389,7 +399,7 @@ def block_join(u, residual, post=None, gate=None, row_off=None, alpha=1.0, dense
     if quantized or quantized_out is not None:
         q = _fp8_out("block_join: quantized_out", quantized_out, rows, cols, dev)
     if stream_out is not None or normed_out is not None or quantized_out is not None:
-        others = [t for t in [u, residual, gate, row_off] + inputs[2:] if t is not None]
+        others = [t for t in [u, residual, gate, row_off] + vectors if t is not None]
         parts = [] if q is None else [q.data, q.exponent]
         _apart("block_join: stream_out", stream, others + parts, (residual, u))
         if z is not None:

@@ -154,7 +154,7 @@ extern "C" {
 int sugar_fp8_quant(const void* d_x, int64_t ldx, int dtype, int64_t rows, int cols, uint8_t* d_q, int64_t ldq,
                     uint8_t* d_e, int64_t lde, void* stream) {
   SUGAR_CHECK_ARG(dtype == SUGAR_F32 || dtype == SUGAR_BF16, "fp8_quant: bad dtype %d", dtype);
-  SUGAR_CHECK_ARG(rows >= 0 && cols > 0 && d_x && ldx >= cols, "fp8_quant: bad arguments");
+  SUGAR_CHECK_ARG(rows >= 0 && cols > 0 && cols < (1 << 24) && d_x && ldx >= cols, "fp8_quant: bad arguments");
   if (int rc = check_operand("fp8_quant", d_q, ldq, d_e, lde, cols)) return rc;
   if (rows == 0) return SUGAR_OK;
   const int esz = dtype == SUGAR_F32 ? 4 : 2;
@@ -174,7 +174,7 @@ int sugar_fp8_quant(const void* d_x, int64_t ldx, int dtype, int64_t rows, int c
 int sugar_fp8_dequant(const uint8_t* d_q, int64_t ldq, const uint8_t* d_e, int64_t lde, int64_t rows, int cols, void* d_y,
                       int64_t ldy, int dtype, void* stream) {
   SUGAR_CHECK_ARG(dtype == SUGAR_F32 || dtype == SUGAR_BF16, "fp8_dequant: bad dtype %d", dtype);
-  SUGAR_CHECK_ARG(rows >= 0 && cols > 0 && d_y && ldy >= cols, "fp8_dequant: bad arguments");
+  SUGAR_CHECK_ARG(rows >= 0 && cols > 0 && cols < (1 << 24) && d_y && ldy >= cols, "fp8_dequant: bad arguments");
   if (int rc = check_operand("fp8_dequant", d_q, ldq, d_e, lde, cols)) return rc;
   if (rows == 0) return SUGAR_OK;
   const int esz = dtype == SUGAR_F32 ? 4 : 2;

@@ -230,7 +230,11 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void block_join_kernel(Jo
         if (j.z_dtype == SUGAR_F32) store8((float*)j.d_z + r * j.ldz, c, C, s[k]);
         else store8((bf16*)j.d_z + r * j.ldz, c, C, s[k]);
       }
-      if (j.d_q) {                                             // (past the row s is 0: the operand's padding columns)
+      if (j.d_q) {
+        if (c + 8 > C) {                                       // the operand's padding columns are 0, whatever a norm of a bad row left there
+#pragma unroll
+          for (int i = 0; i < 8; ++i) s[k][i] = c + i < C ? s[k][i] : 0.f;
+        }
         unsigned big = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) { const unsigned u = fp8_finite_bits(s[k][i]); big = u > big ? u : big; }

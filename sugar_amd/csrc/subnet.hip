@@ -219,6 +219,8 @@ static int cat8_slice(const SugarSubnet* n) { return (int)fp8_ldq(n->c0p); }
 
 static int create(const SugarSubnetDesc* d, int dtype, SugarSubnet* n) {
   n->fp8 = dtype == SUGAR_FP8;
+  SUGAR_CHECK_ARG(!n->fp8 || d->c0 <= SUGAR_JOIN_MAX_COLS, "subnet_create: %d channels, 8-bit block ends take at most %d", d->c0,
+                  SUGAR_JOIN_MAX_COLS);
   if (n->fp8) dtype = SUGAR_BF16;
   const int E = dtype == SUGAR_F32 ? 4 : 8;
   n->dtype = dtype;

@@ -203,6 +203,17 @@ def test_argument_checks_without_a_gpu():
             call()
 
 
+def test_numbers_and_sizes_beyond_the_c_types_are_refused():
+    x = torch.zeros(3, 8)
+    wide = torch.empty(1, 1 << 24, dtype=torch.bfloat16, device="meta")
+    d, e = (t.to("meta") for t in parts(1, 128))
+    for call in (lambda: block_join(x, x, alpha=1e39), lambda: block_join(x, x, alpha=torch.ones(())), lambda: RowNorm("rms", eps=1e39),
+                 lambda: RowNorm("rms", eps=float("nan")), lambda: RowNorm("rms", eps=float("inf")), lambda: quantize_block_fp8(wide),
+                 lambda: BlockFP8(d.expand(1, 128), e, 1 << 24), lambda: block_fp8_linear(BlockFP8(*parts(3, 8), 8), BlockFP8.empty(1 << 24, 8, "meta"))):
+        with pytest.raises(ValueError):
+            call()
+
+
 def test_c_entries_check_their_arguments_before_any_launch():
     lib, p = _lib.lib(), 4096                                            # an address no call may follow
     fails = [
@@ -214,6 +225,8 @@ def test_c_entries_check_their_arguments_before_any_launch():
         lib.sugar_fp8_quant(p, 8, 0, 1, 8, p + 8, 128, p, 4, None),
         lib.sugar_fp8_quant(p, 8, 0, 1, 8, p, 120, p, 4, None),
         lib.sugar_fp8_quant(p, 8, 0, 1, 8, p, 128, p, 2, None),
+        lib.sugar_fp8_quant(p, 1 << 24, 1, 1, 1 << 24, p, 1 << 24, p, 1 << 17, None),
+        lib.sugar_fp8_dequant(p, 1 << 24, p, 1 << 17, 1, 1 << 24, p, 1 << 24, 1, None),
         lib.sugar_fp8_dequant(p, 128, p + 1, 4, 1, 8, p, 8, 0, None),
         lib.sugar_fp8_dequant(p, 128, p, 4, 1, 8, p, 7, 0, None),
         lib.sugar_fp8_linear(p, 128, p, 4, 1, p, 128, p, 4, 0, 8, None, None, 0, p, 8, 0, None),
@@ -373,6 +386,23 @@ def test_linear_scales_reach_every_block():
 
 
 @gpu
+@pytest.mark.parametrize("r", [3, 300])
+def test_linear_tiny_times_huge(r):
+    """Blocks at the lower end of the exponents (values down to e4m3's smallest times 2^-127) against blocks near the upper
+    end.  float32 outputs take the values as bfloat16 numbers: what lies below that type's subnormals is off by at most half
+    of the smallest, 2^-134, each; the 8-bit instruction scales behind the product and loses nothing there."""
+    k, n = 300, 72
+    x, wt = rows_of(1, r, k, spread=0.5) * 2.0 ** -122, rows_of(2, n, k, spread=0.3) * 2.0 ** 100
+    a, w = quantize_block_fp8(x.cuda()), quantize_block_fp8(wt.cuda())
+    assert a.exponent[:, :3].min() == 0 and 215 < w.exponent[:, :3].max() < 247
+    check_linear(a, w, dtype=torch.bfloat16)
+    y, mag = linear64(a, w, None, None, False)
+    got = block_fp8_linear(a, w, out_dtype=torch.float32).cpu().double()
+    lost = 2.0 ** -134 * values64(w).abs().sum(1)
+    assert ((got - y).abs() <= (k + 4) * U32 * mag + lost).all()
+
+
+@gpu
 def test_linear_strides_slices_and_untouched_surroundings():
     a, w = operands(11, 90, 60, 600)
     full = block_fp8_linear(a, w)
@@ -512,6 +542,33 @@ def test_outputs_that_share_memory_are_refused():
             bad()
 
 
+@gpu
+def test_outputs_passed_in_with_any_form_of_the_gate():
+    """Gates and row offsets that are no plain matrix or vector (transposed, other types, every second entry) next to outputs
+    of the caller's; an output that requires a gradient; an operand whose parts lie in each other."""
+    c, r = 136, 24
+    u, res = rows_of(1, r, c, torch.bfloat16).cuda(), rows_of(2, r, c, torch.bfloat16).cuda()
+    off = torch.tensor([0, 7, 10, 3, 24, 9], dtype=torch.int32).cuda()[::2]
+    gate = torch.rand(c, 2).cuda()
+    for kw in (dict(gate=gate.T, row_off=off), dict(gate=gate.T.bfloat16(), row_off=off), dict(gate=torch.rand(c, r).cuda().bfloat16().T),
+               dict(gate=torch.rand(2 * c).cuda()[::2]), dict(gate=torch.rand(c).cuda().double())):
+        want = block_join(u, res, **kw)
+        out = torch.empty_like(u)
+        got = block_join(u, res, stream_out=out, **kw)
+        assert got.stream is out and torch.equal(out, want.stream) and torch.equal(got.normed, want.normed)
+        check_join(want, u, res, **kw)
+    leaf = torch.zeros(r, c, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    q = quantize_block_fp8(u)
+    raw = torch.zeros(r, 1024, dtype=torch.uint8, device="cuda")
+    inside = BlockFP8(raw[:, :256].view(torch.float8_e4m3fn), raw[:, 128:132], c)
+    for bad in (lambda: block_join(u, res, stream_out=leaf), lambda: block_fp8_linear(q, q, out=leaf[:, :r]), lambda: q.dequantize(out=leaf),
+                lambda: quantize_block_fp8(u, out=inside)):
+        with pytest.raises(ValueError):
+            bad()
+    with torch.no_grad():
+        assert torch.equal(q.dequantize(out=leaf), q.dequantize(torch.bfloat16))
+
+
 def stream_like(x):
     return torch.empty_like(x)
 
@@ -528,6 +585,20 @@ def test_join_non_finite_rows_do_not_spread():
     zero = torch.zeros(4, c).cuda()                                      # rows of zeros: eps keeps the norm finite
     j = block_join(zero, zero, post=RowNorm("rms"), pre=RowNorm("layer"), quantized=True)
     assert (j.normed == 0).all() and (values64(j.quantized) == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("c", [200, 520, 1100])
+def test_join_pads_bad_rows_with_zeros(c):
+    """Rows that a norm makes NaN throughout, an infinite factor: the padding columns of the 8-bit output stay 0 and the rest
+    is the quantisation of the float32 output."""
+    u, res = rows_of(1, 9, c), rows_of(2, 9, c)
+    u[3, 17], res[5, c - 1], u[6] = float("inf"), float("nan"), 0.0
+    for kw in (dict(post=norm_of("layer", c, 3), pre=norm_of("layer", c, 5)), dict(alpha=float("inf")), dict(alpha=float("nan")),
+               dict(gate=torch.rand(c).cuda(), alpha=float("-inf"), pre=norm_of("affine", c, 5))):
+        j = block_join(u.cuda(), res.cuda(), quantized=True, **kw)
+        check_quantised(j.quantized, j.normed)
+        assert (j.quantized.data.view(torch.uint8)[:, c:(c + 127) // 128 * 128] == 0).all()
 
 
 # ------------------------------------------------------------------------------------------------ together, streams, graphs
