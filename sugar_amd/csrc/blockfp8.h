@@ -68,7 +68,6 @@ __device__ __forceinline__ u32x2 fp8_pack8(const float* v, float inv) {
 // loads and stores take any address (one instruction either way).
 typedef bf16x8 bf16x8_u __attribute__((aligned(2)));
 typedef f32x4 f32x4_u __attribute__((aligned(4)));
-typedef u32x4 u32x4_u __attribute__((aligned(2)));
 
 // Eight consecutive elements from channel c on; those past `n` (the row's channels) read as 0.
 template <typename T>
@@ -132,8 +131,8 @@ __device__ __forceinline__ f32x4 mfma_fp8(i32x8 a, i32x8 b, f32x4 c, int ea, int
 }
 
 // float32 outputs: the same block as four 16-bit products on the values converted to bf16, block scale included (the
-// conversion instruction applies a power of two; an e4m3 value times one is a bf16 value down to the subnormals, byte 255
-// gives NaN), whose sums are good to f32 (4.6e-8 off on the same operands), at half the rate.  Conversions are one
+// conversion instruction applies a power of two; an e4m3 value times one is a bf16 value from bf16's smallest subnormal,
+// 2^-133, up to 2^128, byte 255 gives NaN), whose sums are good to f32 (4.6e-8 off on the same operands), at half the rate.  Conversions are one
 // instruction per two values and lie under the other wave's products.
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 __device__ __forceinline__ void fp8_to_bf16(i32x8 q, int byte, bf16x8 (&h)[4]) {
