@@ -157,3 +157,59 @@ def test_host_packed_weights_are_the_quantisers(supernet):
     mag = outs.double().abs() @ w.double().abs().t()
     assert ((got - want).abs() <= 2.0 ** -8 * want + 2.0 ** -10 * mag).all()
     sub.release()
+
+
+class _Utts:
+    """Stand-in for sugar.database.Utterance: items are {"file", "input": [1, L]}."""
+
+    def __init__(self, wavs):
+        self.wavs = wavs
+
+    def __len__(self):
+        return len(self.wavs)
+
+    def __getitem__(self, i):
+        return {"file": "utt%04d.wav" % i, "input": self.wavs[i].unsqueeze(0)}
+
+
+class _Trials(list):
+    utterances = None
+
+
+class _Loader:
+    def __init__(self, dataset, batch_size):
+        self.dataset, self.batch_size, self.num_workers = dataset, batch_size, 0
+
+
+@gpu
+def test_lists_and_sweeps(supernet, meta):
+    """extract_vectors over a staged list, its features kept or not, against the model's own forward; a sweep over subnets in
+    this precision, with and without recalibration, against one model at a time."""
+    n = 12
+    wavs = synth.ragged_waveforms(synth.ragged_lengths(n, lo=20000, hi=40000, seed=13).tolist(), seed=13)
+    utts = _Utts(wavs)
+    model = model_of(supernet, layout.BASE, "fp8")
+    want = model([w.to(DEV) for w in wavs], normalize=True)
+    tables = []
+    for keep in (False, True, True):
+        packed = sugar_amd.PackedUtterances(utts, DEV, batch_size=5, cache_features=keep)
+        tables += [sugar_amd.extract_vectors(model, packed).matrix.clone() for _ in range(2)]
+    assert all(torch.equal(t, tables[0]) for t in tables[1:])
+    # other batches: another kernel may serve the same row (float32 sums in another order, then the same bf16 roundings)
+    assert F.cosine_similarity(tables[0].double(), want.double(), dim=1).min() >= 0.9999
+    lab, a, b = synth.trial_pairs(n, 120, seed=13)
+    trials = _Trials({"label": int(lab[i]), "enroll": "utt%04d.wav" % a[i], "test": "utt%04d.wav" % b[i]} for i in range(len(lab)))
+    trials.utterances = utts
+    loader = _Loader(trials, 4)
+    configs = [layout.SMALLEST, layout.BASE, CONFIGS["three_blocks"]]
+    recal = [(synth.waveforms(6, 32000, seed=40),)]
+    for recal_loader in (None, recal):
+        got = sugar_amd.evaluate_subnets(supernet, configs, loader, recal_loader=recal_loader, device=DEV, precision="fp8")
+        assert len(got) == len(configs)
+        for cfg in configs:
+            one = model_of(supernet, cfg, "fp8")
+            if recal_loader is not None:
+                sugar_amd.batch_forward(recal_loader, one, device=DEV)
+            eer, dcf = sugar_amd.veri_validate(loader, one, device=DEV)
+            r = got[(cfg[0], tuple(cfg[1]), tuple(cfg[2]), cfg[3])]
+            assert r["eer"] == eer[0] and r["mindcf"] == dcf[0], (recal_loader is not None, cfg)
