@@ -68,54 +68,87 @@ __device__ __forceinline__ u32x2 fp8_pack8(const float* v, float inv) {
 // loads and stores take any address (one instruction either way).
 typedef bf16x8 bf16x8_u __attribute__((aligned(2)));
 typedef f32x4 f32x4_u __attribute__((aligned(4)));
+template <typename T, int N>
+struct Run { typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T)))); };
+
+// What a lane read at element n - 8 of a row of n >= 8 elements, because its own 8 from element c on reach past the end ->
+// those 8, zeros from n on.  The distance is 8 - n % 8 for the one lane with the row's last elements (a shift that is the same
+// in the whole launch, in three steps); lanes wholly behind the row hold zeros.  (Read one by one,
+// those elements made 48 000 x 511 bf16 rows cost 64 us instead of 42 in the join with two norms, 23 instead of 16 in the
+// quantiser; 512 columns: 33 and 16.)
+__device__ __forceinline__ void ragged_end(float* v, int c, int n) {
+  if (c + 8 <= n) return;
+  const int s = 8 - (n & 7);
+  if (s & 1) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i + 1 < 8 ? v[i + 1] : 0.f;
+  }
+  if (s & 2) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i + 2 < 8 ? v[i + 2] : 0.f;
+  }
+  if (s & 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i + 4 < 8 ? v[i + 4] : 0.f;
+  }
+  if (c >= n) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.f;
+  }
+}
 
 // Eight consecutive elements from channel c on; those past `n` (the row's channels) read as 0.
 template <typename T>
 __device__ __forceinline__ void load8(const T* __restrict__ p, int c, int n, float* v) {
-  if (c + 8 <= n) {
-    if constexpr (sizeof(T) == 2) {
-      const bf16x8 t = *(const bf16x8_u*)(p + c);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
-    } else {
-      const f32x4 t0 = *(const f32x4_u*)(p + c), t1 = *(const f32x4_u*)(p + c + 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { v[i] = t0[i]; v[4 + i] = t1[i]; }
-    }
-  } else {
+  if (n < 8) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = c + i < n ? to_f32(p[c + i]) : 0.f;
+    return;
   }
+  p += min(c, n - 8);
+  if constexpr (sizeof(T) == 2) {
+    const bf16x8 t = *(const bf16x8_u*)p;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
+  } else {
+    const f32x4 t0 = *(const f32x4_u*)p, t1 = *(const f32x4_u*)(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[i] = t0[i]; v[4 + i] = t1[i]; }
+  }
+  ragged_end(v, c, n);
+}
+
+// The first m (1 .. 7) of eight: runs of 4, 2 and 1.
+template <typename T>
+__device__ __forceinline__ void store_first(T* __restrict__ p, int m, typename Run<T, 8>::type t) {
+  if (m & 4) *(typename Run<T, 4>::type*)p = t.lo;
+  const typename Run<T, 4>::type r = m & 4 ? t.hi : t.lo;             // what is left: at most 3
+  if (m & 2) *(typename Run<T, 2>::type*)(p + (m & 4)) = r.lo;
+  const T last = m & 2 ? r.z : r.x;
+  if (m & 1) p[m & 6] = last;
 }
 
 template <typename T>
 __device__ __forceinline__ void store8(T* __restrict__ p, int c, int n, const float* v) {
+  typename Run<T, 8>::type t;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t[i] = from_f32<T>(v[i]);
   if (c + 8 <= n) {
     if constexpr (sizeof(T) == 2) {
-      bf16x8 t;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] = (bf16)v[i];
       *(bf16x8_u*)(p + c) = t;
     } else {
-      *(f32x4_u*)(p + c) = (f32x4){v[0], v[1], v[2], v[3]};
-      *(f32x4_u*)(p + c + 4) = (f32x4){v[4], v[5], v[6], v[7]};
+      *(f32x4_u*)(p + c) = t.lo;
+      *(f32x4_u*)(p + c + 4) = t.hi;
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c + i < n) p[c + i] = from_f32<T>(v[i]);
+  } else if (c < n) {
+    store_first(p + c, n & 7, t);
   }
 }
 
 // eight bf16 of a row of n channels from channel c on, as they lie in memory
 __device__ __forceinline__ void store_bf16x8(bf16* __restrict__ y, int c, int n, bf16x8 o) {
-  if (c + 8 <= n) {
-    *(bf16x8_u*)(y + c) = o;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c + i < n) y[c + i] = o[i];
-  }
+  if (c + 8 <= n) *(bf16x8_u*)(y + c) = o;
+  else if (c < n) store_first(y + c, n & 7, o);
 }
 
 // ---- products -------------------------------------------------------------------------------------------------------

@@ -52,34 +52,27 @@ __device__ __forceinline__ float row_total(float v, float* red, int wv) {
 }
 
 // Eight channels as they lie in memory, fetched without a branch and without touching the values, so that every load of a
-// row is on its way before the first is used: 16-byte loads, a lane that is not whole inside the row reads the row's
-// beginning.  The lane with the last n % 8 channels fetches them one by one when it is asked for the values.
-// WIDE: rows of 8 channels and more; shorter ones are read one by one altogether.
+// row is on its way before the first is used: 16-byte loads, a lane that reaches past the row's end reads the row's last 8
+// (ragged_end puts them right).  WIDE: rows of 8 channels and more; shorter ones are read one by one altogether.
 template <typename T, bool WIDE>
 struct Raw8 {
   typedef typename std::conditional<sizeof(T) == 2, bf16x8_u, f32x4_u>::type Chunk;
   Chunk q[sizeof(T) / 2];
   __device__ __forceinline__ void load(const T* __restrict__ p, int c, int n) {
     if constexpr (WIDE) {
-      const Chunk* s = (const Chunk*)(p + (c + 8 <= n ? c : 0));
+      const Chunk* s = (const Chunk*)(p + min(c, n - 8));
 #pragma unroll
       for (int i = 0; i < (int)sizeof(T) / 2; ++i) q[i] = s[i];
     }
   }
   __device__ __forceinline__ void get(const T* __restrict__ p, float* v, int c, int n) const {
     if constexpr (WIDE) {
-      const bool in = c + 8 <= n;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = in ? to_f32(q[i * sizeof(T) / 16][i % (16 / sizeof(T))]) : 0.f;
-    }
-    if (!WIDE || (n & 7)) {
-      if (c < n && c + 8 > n) {
+      for (int i = 0; i < 8; ++i) v[i] = to_f32(q[i * sizeof(T) / 16][i % (16 / sizeof(T))]);
+      ragged_end(v, c, n);
+    } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c + i < n ? to_f32(p[c + i]) : 0.f;
-      } else if (!WIDE) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.f;
-      }
+      for (int i = 0; i < 8; ++i) v[i] = c + i < n ? to_f32(p[c + i]) : 0.f;
     }
   }
 };

@@ -727,3 +727,47 @@ def test_linear_huge_operand_offsets():
     keep[probe] = False
     bad = ((y.double() - ones.cuda()).abs() > ((k + 4) * U32 * mag).cuda()).any(1) & keep
     assert not bad.any()
+
+
+@gpu
+@pytest.mark.parametrize("c", [8, 9, 15, 121, 127, 130, 253, 519, 1027])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_every_end_of_a_row(c, dtype):
+    """Rows whose last 1 .. 7 columns are no whole group of eight, inside a wider buffer whose other columns are NaN (nothing of
+    them may come in) or 7 (nothing may be written there)."""
+    r = 21
+    big = torch.full((r, c + 11), float("nan"), dtype=dtype)
+    big[:, 3:3 + c] = rows_of(c, r, c, dtype)
+    x = big.cuda()[:, 3:3 + c]
+    q = quantize_block_fp8(x)
+    check_quantised(q, big[:, 3:3 + c])
+    out = torch.full((r, c + 11), 7.0, dtype=dtype, device="cuda")
+    q.dequantize(out=out[:, 5:5 + c])
+    assert torch.equal(out[:, 5:5 + c].cpu().double(), values64(q)) and (out[:, :5] == 7).all() and (out[:, 5 + c:] == 7).all()
+    gate, res = torch.full((r, c + 4), float("nan"), dtype=dtype, device="cuda"), rows_of(c + 1, r, c, dtype).cuda()
+    gate[:, 1:1 + c] = torch.rand(r, c).to(dtype)
+    kw = dict(post=norm_of("layer", c, 3), pre=norm_of("rms", c, 5), gate=gate[:, 1:1 + c])
+    stream, z = (torch.full((r, c + 11), 7.0, dtype=dtype, device="cuda") for _ in range(2))
+    check_join(block_join(x, res, stream_out=stream[:, 1:1 + c], normed_out=z[:, 4:4 + c], quantized=True, **kw), x, res, **kw)
+    for t, lo in ((stream, 1), (z, 4)):
+        assert (t[:, :lo] == 7).all() and (t[:, lo + c:] == 7).all()
+    w = quantize_block_fp8(rows_of(c + 2, c, 200, spread=0.2).cuda() / 14)
+    a = quantize_block_fp8(rows_of(c + 3, 900, 200).cuda())
+    for rows in (3, 900):                                                 # the direct kernel's and the tiles' stores
+        out = torch.full((rows, c + 11), 7.0, dtype=dtype, device="cuda")
+        check_linear(a[:rows], w, dtype=dtype, out=out[:, 2:2 + c])
+        assert (out[:, :2] == 7).all() and (out[:, 2 + c:] == 7).all()
+
+
+@gpu
+def test_quantise_more_rows_than_one_launch_takes():
+    r = (1 << 27) + 77
+    x = torch.ones(r, 1, dtype=torch.bfloat16, device="cuda")
+    probe = [0, 1, (1 << 27) - 1, 1 << 27, (1 << 27) + 1, r - 1]
+    x[probe] = torch.tensor([[3.0], [-0.3], [500.0], [-7.0], [1e-30], [0.11]], dtype=torch.bfloat16, device="cuda")
+    q = quantize_block_fp8(x)
+    for i in probe:
+        check_quantised(q[i:i + 1], x[i:i + 1])
+    y = q.dequantize(torch.bfloat16)
+    assert (y[probe] != 1).all() and int((y == 1).sum()) == r - len(probe)
+    assert bool((q.exponent[:, 0] == 119).sum() == r - len(probe)) and bool((q.exponent[:, 1:] == 127).all())
