@@ -137,22 +137,26 @@ __global__ __launch_bounds__(64 * NW) void fp8_linear_direct_kernel(LinearArgs p
 }
 
 // ------------------------------------------------------------------------------------------ one tile
-// One TM x TN output tile by a workgroup of 8 waves = 2 (channels) x 4 (rows).  Two stages: wait for this wave's share of
+// One TM x TN output tile by a workgroup of NW waves = 2 (channels) x NW / 2 (rows).  Two stages: wait for this wave's share of
 // k-tile t, barrier, issue the DMA of k-tile t + 1 into the buffer k-tile t - 1 was read from, compute; what a workgroup
 // waits for the DMA, the two to four others of its CU fill.  Exponents travel as one dword per row and four k-tiles, staged
 // with the first of the four (double buffer) and shifted down a byte per k-tile.
 // Bound by the DMA into LDS (128 x 128 tiles: 64 operations a byte) and, at few k-tiles, by the first tile's way in and the
-// stores: 301 x 1536 -> 1536 6.1 us (64 x 64), float32 output 8.4; 19264 x 528 -> 536 13.4 us, float32 21.7.
+// stores: 301 x 1536 -> 1536 6.1 us (64 x 64), float32 output 8.4; 19264 x 528 -> 536 13.4 us, float32 23.6.
+// 128 x 128 with float32 outputs: 4 waves of 64 x 64 convert 8 fragments for 16 products where 8 waves of 64 x 32 convert 6 for
+// 8; 77056 x 1536 -> 1536 352 us (1.03 PF) against 377, x 512 -> 512 54 / 57, x 128 -> 192 (154112 rows) 30.5 / 29.1.  Left
+// out one at a time (8 waves): conversions 70 us, products 67, stores 79.  A persistent form that fetches the next tile under
+// the epilogue and spreads the stores over its k-loop was built and dropped: 362.
 constexpr int linear_tile_lds(int TM, int TN) { return (TM + TN) * (2 * 128 + 8) + 8 * TM; }
 
-template <int TM, int TN, bool WIDE>
+template <int TM, int TN, int NW, bool WIDE>
 __device__ __forceinline__ void fp8_tile(const LinearArgs& p, const int co_base, const int r_base) {
   constexpr int STAGE_BYTES = (TM + TN) * 128;
-  constexpr int MI = TM / 32, NJ = TN / 64, CW = TM / 2, FW = TN / 4, WI = TM / 64, XI = TN / 64, SI = (TM + TN) / 64;
-  static_assert(SI <= 8, "one exponent instruction per wave");
+  constexpr int WN = NW / 2, CW = TM / 2, FW = TN / WN, MI = CW / 16, NJ = FW / 16, WI = TM / (8 * NW), XI = TN / (8 * NW), SI = (TM + TN) / 64;
+  static_assert(SI <= NW && TM / 32 <= NW, "one exponent, one affine instruction per wave");
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wv >> 2, wn = wv & 3, fr = lane & 15, fq = lane >> 4;
+  const int wm = wv / WN, wn = wv % WN, fr = lane & 15, fq = lane >> 4;
   unsigned* exps = (unsigned*)(smem + 2 * STAGE_BYTES);          // [2][TM + TN]
   float* aff = (float*)(exps + 2 * (TM + TN));                   // [scale | shift][TM], fetched with the first k-tile
   const int nk = p.kb;
@@ -265,7 +269,7 @@ __device__ __forceinline__ void fp8_tile(const LinearArgs& p, const int co_base,
   }
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // stage memory becomes the epilogue staging
   constexpr int EPI_STRIDE = CW * 2 + 16, CPR = CW / 8, RPP = 64 / CPR;
-  static_assert(8 * 16 * EPI_STRIDE <= 2 * STAGE_BYTES, "epilogue staging fits the stages");
+  static_assert(NW * 16 * EPI_STRIDE <= 2 * STAGE_BYTES, "epilogue staging fits the stages");
   unsigned char* ep = smem + wv * (16 * EPI_STRIDE);             // this wave's [16 rows][CW channels]
 #pragma unroll
   for (int n = 0; n < NJ; ++n) {
@@ -291,20 +295,24 @@ __device__ __forceinline__ void fp8_tile(const LinearArgs& p, const int co_base,
   }
 }
 
-template <int TM, int TN, bool WIDE>
-__global__ __launch_bounds__(512, 4) void fp8_linear_tile_kernel(LinearArgs p) {
+template <int TM, int TN, int NW, bool WIDE>
+__global__ __launch_bounds__(64 * NW, NW / 2) void fp8_linear_tile_kernel(LinearArgs p) {
   const int vid = xcd_remap(blockIdx.x, gridDim.x);
-  fp8_tile<TM, TN, WIDE>(p, (vid % p.n_co_tiles) * TM, (vid / p.n_co_tiles) * TN);
+  const int co = (vid % p.n_co_tiles) * TM, r = (vid / p.n_co_tiles) * TN;
+  // a last tile that is less than half full as half a tile: float32 outputs 3 .. 6 % faster (19264 x 528 -> 536 24.9 -> 23.6 us,
+  // 40000 x 700 -> 300 30.2 -> 28.6), bf16 ones between 3 % faster and 8 % slower (the same: 14.0 -> 15.1, 12.5 -> 12.2)
+  if (WIDE && TM > 64 && p.n - co <= 64) fp8_tile<64, TN, NW, WIDE>(p, co, r);
+  else fp8_tile<TM, TN, NW, WIDE>(p, co, r);
 }
 
-template <int TM, int TN, bool WIDE>
+template <int TM, int TN, int NW, bool WIDE>
 int launch_tile(LinearArgs p, hipStream_t s) {
   constexpr int smem = linear_tile_lds(TM, TN);
   static OptInMask opted{0};
-  if (int rc = lds_opt_in((const void*)fp8_linear_tile_kernel<TM, TN, WIDE>, smem, &opted)) return rc;
+  if (int rc = lds_opt_in((const void*)fp8_linear_tile_kernel<TM, TN, NW, WIDE>, smem, &opted)) return rc;
   p.n_co_tiles = (int)ceil_div(p.n, TM);
   const int64_t grid = p.n_co_tiles * ceil_div(p.rows, TN);
-  hipLaunchKernelGGL((fp8_linear_tile_kernel<TM, TN, WIDE>), dim3((unsigned)grid), dim3(512), smem, s, p);
+  hipLaunchKernelGGL((fp8_linear_tile_kernel<TM, TN, NW, WIDE>), dim3((unsigned)grid), dim3(64 * NW), smem, s, p);
   SUGAR_LAUNCH_CHECK();
   return SUGAR_OK;
 }
@@ -704,9 +712,9 @@ __global__ __launch_bounds__(512, 2) void fp8_linear_persist_kernel(LinearArgs p
     const int tile = rounds * nwg + i / split, sub = i % split;
     const int co_base = (tile % p.n_co_tiles) * PT, r_tile = (tile / p.n_co_tiles) * PT;
     if (split == 4) {
-      if (r_tile + sub * 64 < p.rows) fp8_tile<256, 64, false>(p, co_base, r_tile + sub * 64);
+      if (r_tile + sub * 64 < p.rows) fp8_tile<256, 64, 8, false>(p, co_base, r_tile + sub * 64);
     } else {
-      if (r_tile + sub * 128 < p.rows) fp8_tile<256, 128, false>(p, co_base, r_tile + sub * 128);
+      if (r_tile + sub * 128 < p.rows) fp8_tile<256, 128, 8, false>(p, co_base, r_tile + sub * 128);
     }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the piece's epilogue staging has been read
   }
@@ -754,10 +762,10 @@ int launch_rows(const LinearArgs& p, hipStream_t s) {
   if (!f32 && !p.y2 && p.kb >= 8 && n_cu % 8 == 0 && ceil_div(p.n, 256) * ceil_div(p.rows, 256) >= 2 * n_cu)
     return launch_persist(p, n_cu, s);
   if (ceil_div(p.n, 128) * ceil_div(p.rows, 128) >= n_cu)
-    return f32 ? launch_tile<128, 128, true>(p, s) : launch_tile<128, 128, false>(p, s);
+    return !f32 ? launch_tile<128, 128, 8, false>(p, s) : p.kb >= 4 ? launch_tile<128, 128, 4, true>(p, s) : launch_tile<128, 128, 8, true>(p, s);
   if (4 * ceil_div(p.n, 64) * ceil_div(p.rows, 128) >= 3 * n_cu)
-    return f32 ? launch_tile<64, 128, true>(p, s) : launch_tile<64, 128, false>(p, s);
-  return f32 ? launch_tile<64, 64, true>(p, s) : launch_tile<64, 64, false>(p, s);
+    return f32 ? launch_tile<64, 128, 8, true>(p, s) : launch_tile<64, 128, 8, false>(p, s);
+  return f32 ? launch_tile<64, 64, 8, true>(p, s) : launch_tile<64, 64, 8, false>(p, s);
 }
 
 }  // namespace
