@@ -24,7 +24,8 @@ NORMS = {"affine": 1, "rms": 2, "layer": 3}
 MAX_JOIN_COLS = 8192
 MAX_COLS = 1 << 24                                     # channels of an operand, outputs of a product (32-bit integers at the C ABI)
 F32_MAX, INF = torch.finfo(torch.float32).max, float("inf")
-_raw_stream = torch._C._cuda_getCurrentRawStream       # (torch.cuda.current_stream builds an object, 1 us of a 10 us call)
+# (torch.cuda.current_stream builds an object, torch.cuda.current_device looks whether the GPU is initialised: 1.3 us of a 10 us call)
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 _FN = {}
 
 
@@ -41,11 +42,10 @@ def _gpu(dev):
 def _same_device(dev, tensors):
     """All on `dev` (a GPU), none of them part of a recorded gradient."""
     _gpu(dev)
-    grad = torch.is_grad_enabled()
     for t in tensors:
         if t.device != dev:
             raise ValueError("tensors on %s and %s" % (dev, t.device))
-        if grad and t.requires_grad:
+        if t.requires_grad and torch.is_grad_enabled():
             raise ValueError("no backward pass: call under torch.no_grad() or detach the inputs")
 
 
@@ -55,7 +55,7 @@ def _call(dev, name, *args):
     if fn is None:
         fn = _FN[name] = getattr(_lib.lib(), name)
     idx = dev.index
-    if torch.cuda.current_device() == idx:
+    if _current_device() == idx:
         rc = fn(*args, _raw_stream(idx))
     else:
         with torch.cuda.device(idx):
@@ -65,18 +65,22 @@ def _call(dev, name, *args):
 
 
 def _rows(what, x):
-    """x as a matrix whose columns lie next to each other (a copy when they do not), and its row stride."""
-    if x.dim() != 2 or x.shape[1] == 0:
-        raise ValueError("%s: expected [rows, columns], got %s" % (what, tuple(x.shape)))
-    if x.dtype not in _DT:
+    """x as a matrix whose columns lie next to each other (a copy when they do not), its rows, columns, row stride, type."""
+    shape = x.shape
+    if len(shape) != 2 or shape[1] == 0:
+        raise ValueError("%s: expected [rows, columns], got %s" % (what, tuple(shape)))
+    rows, cols = shape
+    dtype = _DT.get(x.dtype)
+    if dtype is None:
         raise ValueError("%s: dtype %s not in %s" % (what, x.dtype, [str(d) for d in _DT]))
-    if x.shape[1] >= MAX_COLS:
-        raise ValueError("%s: %d columns, fewer than %d are taken" % (what, x.shape[1], MAX_COLS))
-    ld = _row_stride(x)
-    if ld is None:
-        x = x.contiguous()
-        ld = x.shape[1]
-    return x, ld
+    if cols >= MAX_COLS:
+        raise ValueError("%s: %d columns, fewer than %d are taken" % (what, cols, MAX_COLS))
+    ld, step = x.stride()
+    if step != 1 or ld < cols:                          # (all but the plain case)
+        ld = _row_stride(x)
+        if ld is None:
+            x, ld = x.contiguous(), cols
+    return x, rows, cols, ld, dtype
 
 
 def _row_stride(x):
@@ -104,27 +108,28 @@ def _out(what, out, shape, dtypes, dev):
     return ld
 
 
-def _memory(t, ld=None):
-    """(first byte, bytes of a row, bytes from row to row, rows) of a matrix, vector or BlockFP8 part."""
-    if t.dim() == 1:
-        return t.data_ptr(), t.shape[0] * t.element_size(), 0, 1
-    size = t.element_size()
-    return t.data_ptr(), t.shape[1] * size, (_row_stride(t) if ld is None else ld) * size, t.shape[0]
+def _span(t, ld=0):
+    """(first byte, bytes of a row, bytes from row to row, rows) of a matrix with row stride `ld`, or of a vector."""
+    shape, size = t.shape, t.element_size()
+    if len(shape) == 1:
+        return t.data_ptr(), shape[0] * size, 0, 1
+    return t.data_ptr(), shape[1] * size, ld * size, shape[0]
 
 
-def _apart(what, out, others, same=()):
-    """An output passed in must not share memory with what a call reads or writes besides it, except be one of `same`
-    itself (same first element and strides).  Column slices of one buffer are apart."""
-    p, width, step, rows = _memory(out)
-    for t in others:
-        q, w, st, r = _memory(t)
-        if not rows or not r or p >= q + (r - 1) * st + w or q >= p + (rows - 1) * step + width:
+def _apart(what, out, others, itself=()):
+    """The memory of an output that was passed in (a _span) must not be that of anything else a call reads or writes, save
+    exactly that of one of `itself`.  Column slices of one buffer are apart."""
+    p, width, step, rows = out
+    end = p + (rows - 1) * step + width
+    for other in others:
+        q, w, st, r = other
+        if q >= end or p >= q + (r - 1) * st + w or not rows or not r:
             continue
         if st == step and step:
             off = (q - p) % step
             if off >= width and off + w <= step:
                 continue
-        if any(t is x for x in same) and p == q and step == st and t.dtype == out.dtype:
+        if other == out and other in itself:
             continue
         raise ValueError("%s: the output shares memory with another operand" % what)
 
@@ -171,9 +176,9 @@ class BlockFP8(object):
     def empty(cls, rows, cols, device):
         """An operand to be written into: one allocation, values and exponents one behind the other."""
         self = cls.__new__(cls)
-        blocks = -(-int(cols) // cls.BLOCK)
-        self.rows, self.cols, self._ld, self._lde = int(rows), int(cols), blocks * cls.BLOCK, _up(blocks, 4)
-        self._buf = torch.empty(self.rows * (self._ld + self._lde), dtype=torch.uint8, device=device)
+        blocks = (cols + 127) >> 7
+        self.rows, self.cols, self._ld, self._lde = rows, cols, blocks << 7, (blocks + 3) & -4
+        self._buf = torch.empty(rows * (self._ld + self._lde), dtype=torch.uint8, device=device)
         self._data = self._exponent = None
         return self
 
@@ -182,6 +187,12 @@ class BlockFP8(object):
             return self._data.data_ptr(), self._exponent.data_ptr()
         p = self._buf.data_ptr()
         return p, p + self.rows * self._ld
+
+    def _spans(self):
+        """_span of the values and of the exponents."""
+        d, e = self._pointers()
+        return [(d, self._ld if self._buf is not None else self._data.shape[1], self._ld, self.rows),
+                (e, self._lde if self._buf is not None else self._exponent.shape[1], self._lde, self.rows)]
 
     def _split(self):
         n = self.rows * self._ld
@@ -223,7 +234,7 @@ class BlockFP8(object):
             out, ld = torch.empty((rows, cols), dtype=dtype, device=dev), cols
         else:
             ld = _out("dequantize", out, (rows, cols), _DT, dev)
-            _apart("dequantize", out, (self.data, self.exponent))
+            _apart("dequantize", _span(out, ld), self._spans())
         if rows:
             d, e = self._pointers()
             _call(dev, "sugar_fp8_dequant", d, self._ld, e, self._lde, rows, cols, out.data_ptr(), ld, _DT[out.dtype])
@@ -235,7 +246,9 @@ def _fp8_out(what, out, rows, cols, dev):
         return BlockFP8.empty(rows, cols, dev)
     if not isinstance(out, BlockFP8) or out.rows != rows or out.cols != cols or out.device != dev:
         raise ValueError("%s: expected a BlockFP8 of [%d, %d] on %s" % (what, rows, cols, dev))
-    _apart(what, out.data, (out.exponent,))
+    if out._buf is None:
+        data, exponent = out._spans()
+        _apart(what, data, (exponent,))
     return out
 
 
@@ -245,16 +258,15 @@ def quantize_block_fp8(x, out=None):
     keeps its largest finite magnitude within 448; values go to the nearest e4m3, ties to the even one.  Infinities and NaN
     become NaN and do not move the scale of their block.
     """
-    x, ld = _rows("quantize_block_fp8", x)
+    x, rows, cols, ld, dtype = _rows("quantize_block_fp8", x)
     dev = x.device
     _same_device(dev, (x,))
-    rows, cols = x.shape
     q = _fp8_out("quantize_block_fp8", out, rows, cols, dev)
     if out is not None:
-        _apart("quantize_block_fp8", x, (q.data, q.exponent))
+        _apart("quantize_block_fp8", _span(x, ld), q._spans())
     if rows:
         d, e = q._pointers()
-        _call(dev, "sugar_fp8_quant", x.data_ptr(), ld, _DT[x.dtype], rows, cols, d, q._ld, e, q._lde)
+        _call(dev, "sugar_fp8_quant", x.data_ptr(), ld, dtype, rows, cols, d, q._ld, e, q._lde)
     return q
 
 
@@ -288,7 +300,7 @@ def block_fp8_linear(a, w, scale=None, shift=None, relu=False, out_dtype=torch.b
         out, ld = torch.empty((rows, n), dtype=out_dtype, device=dev), n
     else:
         ld = _out("block_fp8_linear", out, (rows, n), _DT, dev)
-        _apart("block_fp8_linear", out, [t for t in (a.data, a.exponent, w.data, w.exponent, scale, shift) if t is not None])
+        _apart("block_fp8_linear", _span(out, ld), a._spans() + w._spans() + [_span(t) for t in (scale, shift) if t is not None])
     if rows:
         (ap, aep), (wp, wep) = a._pointers(), w._pointers()
         _call(dev, "sugar_fp8_linear", ap, a._ld, aep, a._lde, rows, wp, w._ld, wep, w._lde, n, k, sp, tp, flags,
@@ -339,14 +351,13 @@ def block_join(u, residual, post=None, gate=None, row_off=None, alpha=1.0, dense
     is refused.  With row_off, rows in front of the first and behind the last utterance are left as they are (in outputs
     allocated here: undefined).  alpha is a number of the host, passed by value (a captured graph keeps it).
     """
-    u, ldu = _rows("block_join: u", u)
-    residual, ldr = _rows("block_join: residual", residual)
-    rows, cols = u.shape
-    if residual.shape != u.shape:
+    u, rows, cols, ldu, u_dtype = _rows("block_join: u", u)
+    residual, r_rows, r_cols, ldr, r_dtype = _rows("block_join: residual", residual)
+    if r_rows != rows or r_cols != cols:
         raise ValueError("block_join: u %s, residual %s" % (tuple(u.shape), tuple(residual.shape)))
     if cols > MAX_JOIN_COLS:
         raise ValueError("block_join: %d columns, at most %d" % (cols, MAX_JOIN_COLS))
-    if u.dtype == torch.float32 and residual.dtype != torch.float32:
+    if u_dtype == _lib.SUGAR_F32 != r_dtype:
         raise ValueError("block_join: a float32 u needs a float32 residual")
     if isinstance(alpha, torch.Tensor) or (abs(alpha) > F32_MAX and abs(alpha) != INF):
         raise ValueError("block_join: alpha %r is no float32 number" % (alpha,))
@@ -358,37 +369,37 @@ def block_join(u, residual, post=None, gate=None, row_off=None, alpha=1.0, dense
         post_kind, post_eps, post_w, post_b = _norm("post", post, cols, inputs)
     if pre is not None:
         pre_kind, pre_eps, pre_w, pre_b = _norm("pre", pre, cols, inputs)
-    vectors = inputs[2:]
+    n_vectors = len(inputs)
     if gate is not None:
         inputs.append(gate)
     if row_off is not None:
         inputs.append(row_off)
     _same_device(dev, inputs)
-    utts = 0
+    utts = off_ptr = gate_kind = ldg = gate_ptr = 0
     if row_off is not None:
         if row_off.dim() != 1 or row_off.shape[0] < 2 or row_off.dtype != torch.int32:
             raise ValueError("block_join: row_off must be int32 [B + 1], got %s %s" % (row_off.dtype, tuple(row_off.shape)))
         row_off = row_off.contiguous()
-        utts = row_off.shape[0] - 1
-    gate_kind = ldg = 0
+        utts, off_ptr = row_off.shape[0] - 1, row_off.data_ptr()
     if gate is not None:
         if gate.dim() == 1:
             gate, gate_kind, ldg = _vector("gate", gate, cols), 1, cols
         elif row_off is not None and tuple(gate.shape) == (utts, cols):
-            gate, ldg = _rows("block_join: gate", gate if gate.dtype == torch.float32 else gate.float())
+            gate, _, _, ldg, _ = _rows("block_join: gate", gate if gate.dtype == torch.float32 else gate.float())
             gate_kind = 2
         elif row_off is None and gate.shape == u.shape and gate.dtype == u.dtype:
-            gate, ldg = _rows("block_join: gate", gate)
+            gate, _, _, ldg, _ = _rows("block_join: gate", gate)
             gate_kind = 3
         else:
             raise ValueError("block_join: gate %s %s is neither [C], [B, C] with row_off, nor [rows, C] of u's dtype without it"
                              % (gate.dtype, tuple(gate.shape)))
+        gate_ptr = gate.data_ptr()
     if stream_out is None:
         stream, lds = _like(residual, residual.dtype, rows, cols, dev), cols
     else:
         stream, lds = stream_out, _out("block_join: stream_out", stream_out, (rows, cols), (residual.dtype,), dev)
     z = q = None
-    ldz = z_dtype = 0
+    z_ptr = ldz = z_dtype = q_ptr = e_ptr = ldq = lde = 0
     if normed_out is not None:
         z, ldz = normed_out, _out("block_join: normed_out", normed_out, (rows, cols), _DT, dev)
     elif normed:
@@ -396,23 +407,27 @@ def block_join(u, residual, post=None, gate=None, row_off=None, alpha=1.0, dense
         if out_dtype not in _DT:
             raise ValueError("block_join: out_dtype %s not in %s" % (out_dtype, [str(t) for t in _DT]))
         z, ldz = _like(u, out_dtype, rows, cols, dev), cols
+    if z is not None:
+        z_ptr, z_dtype = z.data_ptr(), _DT[z.dtype]
     if quantized or quantized_out is not None:
         q = _fp8_out("block_join: quantized_out", quantized_out, rows, cols, dev)
+        (q_ptr, e_ptr), ldq, lde = q._pointers(), q._ld, q._lde
     if stream_out is not None or normed_out is not None or quantized_out is not None:
-        others = [t for t in [u, residual, gate, row_off] + vectors if t is not None]
-        parts = [] if q is None else [q.data, q.exponent]
-        _apart("block_join: stream_out", stream, others + parts, (residual, u))
+        su, sr, out = _span(u, ldu), _span(residual, ldr), _span(stream, lds)
+        others = [su, sr] + [_span(t, ldg) for t in [gate, row_off] + inputs[2:n_vectors] if t is not None]
+        parts = [] if q is None else q._spans()
+        _apart("block_join: stream_out", out, others + parts, (sr, su) if u_dtype == r_dtype else (sr,))
         if z is not None:
-            _apart("block_join: normed_out", z, others + parts + [stream], (u,))
-        for t in parts:
-            _apart("block_join: quantized_out", t, others)
+            sz = _span(z, ldz)
+            _apart("block_join: normed_out", sz, [out] + parts)
+            _apart("block_join: normed_out", sz, others, (su,) if z_dtype == u_dtype else ())
+        for span in parts:
+            _apart("block_join: quantized_out", span, others)
     if rows:
-        q_ptr, e_ptr = (0, 0) if q is None else q._pointers()
         _call(dev, "sugar_block_join", _JOIN.pack(
-            rows, cols, utts, _DT[u.dtype], _DT[residual.dtype], 0 if z is None else _DT[z.dtype], post_kind, pre_kind, gate_kind,
-            1 if dense else 0, alpha, post_eps, pre_eps, ldu, ldr, ldg, lds, ldz, 0 if q is None else q._ld, 0 if q is None else q._lde,
-            u.data_ptr(), residual.data_ptr(), post_w, post_b, pre_w, pre_b, 0 if gate is None else gate.data_ptr(),
-            0 if row_off is None else row_off.data_ptr(), stream.data_ptr(), 0 if z is None else z.data_ptr(), q_ptr, e_ptr))
+            rows, cols, utts, u_dtype, r_dtype, z_dtype, post_kind, pre_kind, gate_kind, 1 if dense else 0, alpha, post_eps, pre_eps,
+            ldu, ldr, ldg, lds, ldz, ldq, lde, u.data_ptr(), residual.data_ptr(), post_w, post_b, pre_w, pre_b, gate_ptr, off_ptr,
+            stream.data_ptr(), z_ptr, q_ptr, e_ptr))
     return JoinResult(stream, z, q)
 
 
