@@ -400,8 +400,8 @@ __global__ __launch_bounds__(512, 2) void fp8_linear_short_kernel(LinearArgs p, 
     }
   }
   // Every tile but a run's last stores all its rows; where this wave's channels are all inside too, D tiles' stores (and KB
-  // x (D - 1) rows' DMA) are younger than the DMA that is waited for.
-  const bool counted = co + 32 <= p.n && !p.y2;
+  // x (D - 1) rows' DMA, and what goes to a second output) are younger than the DMA that is waited for.
+  const bool counted = co + 32 <= p.n;
   for (int t = 0; t < nt; ++t) {
     if (t + D - 1 < nt) {
       if (counted && t >= D) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * KB + D * NST) : "memory");
