@@ -2,7 +2,7 @@
 """
 bench.py -- speaker embeddings/sec (3 s @ 16 kHz) of the MI355X-native EfficientTDNN extraction path.
 
-    python bench.py [--gpus N] [--steps K] [--warmup W] [--workload base256|largest256|wide256] [--precision bf16|fp32]
+    python bench.py [--gpus N] [--steps K] [--warmup W] [--workload base256|largest256|wide256] [--precision bf16|fp32|fp8]
     python bench.py --workload largest --global-batch 512 [--gpus N]      # BASELINE configs[2] as written: strong scaling
 
 One step = one pass of the hot path (waveforms already resident in HBM -> fused fbank -> TDNN -> L2-normalised

@@ -7,7 +7,8 @@
 // gate = the squeeze-excite scale of the row's utterance, out = y * gate + S, S += out.
 // Everything between the loads and the stores is f32 in registers: a wave (or four, for wide or few rows) holds its row,
 // so a norm's mean and its sum of squares about that mean are two exact passes over registers, not over memory, and z
-// comes from the unrounded s.  Bound: HBM (u and residual in, stream and z out).
+// comes from the unrounded s.  Bound: HBM (u and residual in, stream and z out).  Measured, bf16: 77 056 x 512 with two rms
+// norms 59 us (5.3 TB/s), dense with 8-bit output 48 (5.7); 48 611 x 1024, layer / layer, float32 stream 116 (5.1); one row 3.4.
 #include <type_traits>
 
 #include "blockfp8.h"
