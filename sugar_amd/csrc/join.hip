@@ -25,22 +25,28 @@ struct JoinArgs {
   int e_bytes;               // exponent bytes of a row that are written (the blocks, and padding where the row is an operand of its own)
 };
 
-// Sum over the 64 lanes, the same in every lane: within rows of 16 by DPP, across them by the row / half swaps (of a value
-// with itself: the two results are the two halves, each in all lanes).
-__device__ __forceinline__ float wave_total(float v) {
+// Sum over LPR neighbouring lanes, the same in every one of them: within rows of 16 by DPP, across them by the row / half
+// swaps (of a value with itself: the two results are the two halves, each in all lanes).
+template <int LPR>
+__device__ __forceinline__ float lane_total(float v) {
   v += dpp_row_f32<0xB1>(v);
   v += dpp_row_f32<0x4E>(v);
   v += dpp_row_f32<0x141>(v);
   v += dpp_row_f32<0x140>(v);
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+  if constexpr (LPR > 16) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  }
+  if constexpr (LPR > 32) {
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(b[0]) + __uint_as_float(b[1]);
+  }
+  return v;
 }
 
-template <int WPR>
+template <int WPR, int LPR>
 __device__ __forceinline__ float row_total(float v, float* red, int wv) {
-  v = wave_total(v);
+  v = lane_total<LPR>(v);
   if constexpr (WPR > 1) {
     __syncthreads();                         // the previous total has been read
     if ((threadIdx.x & 63) == 0) red[wv] = v;
@@ -97,7 +103,7 @@ struct NormVec {
 };
 
 // x <- norm(x) over the row's C channels; lanes past the row hold zeros before and after.
-template <int NCH, int WPR, bool WIDE>
+template <int NCH, int WPR, int LPR, bool WIDE>
 __device__ __forceinline__ void row_norm(float (&x)[NCH][8], int kind, const NormVec<NCH, WPR, WIDE>& p, float eps, int C, float inv_c, int cw,
                                          float* red, int wv) {
   if (kind == NORM_NONE) return;
@@ -108,7 +114,7 @@ __device__ __forceinline__ void row_norm(float (&x)[NCH][8], int kind, const Nor
     for (int k = 0; k < NCH; ++k)
 #pragma unroll
       for (int i = 0; i < 8; ++i) t += x[k][i];
-    mean = row_total<WPR>(t, red, wv) * inv_c;
+    mean = row_total<WPR, LPR>(t, red, wv) * inv_c;
   }
   if (kind != NORM_AFFINE) {
     float t = 0.f;
@@ -131,7 +137,7 @@ __device__ __forceinline__ void row_norm(float (&x)[NCH][8], int kind, const Nor
       }
       t += c < C ? tk : 0.f;
     }
-    mul = 1.0f / sqrtf(fmaf(row_total<WPR>(t, red, wv), inv_c, eps));
+    mul = 1.0f / sqrtf(fmaf(row_total<WPR, LPR>(t, red, wv), inv_c, eps));
   }
 #pragma unroll
   for (int k = 0; k < NCH; ++k)
@@ -139,25 +145,27 @@ __device__ __forceinline__ void row_norm(float (&x)[NCH][8], int kind, const Nor
     for (int i = 0; i < 8; ++i) x[k][i] = fmaf((x[k][i] - mean) * mul, p.w[k][i], p.b[k][i]);
 }
 
-// NCH x 8 channels a lane, WPR waves a row.  Each wave (WPR = 1; else each workgroup) takes a run of consecutive rows.
-template <typename TU, typename TS, int NCH, int WPR, bool WIDE, bool NORMS>
+// NCH x 8 channels a lane; WPR waves a row, or (WPR = 1) LPR lanes of a wave.  Each group of lanes that holds a row takes a run
+// of consecutive rows.
+template <typename TU, typename TS, int NCH, int WPR, int LPR, bool WIDE, bool NORMS>
 __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void block_join_kernel(JoinArgs a) {
   __shared__ float red[WPR > 1 ? WPR : 1];
   const SugarBlockJoin& j = a.j;
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const int lane = threadIdx.x & (LPR - 1), wv = threadIdx.x >> 6;
   const int C = j.cols;
   const int cw = (WPR > 1 ? wv * 512 : 0) + lane * 8;          // first channel of this lane's chunk 0
   const float inv_c = 1.0f / (float)C;
-  constexpr int RPB = WPR > 1 ? 1 : 4;                         // runs of rows a workgroup takes
-  const int64_t first = ((int64_t)blockIdx.x * RPB + (WPR > 1 ? 0 : __builtin_amdgcn_readfirstlane(wv))) * a.run;
+  constexpr int RPB = WPR > 1 ? 1 : 256 / LPR;                 // runs of rows a workgroup takes
+  const int64_t first = ((int64_t)blockIdx.x * RPB + (WPR > 1 ? 0 : LPR == 64 ? __builtin_amdgcn_readfirstlane(wv) : (int)threadIdx.x / LPR)) * a.run;
   const int64_t last = first + a.run < j.rows ? first + a.run : j.rows;
   if (first >= last) return;
   int b = 0, b_end = 0, begin = 0;
-  if (j.d_row_off) {                                           // last utterance that begins at or before the first row: 64-ary search
+  if (j.d_row_off) {                                           // last utterance that begins at or before the first row: LPR-ary search
     for (int n = j.n_utts; n > 1;) {
-      const int step = (n + 63) >> 6, i = lane * step;
-      const bool le = i < n && j.d_row_off[b + i] <= first;
-      const int k = max((int)__popcll(__ballot(le)) - 1, 0) * step;
+      const int step = (n + LPR - 1) / LPR, i = lane * step;
+      uint64_t le = __ballot(i < n && j.d_row_off[b + i] <= first);
+      if (LPR < 64) le = le >> (threadIdx.x & 63 & ~(LPR - 1)) & ((1ull << (LPR & 63)) - 1);
+      const int k = max((int)__popcll(le) - 1, 0) * step;
       b += k;
       n = min(step, n - k);
     }
@@ -194,7 +202,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void block_join_kernel(Jo
     float v[NCH][8], s[NCH][8];
 #pragma unroll
     for (int k = 0; k < NCH; ++k) ru[k].get(up, v[k], cw + k * (512 * WPR), C);
-    if (NORMS) row_norm<NCH, WPR, WIDE>(v, j.post_kind, post, j.post_eps, C, inv_c, cw, red, wv);
+    if (NORMS) row_norm<NCH, WPR, LPR, WIDE>(v, j.post_kind, post, j.post_eps, C, inv_c, cw, red, wv);
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       const int c = cw + k * (512 * WPR);
@@ -216,7 +224,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void block_join_kernel(Jo
       if (j.d_stream) store8((TS*)j.d_stream + r * j.lds, c, C, st);
     }
     if (!j.d_z && !j.d_q) continue;
-    if (NORMS) row_norm<NCH, WPR, WIDE>(s, j.pre_kind, pre, j.pre_eps, C, inv_c, cw, red, wv);
+    if (NORMS) row_norm<NCH, WPR, LPR, WIDE>(s, j.pre_kind, pre, j.pre_eps, C, inv_c, cw, red, wv);
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       const int c = cw + k * (512 * WPR);
@@ -244,21 +252,25 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void block_join_kernel(Jo
   }
 }
 
-template <typename TU, typename TS, int NCH, int WPR>
+template <typename TU, typename TS, int NCH, int WPR, int LPR>
 int launch_join(JoinArgs a, int n_cu, hipStream_t s) {
-  constexpr int threads = WPR > 4 ? 64 * WPR : 256;
+  constexpr int threads = WPR > 4 ? 64 * WPR : 256, RPB = WPR > 1 ? 1 : 256 / LPR;
   // Rows a wave (workgroup) takes one after the other.  Many rows: without norms 2 (77 056 x 512 with 8-bit output: 56 / 50 /
   // 52 / 55 us for 1 / 2 / 4 / 8), with norms enough to share the fetch of their vectors (92 / 70 / 60 / 61 us; 48 611 x
   // 1024 layer / layer into a 32-bit stream 128 / 118 / 123 / 124; 40 000 x 2048, a workgroup a row, 180 / 143 / 130 / 126).
   // Few rows: spread over the chip first (301 x 512 4.0 / 4.8 / 6.8 us, 1204 x 1024 by workgroups 8.5 / 8.1 / 10.7).
   const bool norms = a.j.post_kind || a.j.pre_kind;
-  const int64_t most = WPR > 1 ? 8 : !norms || NCH > 1 || sizeof(TU) == 4 ? 2 : 4, share = a.j.rows / (8ll * n_cu * (WPR > 1 ? 1 : 4));
+  const int64_t most = WPR > 1 ? 8 : !norms || NCH > 1 || sizeof(TU) == 4 ? 2 : 4, share = a.j.rows / (8ll * n_cu * RPB);
   a.run = (int)(share < 1 ? 1 : share < most ? share : most);
-  const dim3 grid((unsigned)ceil_div(a.j.rows, (int64_t)a.run * (WPR > 1 ? 1 : 4)));
-  const bool wide = a.j.cols >= 8;
-  if (wide && norms) hipLaunchKernelGGL((block_join_kernel<TU, TS, NCH, WPR, true, true>), grid, dim3(threads), 0, s, a);
-  else if (wide) hipLaunchKernelGGL((block_join_kernel<TU, TS, NCH, WPR, true, false>), grid, dim3(threads), 0, s, a);
-  else hipLaunchKernelGGL((block_join_kernel<TU, TS, NCH, WPR, false, true>), grid, dim3(threads), 0, s, a);
+  const dim3 grid((unsigned)ceil_div(a.j.rows, (int64_t)a.run * RPB));
+  if (a.j.cols < 8) {
+    if constexpr (LPR == 16)
+      hipLaunchKernelGGL((block_join_kernel<TU, TS, NCH, WPR, LPR, false, true>), grid, dim3(threads), 0, s, a);
+  } else if (norms) {
+    hipLaunchKernelGGL((block_join_kernel<TU, TS, NCH, WPR, LPR, true, true>), grid, dim3(threads), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((block_join_kernel<TU, TS, NCH, WPR, LPR, true, false>), grid, dim3(threads), 0, s, a);
+  }
   SUGAR_LAUNCH_CHECK();
   return SUGAR_OK;
 }
@@ -268,10 +280,12 @@ int launch_join_t(const JoinArgs& a, hipStream_t s) {
   int n_cu = 0;
   if (int rc = device_cu_count(&n_cu)) return rc;
   const int C = a.j.cols;
-  if (C <= 512) return launch_join<TU, TS, 1, 1>(a, n_cu, s);
-  if (C <= 1024 && a.j.rows >= 16ll * n_cu) return launch_join<TU, TS, 2, 1>(a, n_cu, s);
-  if (C <= 2048) return launch_join<TU, TS, 1, 4>(a, n_cu, s);
-  return launch_join<TU, TS, 1, 16>(a, n_cu, s);
+  if (C <= 128) return launch_join<TU, TS, 1, 1, 16>(a, n_cu, s);
+  if (C <= 256) return launch_join<TU, TS, 1, 1, 32>(a, n_cu, s);
+  if (C <= 512) return launch_join<TU, TS, 1, 1, 64>(a, n_cu, s);
+  if (C <= 1024 && a.j.rows >= 16ll * n_cu) return launch_join<TU, TS, 2, 1, 64>(a, n_cu, s);
+  if (C <= 2048) return launch_join<TU, TS, 1, 4, 64>(a, n_cu, s);
+  return launch_join<TU, TS, 1, 16, 64>(a, n_cu, s);
 }
 
 bool norm_ok(int kind) { return kind == NORM_NONE || kind == NORM_AFFINE || kind == NORM_RMS || kind == NORM_LAYER; }
