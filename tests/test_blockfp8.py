@@ -772,3 +772,31 @@ def test_quantise_more_rows_than_one_launch_takes():
     y = q.dequantize(torch.bfloat16)
     assert (y[probe] != 1).all() and int((y == 1).sum()) == r - len(probe)
     assert bool((q.exponent[:, 0] == 119).sum() == r - len(probe)) and bool((q.exponent[:, 1:] == 127).all())
+
+
+@gpu
+@pytest.mark.parametrize("c", [5, 20, 128, 150, 256, 300])
+def test_join_many_utterances_in_narrow_rows(c):
+    """Several rows a wave, each with an utterance of its own: more utterances than one step of the search tells apart, empty
+    ones among them, rows in front of the first and behind the last."""
+    g = torch.Generator().manual_seed(c)
+    sizes = torch.randint(0, 5, (1500,), generator=g)
+    off = torch.cat([torch.tensor([3]), 3 + sizes.cumsum(0)]).to(torch.int32)
+    n = int(off[-1])
+    r = n + 6
+    u, res, gate = rows_of(1, r, c, torch.bfloat16).cuda(), rows_of(2, r, c).cuda(), torch.rand(1500, c).cuda()
+    for post, pre in ((None, None), ("rms", "layer")):
+        out = torch.full((r, c), 7.0).cuda()
+        kw = dict(gate=gate, row_off=off.cuda(), post=norm_of(post, c, 3), pre=norm_of(pre, c, 5))
+        j = block_join(u, res, stream_out=out, quantized=True, **kw)
+        check_join(j, u, res, rows=slice(3, n), **kw)
+        assert (out[:3] == 7).all() and (out[n:] == 7).all()
+
+
+@gpu
+@pytest.mark.parametrize("r,c", [(9000, 100), (9001, 256), (7003, 513), (4099, 1025), (3001, 1536), (2003, 2047), (1001, 3000), (70001, 16)])
+def test_join_runs_of_rows(r, c):
+    """Rows enough that a group of lanes takes several, over every number of lanes and waves a row."""
+    u, res = rows_of(1, r, c, torch.bfloat16).cuda(), rows_of(2, r, c, torch.bfloat16).cuda()
+    kw = dict(post=norm_of("layer", c, 3), pre=norm_of("rms", c, 5), gate=torch.rand(c).cuda())
+    check_join(block_join(u, res, quantized=True, **kw), u, res, **kw)
