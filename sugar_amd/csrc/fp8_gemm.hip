@@ -145,9 +145,9 @@ __global__ __launch_bounds__(64 * NW) void fp8_linear_direct_kernel(LinearArgs p
 // Bound by the DMA into LDS (128 x 128 tiles: 64 operations a byte) and, at few k-tiles, by the first tile's way in and the
 // stores: 301 x 1536 -> 1536 6.1 us (64 x 64), float32 output 8.4; 19264 x 528 -> 536 13.4 us, float32 23.6.
 // 128 x 128 with float32 outputs: 4 waves of 64 x 64 convert 8 fragments for 16 products where 8 waves of 64 x 32 convert 6 for
-// 8; 77056 x 1536 -> 1536 352 us (1.03 PF) against 377, x 512 -> 512 54 / 57, x 128 -> 192 (154112 rows) 30.5 / 29.1.  Left
-// out one at a time (8 waves): conversions 70 us, products 67, stores 79.  A persistent form that fetches the next tile under
-// the epilogue and spreads the stores over its k-loop was built and dropped: 362.
+// 8; 77056 x 1536 -> 1536 352 us (1.03 PF) against 377, x 100 -> 1400 121 / 153, 25000 x 300 -> 700 23.9 / 23.0.  Left out one at
+// a time (8 waves): conversions 70 us, products 67, stores 79.  A persistent form that fetches the next tile under the epilogue
+// and spreads the stores over its k-loop was built and dropped: 362.
 constexpr int linear_tile_lds(int TM, int TN) { return (TM + TN) * (2 * 128 + 8) + 8 * TM; }
 
 template <int TM, int TN, int NW, bool WIDE>
@@ -737,20 +737,24 @@ int launch_persist(LinearArgs p, int n_cu, hipStream_t s) {
 int launch_rows(const LinearArgs& p, hipStream_t s) {
   int n_cu = 0;
   if (int rc = device_cu_count(&n_cu)) return rc;
-  // Measured, us (bf16 output unless said; direct | tile 64x64 | 64x128 | 128x128 | persist):
-  //   1 x 1536 -> 1536      3.5 | 5.7                      128 x 512 -> 512      3.2 | 3.8
-  //   256 x 1536 -> 192     4.1 | 5.8                      301 x 512 -> 512      4.1 | 3.8
-  //   301 x 1536 -> 1536    -   | 6.1 |  7.3 |  9.5        float32 output        -   | 9.0 | 11.0 | 16.5
-  //   1204 x 1536 -> 1536   -   | 7.9 |  7.7 | 10.0        float32 output        -   | 13.2 | 11.9 | 17.7
-  //   4816 x 1536 -> 1536   -   | 21.8 | 20.0 | 16.4       19264 x 528 -> 536    -   | 16.2 | 14.0 | 13.4
-  //   77056 x 512 -> 512    -   | 43  | 35   | 31.5 | 31.9   77056 x 768 -> 768      61.3 | 65.8 (the last two)
-  //   77056 x 1152 -> 1152  125.9 | 118.6                    77056 x 1536 -> 1536    231.9 | 180.8
+  // Measured, us.  bf16 outputs (direct | 64 x 64 by 8 waves | by 4 | 64 x 128 | 128 x 128 | persist):
+  //   1 x 1536 -> 1536       3.5 | 5.7                              600 x 1024 -> 600       8.9 | 5.2 | 5.3 | 5.8 | 7.7
+  //   256 x 1536 -> 192      4.1 | 5.8                              1204 x 1536 -> 1536      -  | 8.3 | 7.9 | 8.3 | 10.5
+  //   301 x 1536 -> 1536      -  | 6.3 | 6.6 | 7.4 | 10.1           12000 x 2048 -> 300      -  | 16.3 | 14.5 | 13.4 | 16.8
+  //   4816 x 1536 -> 1536     -  | 22.7 | 20.7 | 20.5 | 16.1        23001 x 1149 -> 264      -  | 18.0 | 16.0 | 17.0 | 18.9
+  //   77056 x 768 -> 768      -  |  -   |  -   |  -   | 61.3 | 65.8   154112 x 128 -> 192    -  | 20.0 | 18.5 | 17.6 | 19.8
+  //   77056 x 1152 -> 1152    -  |  -   |  -   |  -   | 125.9 | 118.6   77056 x 1536 -> 1536  -  |  -  |  -   |  -   | 231.9 | 180.8
+  // float32 outputs (64 x 64 by 8 waves | by 4 | 64 x 128 | 128 x 128 by 4):
+  //   301 x 1536 -> 1536     8.8 | 9.3 | 11.3                       13446 x 704 -> 373      16.0 | 14.1 | 15.7 | 17.4
+  //   4816 x 1536 -> 1536    38.6 | 33.2 | 32.6 | 27.8              154112 x 128 -> 192     26.8 | 24.1 | 26.6 | 29.4
   // weights in registers | 128 x 128:  77056 x 512 -> 512 29.9 | 33.9, -> 1024 49.4 | 59.1, -> 256 21.3 | 20.2;
   //   77056 x 384 -> 384 24.9 | 22.8;  77056 x 128 -> 512 18.3 | 19.6;  38528 x 512 -> 512 19.8 | 19.3
-  // so: direct while its workgroups (each streams its 16 channels' weights once per 16 rows) are at most two a CU, the
-  // larger tile once it fills the CUs, weights in registers for K <= 512 where two slabs or more are three quarters full and
-  // walk rows enough to pay for their fetch, the persistent kernel where k-loops are long enough to hide its epilogue and two
-  // rounds of tiles or more are there.
+  // so: direct while its workgroups (each streams its 16 channels' weights once per 16 rows) are at most two a CU; weights in
+  // registers for K <= 512 where two slabs or more are three quarters full and walk rows enough to pay for their fetch; the
+  // persistent kernel where k-loops are long enough to hide its epilogue and two rounds of tiles or more are there.  Of the tiles
+  // 128 x 128 once they give every CU one, unless the CU with the most of them has more to do than it has with 64 x 128, half the
+  // work and a fifth more time for it (channels that end early in a tile, a second round for a few tiles); 64 x 64 below, by 8
+  // waves while there is no more than one a CU.
   const bool f32 = p.out_f32;
   if (ceil_div(p.n, 16) * ceil_div(p.rows, 16) <= 2ll * n_cu) {
     constexpr int NW = 8;
@@ -765,11 +769,12 @@ int launch_rows(const LinearArgs& p, hipStream_t s) {
     return launch_short(p, n_cu, s);
   if (!f32 && !p.y2 && p.kb >= 8 && n_cu % 8 == 0 && ceil_div(p.n, 256) * ceil_div(p.rows, 256) >= 2 * n_cu)
     return launch_persist(p, n_cu, s);
-  if (ceil_div(p.n, 128) * ceil_div(p.rows, 128) >= n_cu)
-    return !f32 ? launch_tile<128, 128, 8, false>(p, s) : p.kb >= 4 ? launch_tile<128, 128, 4, true>(p, s) : launch_tile<128, 128, 8, true>(p, s);
-  if (4 * ceil_div(p.n, 64) * ceil_div(p.rows, 128) >= 3 * n_cu)
-    return f32 ? launch_tile<64, 128, 8, true>(p, s) : launch_tile<64, 128, 8, false>(p, s);
-  return f32 ? launch_tile<64, 64, 8, true>(p, s) : launch_tile<64, 64, 8, false>(p, s);
+  const int64_t rt = ceil_div(p.rows, 128), half = ceil_div(p.n, 64) * rt, full = ceil_div(p.n, 128) * rt, small = ceil_div(p.n, 64) * ceil_div(p.rows, 64);
+  if (full >= n_cu && 5 * ceil_div(full, n_cu) < 3 * ceil_div(half, n_cu))
+    return f32 ? launch_tile<128, 128, 4, true>(p, s) : launch_tile<128, 128, 8, false>(p, s);
+  if (small <= n_cu) return f32 ? launch_tile<64, 64, 8, true>(p, s) : launch_tile<64, 64, 8, false>(p, s);
+  if (f32) return launch_tile<64, 64, 4, true>(p, s);
+  return small <= 2 * n_cu ? launch_tile<64, 64, 4, false>(p, s) : launch_tile<64, 128, 8, false>(p, s);
 }
 
 }  // namespace

@@ -800,3 +800,25 @@ def test_join_runs_of_rows(r, c):
     u, res = rows_of(1, r, c, torch.bfloat16).cuda(), rows_of(2, r, c, torch.bfloat16).cuda()
     kw = dict(post=norm_of("layer", c, 3), pre=norm_of("rms", c, 5), gate=torch.rand(c).cuda())
     check_join(block_join(u, res, quantized=True, **kw), u, res, **kw)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("r,n,k", [(1492, 1088, 567), (9619, 72, 850), (13446, 373, 704), (2100, 1000, 130), (9000, 1400, 100), (12001, 300, 1030)])
+def test_linear_every_tile(dtype, r, n, k):
+    """Sizes between a few rows and many: each tile and number of waves, rows and channels that end inside one."""
+    a, w = operands(r, r, n, k)
+    s, t = rows_of(8, 1, n)[0].cuda(), rows_of(9, 1, n)[0].cuda()
+    got = block_fp8_linear(a, w, scale=s, shift=t, relu=True, out_dtype=dtype)
+    for lo in (0, r // 2, r - 200):
+        rows = slice(lo, lo + 200)
+        y, mag = linear64(a[rows], w, s, t, True)
+        tol = (k + 4) * U32 * mag
+        if dtype == torch.bfloat16:
+            tol = (tol + cut64(a[rows], w) * s.cpu().double().abs()) * (1 + HALF[dtype]) + HALF[dtype] * y.abs()
+        assert ((got[rows].cpu().double() - y).abs() <= tol).all()
+    # everywhere: the same products by the 64-bit form's inputs in float32, 64 rows of every 500
+    for lo in range(0, r - 64, 500):
+        part = block_fp8_linear(a[lo:lo + 64], w, scale=s, shift=t, relu=True, out_dtype=torch.float32)
+        err = (got[lo:lo + 64].float() - part).abs().amax(1) / part.abs().amax(1).clamp(min=1e-30)
+        assert (err <= (2.0 ** -7 if dtype == torch.bfloat16 else 1e-5)).all()
