@@ -233,7 +233,8 @@ int launch_join(JoinArgs a, int n_cu, hipStream_t s) {
   const bool norms = a.j.post_kind || a.j.pre_kind;
   const int64_t most = !norms ? 2 : WPR > 3 ? 8 : sizeof(TS) == 4 && LPR == 64 ? 2 : 4;
   const int64_t waves = ceil_div(a.j.rows * WPR * LPR, 64), share = (waves + 6 * n_cu) / (12 * n_cu);
-  a.run = (int)(share < 1 ? 1 : share < most ? share : most);
+  const int64_t least = ceil_div(a.j.rows, RPB * ((1ll << 32) / threads - 1));            // a launch has fewer than 2^32 threads
+  a.run = (int)(share >= most ? (most > least ? most : least) : share > 1 ? share : 1);
   const dim3 grid((unsigned)ceil_div(a.j.rows, (int64_t)a.run * RPB));
   if (a.j.cols < 8) {
     if constexpr (LPR == 16) hipLaunchKernelGGL((block_join_kernel<TU, TS, WPR, LPR, false, true>), grid, dim3(threads), 0, s, a);

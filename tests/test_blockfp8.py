@@ -822,3 +822,15 @@ def test_linear_every_tile(dtype, r, n, k):
         part = block_fp8_linear(a[lo:lo + 64], w, scale=s, shift=t, relu=True, out_dtype=torch.float32)
         err = (got[lo:lo + 64].float() - part).abs().amax(1) / part.abs().amax(1).clamp(min=1e-30)
         assert (err <= (2.0 ** -7 if dtype == torch.bfloat16 else 1e-5)).all()
+
+
+@gpu
+def test_join_more_rows_than_short_runs_cover():
+    """A launch has fewer than 2^32 threads: runs of rows get longer."""
+    r = (1 << 29) + 4321
+    u, res = torch.ones(r, 1, dtype=torch.bfloat16, device="cuda"), torch.zeros(r, 1, dtype=torch.bfloat16, device="cuda")
+    probe = torch.tensor([0, 1, 12345, (1 << 29) - 1, 1 << 29, r - 2, r - 1], device="cuda")
+    u[probe, 0] = torch.arange(2, 9, device="cuda").bfloat16()
+    out = block_join(u, res, alpha=2.0, normed=False, stream_out=res).stream
+    assert out[probe, 0].tolist() == [2.0 * i for i in range(2, 9)]
+    assert int((out == 2).sum()) == r - len(probe)
