@@ -8,7 +8,7 @@
 // Everything between the loads and the stores is f32 in registers: a wave (several for wide rows, 16 or 32 lanes for narrow
 // ones) holds its row, so a norm's mean and its sum of squares about that mean are two exact passes over registers, not over memory, and z
 // comes from the unrounded s.  Bound: HBM (u and residual in, stream and z out).  Measured, bf16: 77 056 x 512 with two rms
-// norms 59 us (5.3 TB/s), dense with 8-bit output 48 (5.7); 48 611 x 1024, layer / layer, float32 stream 118 (5.1); one row 3.4.
+// norms 59 us (5.3 TB/s), dense with 8-bit output 48 (5.7); 48 611 x 1024, layer / layer, float32 stream 115 (5.2); one row 3.5.
 #include <type_traits>
 
 #include "blockfp8.h"
@@ -44,16 +44,18 @@ __device__ __forceinline__ float lane_total(float v) {
   return v;
 }
 
+// Sum over the row.  Several waves a row exchange theirs through one half of `red` and the next total's through the other: a half
+// is written again only behind the barrier of the total between.
 template <int WPR, int LPR>
-__device__ __forceinline__ float row_total(float v, float* red, int wv) {
+__device__ __forceinline__ float row_total(float v, float* red, int wv, int& half) {
   v = lane_total<LPR>(v);
   if constexpr (WPR > 1) {
-    __syncthreads();                         // the previous total has been read
-    if ((threadIdx.x & 63) == 0) red[wv] = v;
+    if ((threadIdx.x & 63) == 0) red[half + wv] = v;
     __syncthreads();
-    v = red[0];
+    v = red[half];
 #pragma unroll
-    for (int i = 1; i < WPR; ++i) v += red[i];
+    for (int i = 1; i < WPR; ++i) v += red[half + i];
+    half ^= 16;
   }
   return v;
 }
@@ -101,14 +103,14 @@ struct NormVec {
 // x <- norm(x) over the row's C channels; lanes past the row hold zeros before and after.
 template <int WPR, int LPR, bool WIDE>
 __device__ __forceinline__ void row_norm(float (&x)[8], int kind, const NormVec<WIDE>& p, float eps, int C, float inv_c, int c,
-                                         float* red, int wv) {
+                                         float* red, int wv, int& half) {
   if (kind == NORM_NONE) return;
   float mean = 0.f, mul = 1.f;
   if (kind == NORM_LAYER) {
     float t = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) t += x[i];
-    mean = row_total<WPR, LPR>(t, red, wv) * inv_c;
+    mean = row_total<WPR, LPR>(t, red, wv, half) * inv_c;
   }
   if (kind != NORM_AFFINE) {
     float t = 0.f;
@@ -126,7 +128,7 @@ __device__ __forceinline__ void row_norm(float (&x)[8], int kind, const NormVec<
       }
       t = c < C ? t : 0.f;
     }
-    mul = 1.0f / sqrtf(fmaf(row_total<WPR, LPR>(t, red, wv), inv_c, eps));
+    mul = 1.0f / sqrtf(fmaf(row_total<WPR, LPR>(t, red, wv, half), inv_c, eps));
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = fmaf((x[i] - mean) * mul, p.w[i], p.b[i]);
@@ -136,7 +138,8 @@ __device__ __forceinline__ void row_norm(float (&x)[8], int kind, const NormVec<
 // Each group of lanes that holds a row takes a run of consecutive rows.
 template <typename TU, typename TS, int WPR, int LPR, bool WIDE, bool NORMS>
 __global__ __launch_bounds__(WPR > 1 ? 64 * WPR : 256) void block_join_kernel(JoinArgs a) {
-  __shared__ float red[WPR];
+  __shared__ float red[WPR > 1 ? 32 : 1];
+  int half = 0;
   const SugarBlockJoin& j = a.j;
   const int lane = threadIdx.x & (LPR - 1), wv = threadIdx.x >> 6;
   const int C = j.cols;
@@ -162,31 +165,43 @@ __global__ __launch_bounds__(WPR > 1 ? 64 * WPR : 256) void block_join_kernel(Jo
   NormVec<WIDE> post, pre;                                     // in registers over the rows
   if (NORMS && j.post_kind) post.load(j.d_post_w, j.d_post_b, c, C);
   if (NORMS && j.pre_kind) pre.load(j.d_pre_w, j.d_pre_b, c, C);
+  // the next row is fetched before this one is worked on; a gate per channel once, one per utterance when the utterance changes
+  Raw8<TU, WIDE> nu, ng;
+  Raw8<TS, WIDE> ns;
+  auto fetch = [&](int64_t r) {
+    nu.load((const TU*)j.d_u + r * j.ldu, c, C);
+    ns.load((const TS*)j.d_residual + r * j.ldr, c, C);
+    if (j.gate_kind == SUGAR_GATE_ROW) ng.load((const TU*)j.d_gate + r * j.ldg, c, C);
+  };
+  float g[8];
+  auto fetch_gate = [&](const float* gp) {
+    Raw8<float, WIDE> t;
+    t.load(gp, c, C);
+    t.get(gp, g, c, C);
+  };
+#pragma unroll
+  for (int i = 0; i < 8; ++i) g[i] = 1.f;
+  if (j.gate_kind == SUGAR_GATE_CHANNEL) fetch_gate((const float*)j.d_gate);
+  int gate_of = -1;
+  fetch(first);
   for (int64_t r = first; r < last; ++r) {
+    const Raw8<TU, WIDE> ru = nu, rg = ng;
+    const Raw8<TS, WIDE> rs = ns;
+    if (r + 1 < last) fetch(r + 1);
     if (j.d_row_off) {
       while (r >= b_end && b + 1 < j.n_utts) { ++b; b_end = j.d_row_off[b + 1]; }
       if (r >= b_end || r < begin) continue;                   // a row of no utterance: left as it is
+      if (j.gate_kind == SUGAR_GATE_UTTERANCE && b != gate_of) {
+        fetch_gate((const float*)j.d_gate + b * j.ldg);
+        gate_of = b;
+      }
     }
     const TU* up = (const TU*)j.d_u + r * j.ldu;
     const TS* rp = (const TS*)j.d_residual + r * j.ldr;
-    const void* gp = j.gate_kind == SUGAR_GATE_ROW ? (const void*)((const TU*)j.d_gate + r * j.ldg)
-                                                   : (const void*)((const float*)j.d_gate + (j.gate_kind == SUGAR_GATE_UTTERANCE ? b * j.ldg : 0));
-    Raw8<TU, WIDE> ru, rgu;
-    Raw8<TS, WIDE> rs;
-    Raw8<float, WIDE> rg;
-    ru.load(up, c, C);
-    rs.load(rp, c, C);
-    if (j.gate_kind == SUGAR_GATE_ROW) rgu.load((const TU*)gp, c, C);
-    else if (j.gate_kind) rg.load((const float*)gp, c, C);
-    float v[8], s[8], g[8];
+    float v[8], s[8];
     ru.get(up, v, c, C);
-    if (NORMS) row_norm<WPR, LPR, WIDE>(v, j.post_kind, post, j.post_eps, C, inv_c, c, red, wv);
-    if (j.gate_kind == SUGAR_GATE_ROW) rgu.get((const TU*)gp, g, c, C);
-    else if (j.gate_kind) rg.get((const float*)gp, g, c, C);
-    else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) g[i] = 1.f;
-    }
+    if (NORMS) row_norm<WPR, LPR, WIDE>(v, j.post_kind, post, j.post_eps, C, inv_c, c, red, wv, half);
+    if (j.gate_kind == SUGAR_GATE_ROW) rg.get((const TU*)j.d_gate + r * j.ldg, g, c, C);
     rs.get(rp, s, c, C);
     float st[8];
 #pragma unroll
@@ -197,7 +212,7 @@ __global__ __launch_bounds__(WPR > 1 ? 64 * WPR : 256) void block_join_kernel(Jo
     }
     if (j.d_stream) store8((TS*)j.d_stream + r * j.lds, c, C, st);
     if (!j.d_z && !j.d_q) continue;
-    if (NORMS) row_norm<WPR, LPR, WIDE>(s, j.pre_kind, pre, j.pre_eps, C, inv_c, c, red, wv);
+    if (NORMS) row_norm<WPR, LPR, WIDE>(s, j.pre_kind, pre, j.pre_eps, C, inv_c, c, red, wv, half);
     if (j.d_z) {
       if (j.z_dtype == SUGAR_F32) store8((float*)j.d_z + r * j.ldz, c, C, s);
       else store8((bf16*)j.d_z + r * j.ldz, c, C, s);
@@ -224,14 +239,15 @@ __global__ __launch_bounds__(WPR > 1 ? 64 * WPR : 256) void block_join_kernel(Jo
 template <typename TU, typename TS, int WPR, int LPR>
 int launch_join(JoinArgs a, int n_cu, hipStream_t s) {
   constexpr int threads = WPR > 1 ? 64 * WPR : 256, RPB = WPR > 1 ? 1 : 256 / LPR;
-  // Rows a group of lanes takes one after the other: they share the fetch of the norm vectors and the search of the utterance.
-  // Many rows, us for runs of 1 / 2 / 4 / 8: 77 056 x 512 without norms, 8-bit output 56 / 50 / 52 / 55, two rms norms 92 / 70 / 60 /
-  // 61; 48 611 x 1024 layer / layer, 32-bit stream 110 / 108 / 115 / 116; 30 000 x 1536 rms / rms 87 / 76 / 74 / 76; 40 000 x 2048
-  // 180 / 143 / 130 / 126.  Fewer rows: as many waves as the chip holds at once, about three a SIMD, rather than a second round of
-  // them: 14 857 x 616 33 / 27 / 25 / 24, 12 000 x 300 15.9 / 14.1 / 13.8 / 19.3, 35 438 x 120 13.0 / 12.5 / 12.5 / 17.2 (3: 10.9), 8000 x 200 6.6 /
-  // 7.0 / 9.2 / 14.1, 1480 x 592 5.4 / 5.8 / 7.8 / 11.6, 301 x 512 4.0 / 4.8 / 6.8.
+  // Rows a group of lanes takes one after the other: they share the fetch of the norm vectors, the search of the utterance and its
+  // gate, and each is fetched under the one before.  Many rows, us for runs of 1 / 2 / 4 / 8 (inputs from memory): 77 056 x 512 two rms
+  // norms, gate per utterance 88 / 69 / 65 / 64; 48 611 x 1024 without norms 79 / 72 / 76 / 80, layer / layer into a 32-bit stream 134 /
+  // 115 / 115 / 119 (3: 114); 30 000 x 1536 rms / rms 99 / 81 / 77 / 77; 40 000 x 2048 rms / rms 180 / 143 / 130 / 126.  Fewer rows: as many
+  // waves as the chip holds at once, about three a SIMD, rather than a second round of them: 14 857 x 616 30 / 26 / 24 / 22, 12 000 x
+  // 300 14.9 / 13.3 / 12.9 / 17.4, 35 438 x 120 12.2 / 11.9 / 12.1 / 15.9 (3: 10.4), 8000 x 200 6.5 / 6.7 / 9.0 / 13.8, 1480 x 592 5.2 / 5.5 / 7.6 /
+  // 11.7, 301 x 512 4.0 / 4.8 / 6.8.
   const bool norms = a.j.post_kind || a.j.pre_kind;
-  const int64_t most = !norms ? 2 : WPR > 3 ? 8 : sizeof(TS) == 4 && LPR == 64 ? 2 : 4;
+  const int64_t most = !norms ? 2 : sizeof(TS) == 4 && LPR == 64 ? 3 : WPR > 3 ? 8 : 4;
   const int64_t waves = ceil_div(a.j.rows * WPR * LPR, 64), share = (waves + 6 * n_cu) / (12 * n_cu);
   const int64_t least = ceil_div(a.j.rows, RPB * ((1ll << 32) / threads - 1));            // a launch has fewer than 2^32 threads
   a.run = (int)(share >= most ? (most > least ? most : least) : share > 1 ? share : 1);
@@ -248,7 +264,7 @@ int launch_join(JoinArgs a, int n_cu, hipStream_t s) {
 }
 
 // As many lanes as a row of 8 channels a lane fills: 30 000 x 1536 by three waves a row 74 us, by four 92; 1480 x 592 by two 5.4, by
-// four 8.1; 22 180 x 11 by 16 lanes 8.7, by a wave 19.2.  (Two chunks of 8 a lane instead of two waves: 48 611 x 1024 112 against 108.)
+// four 8.1; 22 180 x 11 by 16 lanes 8.7, by a wave 19.2.
 template <typename TU, typename TS>
 int launch_join_t(const JoinArgs& a, hipStream_t s) {
   int n_cu = 0;
