@@ -231,7 +231,7 @@ class BlockFP8(object):
         if out is None:
             if dtype not in _DT:
                 raise ValueError("dequantize: dtype %s not in %s" % (dtype, [str(d) for d in _DT]))
-            out, ld = torch.empty((rows, cols), dtype=dtype, device=dev), cols
+            out, ld = torch.empty(rows, cols, dtype=dtype, device=dev), cols
         else:
             ld = _out("dequantize", out, (rows, cols), _DT, dev)
             _apart("dequantize", _span(out, ld), self._spans())
@@ -297,7 +297,7 @@ def block_fp8_linear(a, w, scale=None, shift=None, relu=False, out_dtype=torch.b
     if out is None:
         if out_dtype not in _DT:
             raise ValueError("block_fp8_linear: out_dtype %s not in %s" % (out_dtype, [str(d) for d in _DT]))
-        out, ld = torch.empty((rows, n), dtype=out_dtype, device=dev), n
+        out, ld = torch.empty(rows, n, dtype=out_dtype, device=dev), n
     else:
         ld = _out("block_fp8_linear", out, (rows, n), _DT, dev)
         _apart("block_fp8_linear", _span(out, ld), a._spans() + w._spans() + [_span(t) for t in (scale, shift) if t is not None])
@@ -452,4 +452,4 @@ def _norm(side, p, cols, inputs):
 
 def _like(x, dtype, rows, cols, dev):
     """A new contiguous [rows, cols] (empty_like is the cheaper call)."""
-    return torch.empty_like(x) if x.dtype == dtype and x.is_contiguous() else torch.empty((rows, cols), dtype=dtype, device=dev)
+    return torch.empty_like(x) if x.dtype == dtype and x.is_contiguous() else torch.empty(rows, cols, dtype=dtype, device=dev)
