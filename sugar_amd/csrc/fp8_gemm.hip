@@ -138,27 +138,32 @@ __global__ __launch_bounds__(64 * NW) void fp8_linear_direct_kernel(LinearArgs p
 }
 
 // ------------------------------------------------------------------------------------------ one tile
-// One TM x TN output tile by a workgroup of NW waves = 2 (channels) x NW / 2 (rows).  Two stages: wait for this wave's share of
-// k-tile t, barrier, issue the DMA of k-tile t + 1 into the buffer k-tile t - 1 was read from, compute; what a workgroup
-// waits for the DMA, the two to four others of its CU fill.  Exponents travel as one dword per row and four k-tiles, staged
-// with the first of the four (double buffer) and shifted down a byte per k-tile.
+// One TM x TN output tile by a workgroup of NW waves = 2 (channels) x NW / 2 (rows).  Steps of KS k-tiles through two stages: wait
+// for this wave's share of a step, barrier, issue the DMA of the next into the buffer the last was read from, compute; what a
+// workgroup waits for the DMA, the two to four others of its CU fill.  A CU with one workgroup has nothing to fill a step's
+// barrier and latencies with: steps of 4 (301 x 1536 -> 1536 5.5 us, by single k-tiles 5.9; deeper rings of single k-tiles do not
+// help).  Exponents travel as one dword per row and four k-tiles, staged with the first of the four (double buffer) and shifted
+// down a byte per k-tile.
 // Bound by the DMA into LDS (128 x 128 tiles: 64 operations a byte) and, at few k-tiles, by the first tile's way in and the
-// stores: 301 x 1536 -> 1536 6.1 us (64 x 64), float32 output 8.4; 19264 x 528 -> 536 13.4 us, float32 23.6.
+// stores: 301 x 1536 -> 1536 5.5 us (64 x 64), float32 output 8.0; 19264 x 528 -> 536 14.8 us, float32 21.8.
 // 128 x 128 with float32 outputs: 4 waves of 64 x 64 convert 8 fragments for 16 products where 8 waves of 64 x 32 convert 6 for
 // 8; 77056 x 1536 -> 1536 352 us (1.03 PF) against 377, x 100 -> 1400 121 / 153, 25000 x 300 -> 700 23.9 / 23.0.  Left out one at
 // a time (8 waves): conversions 70 us, products 67, stores 79.  A persistent form that fetches the next tile under the epilogue
 // and spreads the stores over its k-loop was built and dropped: 362.
-constexpr int linear_tile_lds(int TM, int TN) { return (TM + TN) * (2 * 128 + 8) + 8 * TM; }
+constexpr int linear_tile_lds(int TM, int TN, int KS) { return (TM + TN) * (2 * KS * 128 + 8) + 8 * TM; }
 
-template <int TM, int TN, int NW, bool WIDE>
+template <int TM, int TN, int NW, bool WIDE, int KS = 1>
 __device__ __forceinline__ void fp8_tile(const LinearArgs& p, const int co_base, const int r_base) {
   constexpr int STAGE_BYTES = (TM + TN) * 128;
   constexpr int WN = NW / 2, CW = TM / 2, FW = TN / WN, MI = CW / 16, NJ = FW / 16, WI = TM / (8 * NW), XI = TN / (8 * NW), SI = (TM + TN) / 64;
+  // Written into the loop the products of a k-tile keep their reads between them, which 128 x 128 tiles with float32 outputs gain 8 %
+  // by (19264 x 528 -> 536); inlined from `multiply` hipcc moves all reads in front, which narrow tiles gain 3 .. 6 % by.
+  constexpr bool SPREAD = WIDE && TM > 64 && KS == 1;
   static_assert(SI <= NW && TM / 32 <= NW, "one exponent, one affine instruction per wave");
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wv / WN, wn = wv % WN, fr = lane & 15, fq = lane >> 4;
-  unsigned* exps = (unsigned*)(smem + 2 * STAGE_BYTES);          // [2][TM + TN]
+  unsigned* exps = (unsigned*)(smem + 2 * KS * STAGE_BYTES);     // [2][TM + TN]
   float* aff = (float*)(exps + 2 * (TM + TN));                   // [scale | shift][TM], fetched with the first k-tile
   const int nk = p.kb;
   const bool relu = p.flags & EPI_RELU, affine = p.flags & EPI_AFFINE;
@@ -183,10 +188,10 @@ __device__ __forceinline__ void fp8_tile(const LinearArgs& p, const int co_base,
   const uint8_t* ebase = wv * 64 < TM ? p.we : p.ae;
   const unsigned eoff = wv * 64 < TM ? (unsigned)min(co_base + erow, p.n - 1) * p.ldwe
                                      : (unsigned)min(r_base + erow - TM, p.rows - 1) * p.ldae;
-  auto stage = [&](int buf, int kt) {
+  auto stage = [&](int slot, int kt) {
     if ((kt & 3) == 0 && wv < SI) dma<4>(ebase + kt, eoff, (unsigned char*)(exps + ((kt >> 2) & 1) * (TM + TN) + wv * 64));
-    unsigned char* wbase = smem + buf * STAGE_BYTES + wv * (WI * 8) * 128;
-    unsigned char* xbase = smem + buf * STAGE_BYTES + TM * 128 + wv * (XI * 8) * 128;
+    unsigned char* wbase = smem + slot * STAGE_BYTES + wv * (WI * 8) * 128;
+    unsigned char* xbase = smem + slot * STAGE_BYTES + TM * 128 + wv * (XI * 8) * 128;
 #pragma unroll
     for (int i = 0; i < WI; ++i) dma<16>(p.w + kt * 128, woff[i], wbase + i * 1024);
 #pragma unroll
@@ -200,21 +205,9 @@ __device__ __forceinline__ void fp8_tile(const LinearArgs& p, const int co_base,
     for (int n = 0; n < NJ; ++n) acc[m][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
   int ew[MI], ex[NJ];
 
-  stage(0, 0);
-  for (int kt = 0; kt < nk; ++kt) {
-    const int cur = kt & 1;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // this wave's share of k-tile kt has landed, then everyone's
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (kt + 1 < nk) stage(cur ^ 1, kt + 1);
-    const unsigned char* wb = smem + cur * STAGE_BYTES;
+  auto multiply = [&](int slot) {
+    const unsigned char* wb = smem + slot * STAGE_BYTES;
     const unsigned char* xb = wb + TM * 128;
-    if ((kt & 3) == 0) {
-      const unsigned* e = exps + ((kt >> 2) & 1) * (TM + TN);
-#pragma unroll
-      for (int m = 0; m < MI; ++m) ew[m] = e[wm * CW + m * 16 + fr];
-#pragma unroll
-      for (int n = 0; n < NJ; ++n) ex[n] = e[TM + wn * FW + n * 16 + fr];
-    }
     if constexpr (WIDE) {
       bf16x8 xh[NJ][4];
 #pragma unroll
@@ -241,6 +234,48 @@ __device__ __forceinline__ void fp8_tile(const LinearArgs& p, const int co_base,
     for (int m = 0; m < MI; ++m) ew[m] = (int)((unsigned)ew[m] >> 8);
 #pragma unroll
     for (int n = 0; n < NJ; ++n) ex[n] = (int)((unsigned)ex[n] >> 8);
+  };
+  stage(0, 0);
+#pragma unroll
+  for (int q = 1; q < KS; ++q)
+    if (q < nk) stage(q, q);
+  for (int kt = 0; kt < nk; kt += KS) {
+    const int cur = (kt / KS) & 1;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // this wave's share of these k-tiles has landed, then everyone's
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+    for (int q = 0; q < KS; ++q)
+      if (kt + KS + q < nk) stage((cur ^ 1) * KS + q, kt + KS + q);
+    if ((kt & 3) == 0) {
+      const unsigned* e = exps + ((kt >> 2) & 1) * (TM + TN);
+#pragma unroll
+      for (int m = 0; m < MI; ++m) ew[m] = e[wm * CW + m * 16 + fr];
+#pragma unroll
+      for (int n = 0; n < NJ; ++n) ex[n] = e[TM + wn * FW + n * 16 + fr];
+    }
+    if constexpr (SPREAD) {
+      const unsigned char* wb = smem + cur * STAGE_BYTES;
+      const unsigned char* xb = wb + TM * 128;
+      bf16x8 xh[NJ][4];
+#pragma unroll
+      for (int n = 0; n < NJ; ++n) fp8_to_bf16(frag(xb, wn * FW + n * 16 + fr, fq), ex[n], xh[n]);
+#pragma unroll
+      for (int m = 0; m < MI; ++m) {
+        bf16x8 wh[4];
+        fp8_to_bf16(frag(wb, wm * CW + m * 16 + fr, fq), ew[m], wh);
+#pragma unroll
+        for (int n = 0; n < NJ; ++n) acc[m][n] = mfma_wide(wh, xh[n], acc[m][n]);
+      }
+#pragma unroll
+      for (int m = 0; m < MI; ++m) ew[m] = (int)((unsigned)ew[m] >> 8);
+#pragma unroll
+      for (int n = 0; n < NJ; ++n) ex[n] = (int)((unsigned)ex[n] >> 8);
+    } else if (kt + KS <= nk) {
+#pragma unroll
+      for (int q = 0; q < KS; ++q) multiply(cur * KS + q);
+    } else {
+      for (int q = 0; kt + q < nk; ++q) multiply(cur * KS + q);
+    }
   }
 
   // ---- epilogue: accumulator tile (m, n): lane (fr, fq) holds row wn FW + n 16 + fr, channels wm CW + m 16 + 4 fq + 0..3
@@ -270,7 +305,7 @@ __device__ __forceinline__ void fp8_tile(const LinearArgs& p, const int co_base,
   }
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // stage memory becomes the epilogue staging
   constexpr int EPI_STRIDE = CW * 2 + 16, CPR = CW / 8, RPP = 64 / CPR;
-  static_assert(NW * 16 * EPI_STRIDE <= 2 * STAGE_BYTES, "epilogue staging fits the stages");
+  static_assert(NW * 16 * EPI_STRIDE <= 2 * KS * STAGE_BYTES, "epilogue staging fits the stages");
   unsigned char* ep = smem + wv * (16 * EPI_STRIDE);             // this wave's [16 rows][CW channels]
 #pragma unroll
   for (int n = 0; n < NJ; ++n) {
@@ -296,24 +331,24 @@ __device__ __forceinline__ void fp8_tile(const LinearArgs& p, const int co_base,
   }
 }
 
-template <int TM, int TN, int NW, bool WIDE>
+template <int TM, int TN, int NW, bool WIDE, int KS = 1>
 __global__ __launch_bounds__(64 * NW, NW / 2) void fp8_linear_tile_kernel(LinearArgs p) {
   const int vid = xcd_remap(blockIdx.x, gridDim.x);
   const int co = (vid % p.n_co_tiles) * TM, r = (vid / p.n_co_tiles) * TN;
   // a last tile that is less than half full as half a tile: float32 outputs 3 .. 6 % faster (19264 x 528 -> 536 24.9 -> 23.6 us,
   // 40000 x 700 -> 300 30.2 -> 28.6), bf16 ones between 3 % faster and 8 % slower (the same: 14.0 -> 15.1, 12.5 -> 12.2)
-  if (WIDE && TM > 64 && p.n - co <= 64) fp8_tile<64, TN, NW, WIDE>(p, co, r);
-  else fp8_tile<TM, TN, NW, WIDE>(p, co, r);
+  if (WIDE && TM > 64 && p.n - co <= 64) fp8_tile<64, TN, NW, WIDE, KS>(p, co, r);
+  else fp8_tile<TM, TN, NW, WIDE, KS>(p, co, r);
 }
 
-template <int TM, int TN, int NW, bool WIDE>
+template <int TM, int TN, int NW, bool WIDE, int KS = 1>
 int launch_tile(LinearArgs p, hipStream_t s) {
-  constexpr int smem = linear_tile_lds(TM, TN);
+  constexpr int smem = linear_tile_lds(TM, TN, KS);
   static OptInMask opted{0};
-  if (int rc = lds_opt_in((const void*)fp8_linear_tile_kernel<TM, TN, NW, WIDE>, smem, &opted)) return rc;
+  if (int rc = lds_opt_in((const void*)fp8_linear_tile_kernel<TM, TN, NW, WIDE, KS>, smem, &opted)) return rc;
   p.n_co_tiles = (int)ceil_div(p.n, TM);
   const int64_t grid = p.n_co_tiles * ceil_div(p.rows, TN);
-  hipLaunchKernelGGL((fp8_linear_tile_kernel<TM, TN, NW, WIDE>), dim3((unsigned)grid), dim3(64 * NW), smem, s, p);
+  hipLaunchKernelGGL((fp8_linear_tile_kernel<TM, TN, NW, WIDE, KS>), dim3((unsigned)grid), dim3(64 * NW), smem, s, p);
   SUGAR_LAUNCH_CHECK();
   return SUGAR_OK;
 }
@@ -744,12 +779,12 @@ int launch_rows(const LinearArgs& p, hipStream_t s) {
   // Measured, us.  bf16 outputs (direct | 64 x 64 by 8 waves | by 4 | 64 x 128 | 128 x 128 | persist):
   //   1 x 1536 -> 1536       3.5 | 5.7                              600 x 1024 -> 600       8.9 | 5.2 | 5.3 | 5.8 | 7.7
   //   256 x 1536 -> 192      4.1 | 5.8                              1204 x 1536 -> 1536      -  | 8.3 | 7.9 | 8.3 | 10.5
-  //   301 x 1536 -> 1536      -  | 6.3 | 6.6 | 7.4 | 10.1           12000 x 2048 -> 300      -  | 16.3 | 14.5 | 13.4 | 16.8
+  //   301 x 1536 -> 1536      -  | 5.5 | 6.6 | 7.4 | 10.1           12000 x 2048 -> 300      -  | 16.3 | 14.5 | 13.4 | 16.8
   //   4816 x 1536 -> 1536     -  | 22.7 | 20.7 | 20.5 | 16.1        23001 x 1149 -> 264      -  | 18.0 | 16.0 | 17.0 | 18.9
   //   77056 x 768 -> 768      -  |  -   |  -   |  -   | 61.3 | 65.8   154112 x 128 -> 192    -  | 20.0 | 18.5 | 17.6 | 19.8
   //   77056 x 1152 -> 1152    -  |  -   |  -   |  -   | 125.9 | 118.6   77056 x 1536 -> 1536  -  |  -  |  -   |  -   | 231.9 | 180.8
   // float32 outputs (64 x 64 by 8 waves | by 4 | 64 x 128 | 128 x 128 by 4):
-  //   301 x 1536 -> 1536     8.8 | 9.3 | 11.3                       13446 x 704 -> 373      16.0 | 14.1 | 15.7 | 17.4
+  //   301 x 1536 -> 1536     8.0 | 9.3 | 11.3                       13446 x 704 -> 373      16.0 | 14.1 | 15.7 | 17.4
   //   4816 x 1536 -> 1536    38.6 | 33.2 | 32.6 | 27.8              154112 x 128 -> 192     26.8 | 24.1 | 26.6 | 29.4
   // weights in registers | 128 x 128:  77056 x 512 -> 512 29.9 | 33.9, -> 1024 49.4 | 59.1, -> 256 21.3 | 20.2;
   //   77056 x 384 -> 384 24.9 | 22.8;  77056 x 128 -> 512 18.3 | 19.6;  38528 x 512 -> 512 19.8 | 19.3
@@ -758,7 +793,7 @@ int launch_rows(const LinearArgs& p, hipStream_t s) {
   // persistent kernel where k-loops are long enough to hide its epilogue and two rounds of tiles or more are there.  Of the tiles
   // 128 x 128 once they give every CU one, unless the CU with the most of them has more to do than it has with 64 x 128, half the
   // work and a fifth more time for it (channels that end early in a tile, a second round for a few tiles); 64 x 64 below, by 8
-  // waves while there is no more than one a CU.
+  // waves (and in steps of four k-tiles, 128 KiB of LDS, where there are four) while there is no more than one a CU.
   const bool f32 = p.out_f32;
   if (ceil_div(p.n, 16) * ceil_div(p.rows, 16) <= 2ll * n_cu) {
     constexpr int NW = 8;
@@ -776,6 +811,7 @@ int launch_rows(const LinearArgs& p, hipStream_t s) {
   const int64_t rt = ceil_div(p.rows, 128), half = ceil_div(p.n, 64) * rt, full = ceil_div(p.n, 128) * rt, small = ceil_div(p.n, 64) * ceil_div(p.rows, 64);
   if (full >= n_cu && 5 * ceil_div(full, n_cu) < 3 * ceil_div(half, n_cu))
     return f32 ? launch_tile<128, 128, 4, true>(p, s) : launch_tile<128, 128, 8, false>(p, s);
+  if (small <= n_cu && p.kb >= 4) return f32 ? launch_tile<64, 64, 8, true, 4>(p, s) : launch_tile<64, 64, 8, false, 4>(p, s);
   if (small <= n_cu) return f32 ? launch_tile<64, 64, 8, true>(p, s) : launch_tile<64, 64, 8, false>(p, s);
   if (f32) return launch_tile<64, 64, 4, true>(p, s);
   return small <= 2 * n_cu ? launch_tile<64, 64, 4, false>(p, s) : launch_tile<64, 128, 8, false>(p, s);
