@@ -10,12 +10,14 @@
 
 The precision "fp8" of the embedding path runs on the same kernels.  Calls run on the current stream of the tensors'
 device, allocate only their outputs (none when they are passed in) and never synchronise, so they can be captured into a
-graph; there is no backward pass: tensors that require a gradient are refused while gradients are recorded.
+graph; there is no backward pass: tensors that require a gradient are refused while gradients are recorded, and so are the
+dual tensors of forward-mode differentiation.
 """
 import collections
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -39,14 +41,21 @@ def _gpu(dev):
     return dev
 
 
+def _has_tangent(t):
+    """Whether t is a dual tensor of forward-mode differentiation (its requires_grad is False, torch.no_grad() does not matter)."""
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
 def _same_device(dev, tensors):
-    """All on `dev` (a GPU), none of them part of a recorded gradient."""
+    """All on `dev` (a GPU), none of them part of a recorded gradient or of a forward derivative."""
     _gpu(dev)
     for t in tensors:
         if t.device != dev:
             raise ValueError("tensors on %s and %s" % (dev, t.device))
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError("no backward pass: call under torch.no_grad() or detach the inputs")
+    if forward_ad._current_level >= 0 and any(_has_tangent(t) for t in tensors):
+        raise ValueError("no forward derivative: a dual tensor; pass its primal (torch.autograd.forward_ad.unpack_dual)")
 
 
 def _call(dev, name, *args):
@@ -97,8 +106,8 @@ def _row_stride(x):
 
 def _out(what, out, shape, dtypes, dev):
     """Row stride of a tensor to write into."""
-    if out.requires_grad and torch.is_grad_enabled():
-        raise ValueError("%s: an output that requires a gradient" % what)
+    if out.requires_grad and torch.is_grad_enabled() or _has_tangent(out):
+        raise ValueError("%s: an output that requires a gradient, or a dual tensor" % what)
     if tuple(out.shape) != tuple(shape) or out.dtype not in dtypes or out.device != dev:
         raise ValueError("%s: expected %s %s on %s, got %s %s on %s" % (what, tuple(shape), "/".join(str(d) for d in dtypes), dev,
                                                                         tuple(out.shape), out.dtype, out.device))
@@ -164,8 +173,8 @@ class BlockFP8(object):
                              % (cols, blocks * self.BLOCK, _up(blocks, 4), tuple(data.shape), tuple(exponent.shape)))
         if data.device != exponent.device:
             raise ValueError("BlockFP8: data on %s, exponent on %s" % (data.device, exponent.device))
-        if data.requires_grad:
-            raise ValueError("BlockFP8: no backward pass: detach the data")
+        if data.requires_grad or _has_tangent(data):
+            raise ValueError("BlockFP8: no backward pass, no forward derivative: detach the data, take the primal")
         ld, lde = _row_stride(data), _row_stride(exponent)
         if ld is None or lde is None or ld % 16 or lde % 4 or data.data_ptr() % 16 or exponent.data_ptr() % 4:
             raise ValueError("BlockFP8: contiguous columns, data rows 16-byte aligned, exponent rows 4-byte aligned")

@@ -1,0 +1,61 @@
+"""
+What the 8-bit operators hand to the library and what they refuse, on the CPU: the check for a GPU is taken out and the
+library call is replaced by a record of its arguments, so nothing is launched.
+"""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import sugar_amd
+from sugar_amd import BlockFP8, RowNorm, block_fp8_linear, block_join, blockfp8, quantize_block_fp8
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The library calls a test makes, [(name, arguments)]; CPU tensors stand for the GPU's."""
+    made = []
+    monkeypatch.setattr(blockfp8, "_gpu", lambda dev: dev)
+    monkeypatch.setattr(blockfp8, "_call", lambda dev, name, *args: made.append((name, args)))
+    return made
+
+
+def operand(rows, cols):
+    q = BlockFP8.empty(rows, cols, "cpu")
+    q.data.view(torch.uint8).zero_()
+    q.exponent.fill_(127)
+    return q
+
+
+def join_args(call):
+    """The descriptor of a recorded join."""
+    name, (packed,) = call
+    assert name == "sugar_block_join"
+    return sugar_amd._lib.SugarBlockJoin.from_buffer_copy(packed)
+
+
+def test_dual_tensors_are_refused(calls):
+    """Forward-mode differentiation: a dual tensor does not require a gradient, its tangent would be dropped silently."""
+    c, r = 128, 4
+    x, res, vec, gate = torch.randn(r, c), torch.randn(r, c), torch.randn(c), torch.rand(r, c)
+    q = operand(r, c)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        bad = (lambda: quantize_block_fp8(dual(x)), lambda: block_fp8_linear(q, q, scale=dual(torch.randn(r))),
+               lambda: block_fp8_linear(q, q, shift=dual(torch.randn(r))), lambda: block_join(dual(x), res),
+               lambda: block_join(x, dual(res)), lambda: block_join(x, res, gate=dual(gate)), lambda: block_join(x, res, gate=dual(vec)),
+               lambda: block_join(x, res, post=RowNorm("rms", dual(vec))), lambda: block_join(x, res, pre=RowNorm("layer", None, dual(vec))),
+               lambda: block_join(x, res, pre=RowNorm("layer", dual(vec.double()))),
+               lambda: block_join(x, res, stream_out=dual(x.clone())), lambda: q.dequantize(out=dual(x.clone())),
+               lambda: block_fp8_linear(q, q, out_dtype=torch.float32, out=dual(torch.zeros(r, r))))
+        for grad in (True, False):                      # torch.no_grad() records no gradients, but forward derivatives all the same
+            with torch.set_grad_enabled(grad):
+                for call in bad:
+                    with pytest.raises(ValueError, match="dual"):
+                        call()
+        with pytest.raises(ValueError, match="forward derivative"):
+            BlockFP8(dual(q.data), q.exponent, c)
+        assert not calls
+        quantize_block_fp8(x)                            # plain tensors at a level, and what a dual tensor stands for
+        block_join(forward_ad.unpack_dual(dual(x)).primal, res, gate=gate)
+    block_join(x, res)
+    assert [name for name, _ in calls] == ["sugar_fp8_quant", "sugar_block_join", "sugar_block_join"]
