@@ -86,6 +86,7 @@ def _rows(what, x):
         raise ValueError("%s: %d columns, fewer than %d are taken" % (what, cols, MAX_COLS))
     ld, step = x.stride()
     if step != 1 or ld < cols:                          # (all but the plain case)
+        x = x.resolve_neg()                             # (one column of z.conj().imag: the memory holds the values negated)
         ld = _row_stride(x)
         if ld is None:
             x, ld = x.contiguous(), cols
@@ -112,8 +113,8 @@ def _out(what, out, shape, dtypes, dev):
         raise ValueError("%s: expected %s %s on %s, got %s %s on %s" % (what, tuple(shape), "/".join(str(d) for d in dtypes), dev,
                                                                         tuple(out.shape), out.dtype, out.device))
     ld = _row_stride(out)
-    if ld is None:
-        raise ValueError("%s: the columns of an output must be contiguous, its rows apart" % what)
+    if ld is None or out.is_neg():
+        raise ValueError("%s: the columns of an output must be contiguous, its rows apart, its values not a negated view" % what)
     return ld
 
 
@@ -145,11 +146,11 @@ def _apart(what, out, others, itself=()):
 
 def _vector(what, v, n):
     """A contiguous float32 vector of n (other float types and strides are converted)."""
-    if v.dtype is torch.float32 and v.shape == (n,) and v.is_contiguous():
+    if v.dtype is torch.float32 and v.shape == (n,) and v.is_contiguous() and not (n == 1 and v.is_neg()):
         return v
     if v.dim() != 1 or v.shape[0] != n or not v.dtype.is_floating_point:
         raise ValueError("%s: expected a floating vector of %d, got %s %s" % (what, n, v.dtype, tuple(v.shape)))
-    return v.to(torch.float32).contiguous()
+    return v.resolve_neg().to(torch.float32).contiguous()
 
 
 class BlockFP8(object):

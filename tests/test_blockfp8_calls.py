@@ -59,3 +59,22 @@ def test_dual_tensors_are_refused(calls):
         block_join(forward_ad.unpack_dual(dual(x)).primal, res, gate=gate)
     block_join(x, res)
     assert [name for name, _ in calls] == ["sugar_fp8_quant", "sugar_block_join", "sugar_block_join"]
+
+
+def test_views_whose_memory_holds_the_negated_values(calls):
+    """The imaginary part of a conjugate is a view with the sign still to be applied; one column of it passes for a plain matrix."""
+    view = torch.randn(6, 1, dtype=torch.complex64).conj().imag
+    vec = torch.randn(1, dtype=torch.complex64).conj().imag
+    assert view.is_neg() and vec.is_neg() and vec.is_contiguous()
+    x = torch.randn(6, 1)
+    quantize_block_fp8(view)
+    assert calls[-1][1][0] != view.data_ptr()
+    block_join(view, x, gate=vec)
+    j = join_args(calls[-1])
+    assert j.d_u != view.data_ptr() and j.d_gate != vec.data_ptr()
+    assert torch.equal(RowNorm("affine", vec).weight, vec) and not RowNorm("affine", vec).weight.is_neg()
+    n = len(calls)
+    for call in (lambda: operand(6, 1).dequantize(out=view), lambda: block_join(x, x.clone(), stream_out=view)):
+        with pytest.raises(ValueError, match="negated"):
+            call()
+    assert len(calls) == n
