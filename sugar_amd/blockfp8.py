@@ -424,15 +424,19 @@ def block_join(u, residual, post=None, gate=None, row_off=None, alpha=1.0, dense
         (q_ptr, e_ptr), ldq, lde = q._pointers(), q._ld, q._lde
     if stream_out is not None or normed_out is not None or quantized_out is not None:
         su, sr, out = _span(u, ldu), _span(residual, ldr), _span(stream, lds)
-        others = [su, sr] + [_span(t, ldg) for t in [gate, row_off] + inputs[2:n_vectors] if t is not None]
+        # read where they are written (an output may be u or residual itself), or by rows that others write
+        own, shared = [su, sr], [_span(t) for t in [row_off] + inputs[2:n_vectors] if t is not None]
+        if gate is not None:
+            (own if gate_kind == 3 else shared).append(_span(gate, ldg))
         parts = [] if q is None else q._spans()
-        _apart("block_join: stream_out", out, others + parts, (sr, su) if u_dtype == r_dtype else (sr,))
+        _apart("block_join: stream_out", out, shared + parts)
+        _apart("block_join: stream_out", out, own, (sr, su) if u_dtype == r_dtype else (sr,))
         if z is not None:
             sz = _span(z, ldz)
-            _apart("block_join: normed_out", sz, [out] + parts)
-            _apart("block_join: normed_out", sz, others, (su,) if z_dtype == u_dtype else ())
+            _apart("block_join: normed_out", sz, [out] + shared + parts)
+            _apart("block_join: normed_out", sz, own, (su,) if z_dtype == u_dtype else ())
         for span in parts:
-            _apart("block_join: quantized_out", span, others)
+            _apart("block_join: quantized_out", span, own + shared)
     if rows:
         _call(dev, "sugar_block_join", _JOIN.pack(
             rows, cols, utts, u_dtype, r_dtype, z_dtype, post_kind, pre_kind, gate_kind, 1 if dense else 0, alpha, post_eps, pre_eps,

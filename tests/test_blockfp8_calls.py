@@ -78,3 +78,21 @@ def test_views_whose_memory_holds_the_negated_values(calls):
         with pytest.raises(ValueError, match="negated"):
             call()
     assert len(calls) == n
+
+
+def test_an_output_that_is_the_gate_of_other_rows(calls):
+    """stream_out = u and normed_out = u are allowed because every value is read by the lane that writes it.  A gate per utterance
+    that is u as well is read for other rows too, by workgroups that may run later."""
+    c, r = 128, 6
+    off = torch.tensor([0, 3, 3, 4, 5, 6, 6], dtype=torch.int32)
+    u, res = torch.randn(r, c), torch.randn(r, c)
+    for kw in (dict(stream_out=u, gate=u), dict(normed_out=u, gate=u), dict(stream_out=res, gate=res)):
+        with pytest.raises(ValueError, match="shares memory"):
+            block_join(u, res, row_off=off, **kw)
+    assert not calls
+    block_join(u, res, row_off=off, gate=u)                                # outputs of their own
+    block_join(u, res, row_off=off, gate=torch.rand(r, c), stream_out=u)
+    block_join(u, res, gate=u, stream_out=u)                               # a gate per row is read where it is written
+    block_join(u, res, gate=res, stream_out=res, normed_out=u)
+    block_join(u, u, gate=u, stream_out=u)
+    assert len(calls) == 5
