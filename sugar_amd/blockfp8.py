@@ -301,9 +301,13 @@ def block_fp8_linear(a, w, scale=None, shift=None, relu=False, out_dtype=torch.b
     flags, sp, tp = _lib.EPI_RELU if relu else 0, None, None
     if scale is not None or shift is not None:
         _same_device(dev, [t for t in (scale, shift) if t is not None])
-        scale = torch.ones(n, device=dev) if scale is None else _vector("scale", scale, n)
-        shift = torch.zeros(n, device=dev) if shift is None else _vector("shift", shift, n)
-        flags, sp, tp = flags | _lib.EPI_AFFINE, scale.data_ptr(), shift.data_ptr()
+        flags |= _lib.EPI_AFFINE
+        if scale is not None:
+            scale = _vector("scale", scale, n)
+            sp = scale.data_ptr()
+        if shift is not None:
+            shift = _vector("shift", shift, n)
+            tp = shift.data_ptr()
     if out is None:
         if out_dtype not in _DT:
             raise ValueError("block_fp8_linear: out_dtype %s not in %s" % (out_dtype, [str(d) for d in _DT]))

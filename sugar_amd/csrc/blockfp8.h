@@ -215,7 +215,8 @@ struct Fp8Out {
   int y2_from = 0;
 };
 
-// y[r][o] = epilogue(sum_k a[r][k] w[o][k]), flags EPI_RELU | EPI_AFFINE (scale / shift [n], applied after the ReLU)
+// y[r][o] = epilogue(sum_k a[r][k] w[o][k]), flags EPI_RELU | EPI_AFFINE (scale / shift [n], applied after the ReLU; one of them
+// may be nullptr: 1 / 0)
 int launch_fp8_linear(const Fp8Operand& a, int64_t rows, const Fp8Operand& w, int n, int k, const float* scale,
                       const float* shift, int flags, const Fp8Out& out, hipStream_t s);
 

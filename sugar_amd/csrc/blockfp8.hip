@@ -202,7 +202,7 @@ int sugar_fp8_linear(const uint8_t* d_a, int64_t lda, const uint8_t* d_ae, int64
   SUGAR_CHECK_ARG(rows >= 0 && rows < (1ll << 27) && n > 0 && n < (1 << 24) && k > 0 && k < (1 << 24),
                   "fp8_linear: sizes out of range (rows %lld, n %d, k %d)", (long long)rows, n, k);
   SUGAR_CHECK_ARG((flags & ~(EPI_RELU | EPI_AFFINE)) == 0, "fp8_linear: unknown flags %d", flags);
-  SUGAR_CHECK_ARG(!(flags & EPI_AFFINE) || (d_scale && d_shift), "fp8_linear: affine epilogue without scale / shift");
+  SUGAR_CHECK_ARG(!(flags & EPI_AFFINE) || d_scale || d_shift, "fp8_linear: affine epilogue without scale and shift");
   SUGAR_CHECK_ARG(d_y && ldy >= n && (uintptr_t)d_y % (dtype == SUGAR_F32 ? 4 : 2) == 0, "fp8_linear: bad output");
   SUGAR_CHECK_ARG((uintptr_t)d_scale % 4 == 0 && (uintptr_t)d_shift % 4 == 0, "fp8_linear: unaligned scale / shift");
   int rc;

@@ -20,7 +20,7 @@ struct LinearArgs {
   unsigned lda, ldae, ldw, ldwe;      // rows x stride fits 32 bits (launch_fp8_linear cuts longer operands)
   int64_t ldy;
   void* y;
-  const float *scale, *shift;
+  const float *scale, *shift;         // under EPI_AFFINE; either may be missing (1 / 0), not both
   int rows, n, kb, flags, out_f32;
   int n_co_tiles;
   bf16* y2;                           // second store of columns >= y2_from (whole chunks of 8), or nullptr
@@ -129,8 +129,8 @@ __global__ __launch_bounds__(64 * NW) void fp8_linear_direct_kernel(LinearArgs p
   if (p.flags & EPI_AFFINE) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      sc[i] = p.scale[min(co + 4 * fq + i, p.n - 1)];
-      sh[i] = p.shift[min(co + 4 * fq + i, p.n - 1)];
+      if (p.scale) sc[i] = p.scale[min(co + 4 * fq + i, p.n - 1)];
+      if (p.shift) sh[i] = p.shift[min(co + 4 * fq + i, p.n - 1)];
     }
   }
   v = epilogue4(v, p.flags & EPI_RELU, p.flags & EPI_AFFINE, sc, sh);
@@ -169,8 +169,10 @@ __device__ __forceinline__ void fp8_tile(const LinearArgs& p, const int co_base,
   const bool relu = p.flags & EPI_RELU, affine = p.flags & EPI_AFFINE;
   if (affine && wv < TM / 32) {
     const int c = (wv % (TM / 64)) * 64;
-    dma<4>((const uint8_t*)(wv < TM / 64 ? p.scale : p.shift), 4 * min(co_base + c + lane, p.n - 1),
-           (unsigned char*)(aff + (wv < TM / 64 ? 0 : TM) + c));
+    const float* src = wv < TM / 64 ? p.scale : p.shift;
+    float* dst = aff + (wv < TM / 64 ? 0 : TM) + c;
+    if (src) dma<4>((const uint8_t*)src, 4 * min(co_base + c + lane, p.n - 1), (unsigned char*)dst);
+    else dst[lane] = wv < TM / 64 ? 1.f : 0.f;
   }
 
   unsigned woff[WI], xoff[XI];
@@ -431,8 +433,8 @@ __global__ __launch_bounds__(512, 2) void fp8_linear_short_kernel(LinearArgs p, 
   if (affine) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      sc[i] = p.scale[min(cl + i, p.n - 1)];
-      sh[i] = p.shift[min(cl + i, p.n - 1)];
+      if (p.scale) sc[i] = p.scale[min(cl + i, p.n - 1)];
+      if (p.shift) sh[i] = p.shift[min(cl + i, p.n - 1)];
     }
   }
   // Every tile but a run's last stores all its rows; where this wave's channels are all inside too, D tiles' stores (and KB
@@ -541,6 +543,8 @@ __device__ __forceinline__ void fp8_tiles_persist(const LinearArgs& p, const int
   const bool relu = p.flags & EPI_RELU, affine = p.flags & EPI_AFFINE;
   unsigned* exps = (unsigned*)(smem + PEXPS);                    // [2][256 channels | 256 rows]
   float* aff = (float*)(smem + PAFF);                            // [scale 256 | shift 256]
+  const float* vec = wv < 4 ? p.scale : p.shift;
+  if (affine && !vec) aff[wv * 64 + lane] = wv < 4 ? 1.f : 0.f;  // the missing one, for all tiles
 
   unsigned woff[4], xoff[4], eoff;
   const uint8_t* ebase = wv < 4 ? p.we : p.ae;                   // exponents: waves 0..3 the channels', 4..7 the rows'
@@ -603,9 +607,9 @@ __device__ __forceinline__ void fp8_tiles_persist(const LinearArgs& p, const int
     if (counted) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NSTORE) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the tile's first k-tile is there, every wave out of its epilogue
-    if (affine) {                                                // the tile's 256 scales | 256 shifts, 64 a wave
+    if (affine && vec) {                                         // the tile's 256 scales | 256 shifts, 64 a wave
       const int c = min(co_base + (wv & 3) * 64 + lane, p.n - 1);
-      dma<4>((const uint8_t*)(wv < 4 ? p.scale : p.shift), 4 * c, (unsigned char*)(aff + wv * 64));
+      dma<4>((const uint8_t*)vec, 4 * c, (unsigned char*)(aff + wv * 64));
     }
     dma_x(par ^ 1, 1, 0);                                        // (not staged earlier: the epilogue went through that stage)
     dma_x(par ^ 1, 1, 2);

@@ -1,6 +1,6 @@
 """
-What the 8-bit operators hand to the library and what they refuse, on the CPU: the check for a GPU is taken out and the
-library call is replaced by a record of its arguments, so nothing is launched.
+What the 8-bit operators hand to the library and what they refuse.  On the CPU the check for a GPU is taken out and the library
+call is replaced by a record of its arguments, so nothing is launched; what the kernels make of such calls is tested on a GPU.
 """
 import pytest
 import torch
@@ -8,6 +8,8 @@ from torch.autograd import forward_ad
 
 import sugar_amd
 from sugar_amd import BlockFP8, RowNorm, block_fp8_linear, block_join, blockfp8, quantize_block_fp8
+
+gpu = pytest.mark.gpu
 
 
 @pytest.fixture
@@ -96,3 +98,61 @@ def test_an_output_that_is_the_gate_of_other_rows(calls):
     block_join(u, res, gate=res, stream_out=res, normed_out=u)
     block_join(u, u, gate=u, stream_out=u)
     assert len(calls) == 5
+
+
+def test_one_affine_vector_is_passed_on_alone(calls, monkeypatch):
+    """scale without shift, or the other way: no vector is made up for the missing one (an allocation and a launch a call)."""
+    a, w, out = operand(5, 256), operand(16, 256), torch.zeros(5, 16)
+    s = torch.randn(16)
+    for name in ("ones", "zeros", "full", "empty"):
+        monkeypatch.setattr(torch, name, None)
+    for kw, want in ((dict(scale=s), (s.data_ptr(), None)), (dict(shift=s), (None, s.data_ptr())), (dict(scale=s, shift=s), 2 * (s.data_ptr(),)),
+                     (dict(), (None, None))):
+        block_fp8_linear(a, w, out=out, **kw)
+        name, args = calls[-1]
+        assert name == "sugar_fp8_linear" and args[11:13] == want and args[13] == (2 if kw else 0)
+
+
+# ------------------------------------------------------------------------------------------------ the same on a GPU
+def rows_of(seed, r, c, spread=0.5):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(r, c, generator=g) * torch.exp(spread * torch.randn(c, generator=g))
+
+
+@gpu
+@pytest.mark.parametrize("r,n,k", [(3, 40, 300), (600, 600, 300), (301, 1536, 1536), (1204, 1530, 1536), (12000, 300, 1030), (9000, 1400, 100),
+                                   (12001, 536, 528), (60000, 511, 512), (52016, 1000, 200), (23000, 1536, 1152), (44000, 776, 1400),
+                                   (100001, 264, 1024)])
+def test_one_affine_vector_is_the_same_as_two(r, n, k):
+    """Every kernel of the product: a missing scale is 1 and a missing shift 0, bit for bit, and columns around
+    the output are left alone."""
+    a, w = quantize_block_fp8(rows_of(r, r, k).cuda()), quantize_block_fp8(rows_of(r + 1, n, k).cuda() / k ** 0.5)
+    s, t = (rows_of(8 + i, 1, n)[0].cuda() for i in range(2))
+    for dtype in (torch.bfloat16, torch.float32):
+        out = torch.full((r, n + 3), 7.0, dtype=dtype, device="cuda")
+        for kw, both in ((dict(scale=s), (s, torch.zeros_like(s))), (dict(shift=t, relu=True), (torch.ones_like(t), t))):
+            want = block_fp8_linear(a, w, scale=both[0], shift=both[1], relu=kw.get("relu", False), out_dtype=dtype)
+            block_fp8_linear(a, w, out=out[:, 1:n + 1], **kw)
+            assert torch.equal(out[:, 1:n + 1], want), (dtype, sorted(kw))
+            assert (out[:, 0] == 7).all() and (out[:, n + 1:] == 7).all()
+
+
+@gpu
+def test_calls_with_their_outputs_passed_in_allocate_nothing():
+    r, c, n = 300, 512, 264
+    x, res = rows_of(1, r, c).bfloat16().cuda(), rows_of(2, r, c).bfloat16().cuda()
+    w, s = quantize_block_fp8(rows_of(3, n, c).cuda()), rows_of(4, 1, n)[0].cuda()
+    q, y, back = BlockFP8.empty(r, c, "cuda"), torch.empty(r, n, device="cuda"), torch.empty_like(x)
+    norm, gate, off = RowNorm("layer", rows_of(5, 1, c)[0].cuda()), torch.rand(2, c).cuda(), torch.tensor([0, 9, r], dtype=torch.int32).cuda()
+    stream, z = torch.empty_like(x), torch.empty_like(x)
+
+    def run():
+        quantize_block_fp8(x, out=q)
+        q.dequantize(out=back)
+        for kw in (dict(), dict(scale=s), dict(shift=s), dict(scale=s, shift=s)):
+            block_fp8_linear(q, w, out=y, **kw)
+        block_join(x, res, post=norm, gate=gate, row_off=off, pre=norm, stream_out=stream, normed_out=z, quantized_out=q)
+    run()
+    before = torch.cuda.memory_stats()["allocation.all.allocated"]
+    run()
+    assert torch.cuda.memory_stats()["allocation.all.allocated"] == before
