@@ -827,11 +827,11 @@ int launch_fp8_linear(const Fp8Operand& a, int64_t rows, const Fp8Operand& w, in
                       const float* shift, int flags, const Fp8Out& out, hipStream_t s) {
   // the kernels' row offsets are 32-bit: weights that do not fit are refused, rows beyond go to a launch of their own
   constexpr int64_t SPAN = (1ll << 32) - 4096;
-  SUGAR_CHECK_ARG(n * w.ldq <= SPAN && n * w.lde <= SPAN, "fp8_linear: weights of %d rows with stride %lld are too large", n,
-                  (long long)w.ldq);
-  SUGAR_CHECK_ARG(a.ldq <= SPAN / 256 && a.lde <= SPAN / 256, "fp8_linear: row stride %lld too large", (long long)a.ldq);
+  const int64_t w_ld = w.ldq > w.lde ? w.ldq : w.lde, a_ld = a.ldq > a.lde ? a.ldq : a.lde;
+  SUGAR_CHECK_ARG(w_ld <= SPAN / n, "fp8_linear: weights of %d rows with stride %lld are too large", n, (long long)w_ld);
+  SUGAR_CHECK_ARG(a_ld <= SPAN, "fp8_linear: row stride %lld too large", (long long)a_ld);
   SUGAR_CHECK_ARG(!out.y2 || (n % 8 == 0 && out.y2_from % 8 == 0 && out.dtype == SUGAR_BF16), "fp8_linear: second output of ragged chunks");
-  const int64_t per = SPAN / (a.ldq > a.lde ? a.ldq : a.lde) / 256 * 256;
+  const int64_t fit = SPAN / a_ld, per = fit >= 256 ? fit / 256 * 256 : fit;
   const int esz = out.dtype == SUGAR_F32 ? 4 : 2;
   LinearArgs p;
   p.lda = (unsigned)a.ldq; p.ldae = (unsigned)a.lde;

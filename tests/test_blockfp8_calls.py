@@ -156,3 +156,35 @@ def test_calls_with_their_outputs_passed_in_allocate_nothing():
     before = torch.cuda.memory_stats()["allocation.all.allocated"]
     run()
     assert torch.cuda.memory_stats()["allocation.all.allocated"] == before
+
+
+@gpu
+def test_the_widest_operands():
+    """2^24 - 1 columns, the most that the documentation allows; a launch of the product takes 255 such rows.  Ones, zeros and twos:
+    sums below 2^24 are exact in float32, and in the 8-bit instruction too (products of 1, 2 and 4)."""
+    k, r, n = (1 << 24) - 1, 300, 5
+    x = torch.zeros(2, k, device="cuda", dtype=torch.bfloat16)
+    x[0, ::3], x[1, -1], x[1, 7] = 1.5, -448.0, 0.25
+    assert torch.equal(quantize_block_fp8(x).dequantize(torch.bfloat16), x)
+    one, two = 0x38, 0x40                                                  # 1.0 and 2.0
+    a, w = BlockFP8.empty(r, k, "cuda"), BlockFP8.empty(n, k, "cuda")
+    for q in (a, w):
+        q.data.view(torch.uint8).zero_()
+        q.exponent.fill_(127)
+    ab, wb = a.data.view(torch.uint8), w.data.view(torch.uint8)
+    ab[:, :1 << 23] = one
+    rows = torch.arange(r, device="cuda")
+    ab[rows, 1000 * rows] = two
+    ab[:, k - 1] = one
+    ab[::2, k - 1] = two
+    wb[0, :k] = one                                                        # sums of rows
+    wb[1, k - 1] = one                                                     # the last column
+    wb[2, 255 * 1000] = one                                                # the column of row 255, the second launch's first
+    wb[3, :1 << 22] = two
+    last = torch.where(rows % 2 == 0, 2.0, 1.0).double()
+    want = torch.stack([(1 << 23) + 1 + last, last, 1.0 + (rows == 255), 2.0 * ((1 << 22) + (1000 * rows < 1 << 22)), 0 * last], 1)
+    assert torch.equal(block_fp8_linear(a, w, out_dtype=torch.float32).double(), want)
+    assert torch.equal(block_fp8_linear(a, w), want.to(torch.bfloat16))
+    assert torch.equal(block_fp8_linear(a[253:257], w, out_dtype=torch.float32).double(), want[253:257])
+    with pytest.raises(ValueError, match="too large"):                     # weights of 4 GiB and more
+        block_fp8_linear(w, a)
