@@ -834,3 +834,48 @@ def test_join_more_rows_than_short_runs_cover():
     out = block_join(u, res, alpha=2.0, normed=False, stream_out=res).stream
     assert out[probe, 0].tolist() == [2.0 * i for i in range(2, 9)]
     assert int((out == 2).sum()) == r - len(probe)
+
+
+@gpu
+@pytest.mark.parametrize("tu,ts", TYPES)
+@pytest.mark.parametrize("r,c", [(12000, 512), (20011, 200), (40003, 100), (9001, 600), (5003, 1500), (3001, 3000), (40003, 5)])
+def test_join_utterances_begin_inside_runs_of_rows(tu, ts, r, c):
+    """Rows enough that a group of lanes takes 2 .. 4 of them one after the other (share of launch_join >= 2 on 256 CUs).  Utterances
+    of 0 .. 6 rows begin inside those runs: the gate changes within them, rows of no utterance end them."""
+    g = torch.Generator().manual_seed(r + c)
+    sizes = torch.randint(0, 7, (r // 3,), generator=g)
+    sizes = sizes[sizes.cumsum(0) < r - 9]
+    off = torch.cat([torch.tensor([3]), 3 + sizes.cumsum(0)]).to(torch.int32)
+    n, b = int(off[-1]), len(sizes)
+    u, res, gate = rows_of(1, r, c, tu).cuda(), rows_of(2, r, c, ts).cuda(), torch.rand(b, c, generator=g).cuda()
+    for kw in (dict(dense=True), dict(post=norm_of("rms", c, 3), pre=norm_of("layer", c, 5), alpha=0.7)):
+        kw.update(gate=gate, row_off=off.cuda())
+        stream, z, q = torch.full((r, c), 7.0, dtype=ts).cuda(), torch.full((r, c), 7.0).cuda(), BlockFP8.empty(r, c, "cuda")
+        q.data.view(torch.uint8).fill_(0x55)
+        q.exponent.fill_(9)
+        j = block_join(u, res, stream_out=stream, normed_out=z, quantized_out=q, **kw)
+        check_join(j, u, res, rows=slice(3, n), **kw)
+        for rows in (slice(0, 3), slice(n, r)):
+            assert (stream[rows] == 7).all() and (z[rows] == 7).all()
+            assert (q.data[rows].view(torch.uint8) == 0x55).all() and (q.exponent[rows] == 9).all()
+
+
+@gpu
+@pytest.mark.parametrize("tu,ts", TYPES)
+@pytest.mark.parametrize("r,c", [(12000, 512), (20011, 200), (40003, 100), (9001, 600), (5003, 1500), (40003, 5)])
+def test_join_runs_of_rows_with_gates_and_in_place(tu, ts, r, c):
+    """The same runs with a gate per row, fetched with the row ahead, with one per channel and with none; outputs in place of the
+    inputs, whose next row has been fetched by then."""
+    u, res = rows_of(1, r, c, tu).cuda(), rows_of(2, r, c, ts).cuda()
+    norms = dict(post=norm_of("layer", c, 3), pre=norm_of("rms", c, 5))
+    row_gate, channel_gate = torch.rand(r, c).to(tu).cuda(), torch.rand(c).cuda()
+    for kw in (dict(gate=row_gate), dict(gate=row_gate, **norms), dict(gate=channel_gate), dict(gate=channel_gate, **norms), dict(alpha=-2.0)):
+        want = block_join(u, res, quantized=True, **kw)
+        check_join(want, u, res, **kw)
+        u2, res2 = u.clone(), res.clone()
+        got = block_join(u2, res2, stream_out=res2, normed_out=u2, quantized=True, **kw)
+        assert torch.equal(res2, want.stream) and torch.equal(u2, want.normed) and torch.equal(got.quantized.exponent, want.quantized.exponent)
+        assert torch.equal(got.quantized.data.view(torch.uint8), want.quantized.data.view(torch.uint8))
+        if tu == ts:
+            u2 = u.clone()
+            assert block_join(u2, res, stream_out=u2, **kw).stream is u2 and torch.equal(u2, want.stream)
