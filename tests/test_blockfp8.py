@@ -879,3 +879,13 @@ def test_join_runs_of_rows_with_gates_and_in_place(tu, ts, r, c):
         if tu == ts:
             u2 = u.clone()
             assert block_join(u2, res, stream_out=u2, **kw).stream is u2 and torch.equal(u2, want.stream)
+
+
+@gpu
+@pytest.mark.parametrize("r,n,k", [(52007, 457, 100), (52016, 1001, 200), (35001, 779, 384), (60000, 511, 512),          # weights in registers
+                                   (23000, 1531, 1152), (44000, 773, 1400), (100001, 261, 1024),                     # persistent, each tail
+                                   (9000, 1399, 100), (4816, 1533, 640)])                                                # 128 x 128 tiles
+def test_linear_many_rows_of_odd_widths(r, n, k):
+    """Output widths that are no multiple of 8 over many rows: every kernel's stores of the last 1 .. 7 channels, and the half
+    tile of float32 outputs (773)."""
+    check_many_rows(r, n, k)
