@@ -289,8 +289,9 @@ int sugar_snorm_trials(const float* d_scores, const int32_t* d_enroll, const int
  * sugar_fp8_dequant: d_y [rows][ldy] dtype <- the values (exact in either dtype within its normal range; a float32
  *   magnitude that rounded up to 2^128 reads back as infinity).
  * sugar_fp8_linear: d_y[r][o] = epilogue(sum_k a[r][k] w[o][k]), f32 accumulation.  SUGAR_F32 outputs: exact
- *   products of the values as bfloat16 numbers (which they are from 2^-133 up to 2^128), float32 sums.  SUGAR_BF16 outputs: the 8-bit matrix instruction, which aligns 8 neighbouring products to the
- *   largest and cuts them 2^-13 below its leading bit (1.5e-5 of the result on random operands; bf16 rounds by 1.7e-3).
+ *   products of the values as bfloat16 numbers (which they are from 2^-133 up to 2^128), float32 sums.  SUGAR_BF16 outputs:
+ *   the 8-bit matrix instruction, which aligns 8 neighbouring products to the largest and cuts them 2^-13 below its leading
+ *   bit (1.5e-5 of the result in the 2-norm on random operands, more of a sum that cancels; bf16 rounds by 1.7e-3).
  *   flags bit0 ReLU, bit1 * d_scale[o] + d_shift[o] after it (float32 [n]; one of them may be NULL: 1 / 0); d_y [rows][ldy]
  *   dtype.  The left operand is rows x k, the weights n x k; a call allocates nothing and needs no workspace. */
 int sugar_fp8_quant(const void* d_x, int64_t ldx, int dtype, int64_t rows, int cols, uint8_t* d_q, int64_t ldq,

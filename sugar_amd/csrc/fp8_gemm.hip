@@ -144,7 +144,7 @@ __global__ __launch_bounds__(64 * NW) void fp8_linear_direct_kernel(LinearArgs p
 // barrier and latencies with: steps of 4 (301 x 1536 -> 1536 5.5 us, by single k-tiles 5.9; deeper rings of single k-tiles do not
 // help).  Exponents travel as one dword per row and four k-tiles, staged with the first of the four (double buffer) and shifted
 // down a byte per k-tile.
-// Bound by the DMA into LDS (128 x 128 tiles: 64 operations a byte) and, at few k-tiles, by the first tile's way in and the
+// Bound by the DMA into LDS (128 x 128 tiles: 128 operations a byte) and, at few k-tiles, by the first tile's way in and the
 // stores: 301 x 1536 -> 1536 5.5 us (64 x 64), float32 output 8.0; 19264 x 528 -> 536 14.8 us, float32 21.8.
 // 128 x 128 with float32 outputs: 4 waves of 64 x 64 convert 8 fragments for 16 products where 8 waves of 64 x 32 convert 6 for
 // 8; 77056 x 1536 -> 1536 352 us (1.03 PF) against 377, x 100 -> 1400 121 / 153, 25000 x 300 -> 700 23.9 / 23.0.  Left out one at
@@ -358,8 +358,8 @@ int launch_tile(LinearArgs p, hipStream_t s) {
 // ------------------------------------------------------------------------------------------ weights in registers, many rows
 // A tile kernel stages both operands of every tile (77 056 x 512 x 512 in 128 x 128 tiles: 315 MB through LDS for 118 MB of
 // tensors), and at K <= 512 that DMA bounds it.  Here the WEIGHTS stay: a workgroup owns a slab of 256 channels, each of its
-// 8 waves the fragments of 32 of them for the whole of K in registers (16 KB a lane), and walks a run of rows in tiles of
-// 64.  Only rows move, once per slab, through a ring of LDS stages ([64 rows][128 bytes] per block) that runs on across
+// 8 waves the fragments of 32 of them for the whole of K in registers (16 KB a wave, 256 bytes a lane, at K = 512), and walks a
+// run of rows in tiles of 64.  Only rows move, once per slab, through a ring of LDS stages ([64 rows][128 bytes] per block) that runs on across
 // tiles; one barrier a tile.  Row i of a wave's 16-channel tile m is channel 8 (i / 4) + 4 m + i % 4 of its 32 (wreg_row), so
 // that a lane's 8 results of a row are neighbours: one 16-byte store straight from the accumulators.
 // 77 056 x 512 -> 512: 30 us (3.9 TB/s; 128 x 128 tiles 33), of which the rows beyond the first take 0.27 ns each (5.7 TB/s)
