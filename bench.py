@@ -76,21 +76,28 @@ HBM_PEAK_GBS = 8000.0      # MI355X_MICROARCH.md: HBM3E ~8 TB/s
 
 def stage_roofline(stages_ms, config, B, L, R, precision):
     """Per stage: algorithmic GFLOP and MB per step, the roofline that bounds it and the fraction
-    of that roofline the measured time reaches.  Bytes count each activation tensor once in and once out."""
+    of that roofline the measured time reaches.  Bytes count each activation tensor once in and once out.
+    "fp8": block outputs are one byte a value and one a block of 128, and catconv and the first convs behind a block multiply in
+    8 bits; where a block's output is no multiple of 512 channels those first convs read it in 16 bits, and it is written in both."""
     depth, ch, ks, ccat = config
-    esz = 4 if precision == "fp32" else 2        # ("fp8": block outputs are one byte, the rest of the path two)
+    esz = 4 if precision == "fp32" else 2        # of what is not held in 8 bits
     c0 = ch[0]
+    fp8 = precision == "fp8"
+    first8 = fp8 and -(-c0 // 128) % 4 == 0      # (the exponent bytes of its column slice begin on a dword)
+    cat_sz = 1 + 1 / 128 if fp8 else esz         # a value of a block's output as catconv reads it
+    join_sz = cat_sz + (esz if fp8 and not first8 else 0)    # and as it is written where a block follows
     w = [ch[i + 1] // 8 for i in range(depth)]
     mid = [8 * x for x in w]
     work = {   # stage: (flops, bytes)
         "fbank_dft+instnorm": (0.0, 4.0 * B * L + esz * 80.0 * R),
         "layer1": (2.0 * R * c0 * 80 * ks[0], (80.0 + c0) * R * esz),
-        "first_conv": (sum(2.0 * R * c0 * m for m in mid), sum((c0 + m) * R * esz for m in mid)),
+        "first_conv": (sum(2.0 * R * c0 * m for m in mid),
+                       sum((c0 * (cat_sz if first8 and i else esz) + m * esz) * R for i, m in enumerate(mid))),
         "res2_steps": (sum(7 * 2.0 * R * x * x * ks[i + 1] for i, x in enumerate(w)), sum(2.0 * 7 * x * R * esz for x in w)),
         "last_conv": (sum(2.0 * R * m * c0 for m in mid), sum((m + c0) * R * esz for m in mid)),
         "se_scale": (0.0, depth * c0 * R * esz * 1.0),
-        "se_apply": (0.0, (4.0 * (depth - 1) + 3.0) * c0 * R * esz),
-        "catconv": (2.0 * R * depth * c0 * ccat, (depth * c0 + ccat) * R * esz * 1.0),
+        "se_apply": (0.0, ((3.0 * esz + join_sz) * (depth - 1) + 2.0 * esz + cat_sz) * c0 * R),
+        "catconv": (2.0 * R * depth * c0 * ccat, (depth * c0 * cat_sz + ccat * esz) * R * 1.0),
         "pool_linear1": (2.0 * R * ccat * 128, (ccat + 128.0) * R * esz),
         "pool_stats": (2.0 * R * 128 * ccat, (ccat + 128.0) * R * esz),
     }
@@ -99,9 +106,11 @@ def stage_roofline(stages_ms, config, B, L, R, precision):
         ms = stages_ms.get(name)
         if not ms:
             continue
-        # "fp8": catconv in 8 bits (and most first convs; priced at the 16-bit peak here), every other product in 16
-        peak_tf = PEAK["bf16" if precision == "fp8" and name != "catconv" else precision][0]
-        t_mfma, t_hbm = flops / (peak_tf * 1e12), nbytes / (HBM_PEAK_GBS * 1e9)
+        in8 = 0.0                                # operations in 8 bits
+        if fp8:
+            in8 = flops if name == "catconv" else sum(2.0 * R * c0 * m for m in mid[1:]) if first8 and name == "first_conv" else 0.0
+        t_mfma = (flops - in8) / (PEAK["bf16" if fp8 else precision][0] * 1e12) + in8 / (PEAK["fp8"][0] * 1e12)
+        t_hbm = nbytes / (HBM_PEAK_GBS * 1e9)
         bound = "mfma" if t_mfma > t_hbm else "hbm"
         out[name] = {"ms": ms, "gflop": round(flops / 1e9, 2), "mbytes": round(nbytes / 1e6, 1), "bound": bound,
                      "tflops": round(flops / (ms * 1e-3) / 1e12, 1), "gbytes_per_s": round(nbytes / (ms * 1e-3) / 1e9, 1),
@@ -341,7 +350,7 @@ def main():
                        "weights": "deterministic synthetic (sugar_amd/synth.py)"},
             "roofline": {"kernel": "%s catconv launch [%d frames x K %d -> %d]"
                                    % ("gemm1x1_persist_kernel (256x256x64 LDS-DMA MFMA GEMM, quadrant ping-pong schedule, persistent split-tail grid)" if args.precision == "bf16"
-                                      else "fp8_linear_persist_kernel (256x256x128 block-scaled 8-bit product, persistent)" if args.precision == "fp8"
+                                      else "block-scaled 8-bit product (sugar_fp8_linear)" if args.precision == "fp8"
                                       else "conv_gemm_kernel<float,128,128>", R, depth * ch[0], ccat),
                          "bound": "mfma", "achieved": round(achieved, 2) if achieved else None, "peak": peak,
                          "unit": "TFLOP/s", "frac": round(achieved / peak, 4) if achieved else None,

@@ -213,3 +213,33 @@ def test_lists_and_sweeps(supernet, meta):
             eer, dcf = sugar_amd.veri_validate(loader, one, device=DEV)
             r = got[(cfg[0], tuple(cfg[1]), tuple(cfg[2]), cfg[3])]
             assert r["eer"] == eer[0] and r["mindcf"] == dcf[0], (recal_loader is not None, cfg)
+
+
+def test_stage_roofline_counts_8_bit_tensors_and_products():
+    """bench.py's bytes and operations a stage, against counts written out here."""
+    import bench
+    B, T = 4, 301
+    R, ones = B * T, {k: 1.0 for k in ("first_conv", "se_apply", "catconv", "last_conv")}
+    e8 = 1 + 1 / 128
+    got = {}
+    for name in ("base", "three_blocks"):
+        depth, ch, ks, ccat = CONFIGS[name]
+        for p in ("bf16", "fp8"):
+            got[name, p] = bench.stage_roofline(ones, CONFIGS[name], B, 48000, R, p)
+            assert got[name, p]["catconv"]["gflop"] == round(2.0 * R * depth * ch[0] * ccat / 1e9, 2)
+    mb = lambda per_row: round(per_row * R / 1e6, 1)
+    c = 512                                             # base: 3 blocks of 512, all first convs but the first in 8 bits, 1536 out
+    assert got["base", "bf16"]["se_apply"]["mbytes"] == mb(11 * c * 2) and got["base", "bf16"]["catconv"]["mbytes"] == mb((3 * c + 1536) * 2)
+    assert got["base", "bf16"]["first_conv"]["mbytes"] == mb(3 * 2 * c * 2)
+    assert got["base", "fp8"]["se_apply"]["mbytes"] == mb(2 * (6 + e8) * c + (4 + e8) * c)
+    assert got["base", "fp8"]["catconv"]["mbytes"] == mb(3 * c * e8 + 1536 * 2)
+    assert got["base", "fp8"]["first_conv"]["mbytes"] == mb(3 * c * 2 + c * 2 + 2 * c * e8)
+    c = 384                                             # three scale blocks a slice: 16-bit first convs, block outputs in both types
+    mid = [8 * (x // 8) for x in CONFIGS["three_blocks"][1][1:]]
+    assert got["three_blocks", "fp8"]["first_conv"] == got["three_blocks", "bf16"]["first_conv"]
+    assert got["three_blocks", "fp8"]["se_apply"]["mbytes"] == mb(2 * (8 + e8) * c + (4 + e8) * c)
+    assert got["three_blocks", "fp8"]["last_conv"]["mbytes"] == mb(sum(m + c for m in mid) * 2)
+    # a product that is bound by the matrix pipes: two of three first convs at twice the rate
+    wide = (3, [4096, 4096, 4096, 4096], [5, 3, 3, 3], 1536)
+    t = {p: bench.stage_roofline(ones, wide, B, 48000, R, p)["first_conv"] for p in ("bf16", "fp8")}
+    assert t["bf16"]["bound"] == t["fp8"]["bound"] == "mfma" and abs(t["fp8"]["frac"] / t["bf16"]["frac"] - 2 / 3) < 0.02
