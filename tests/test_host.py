@@ -326,3 +326,13 @@ def test_dataset_walk_keeps_order_and_surfaces_loader_errors():
             break                                                     # the generator is closed: its pool shuts down
     assert len(d.seen) < 200
     assert list(_walk(Data(0, 0), 4)) == [] and len(list(_walk(Data(3, 0), 4))) == 3
+
+
+def test_entry_build_compiles_whatever_is_there(monkeypatch):
+    """build() compiles on every call, a library that is up to date by its files' times included."""
+    import __graft_entry__ as entry
+    from sugar_amd import build
+    seen = []
+    monkeypatch.setattr(build, "build", lambda force=False, verbose=True: seen.append(force))
+    entry.build()
+    assert seen == [True]
