@@ -49,6 +49,17 @@ typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(2))) float f32x2;
 typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
 
+// Bijective XCD-aware remap of a launch index (blocks b and b + 8 share an XCD's L2): consecutive results stay on one XCD, so
+// tiles that re-read one activation row tile hit that XCD's L2.
+__device__ __forceinline__ int xcd_remap(int bid, int nwg) {
+  const int q = nwg >> 3, r = nwg & 7, xcd = bid & 7, seq = bid >> 3;
+  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + seq;
+}
+
+// Byte offset of a 16-byte chunk in an LDS tile whose rows are 128 bytes; the chunks of a row are permuted by the row so that
+// 16 lanes reading one chunk of 16 rows spread over the banks.
+__device__ __forceinline__ int swz(int row, int chunk) { return row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4); }
+
 // Opt a kernel in to more than 64 KiB of dynamic LDS.  Function attributes are per device, so the "done" state is a
 // bit per device ordinal (one atomic word per call site); a race between two threads only repeats the call.
 typedef std::atomic<unsigned long long> OptInMask;

@@ -69,13 +69,6 @@ __device__ long long* g_gemm_stamps;
 #define GEMM_STAMP() do {} while (0)
 #endif
 
-__device__ __forceinline__ int swz(int row, int chunk) { return row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4); }
-
-__device__ __forceinline__ int xcd_remap2(int bid, int nwg) {
-  const int q = nwg >> 3, r = nwg & 7, xcd = bid & 7, seq = bid >> 3;
-  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + seq;
-}
-
 // One TM x TN output tile at (co_base, r_base), by the whole 512-thread workgroup.
 template <int TM, int TN, int NS, int PP = 0>
 __device__ __forceinline__ void gemm_tile(const Gemm1x1Args& a, const int co_base, const int r_base) {
@@ -324,7 +317,7 @@ __device__ __forceinline__ void gemm_tile(const Gemm1x1Args& a, const int co_bas
 // Uniform grid: every workgroup one TM x TN tile.
 template <int TM, int TN, int NS, int PP = 0>
 __global__ __launch_bounds__(512, TM == 256 ? 2 : 4) void gemm1x1_kernel(Gemm1x1Args a) {
-  const int vid = xcd_remap2(blockIdx.x, gridDim.x);
+  const int vid = xcd_remap(blockIdx.x, gridDim.x);
   gemm_tile<TM, TN, NS, PP>(a, (vid % a.n_co_tiles) * TM, (vid / a.n_co_tiles) * TN);
 }
 
@@ -338,7 +331,7 @@ template <int NS, int PP = 0>
 __global__ __launch_bounds__(512, 2) void gemm1x1_split_kernel(Gemm1x1Args a, int n_main, int split) {
   const int bid = blockIdx.x;
   if (bid < n_main) {
-    const int vid = xcd_remap2(bid, n_main);
+    const int vid = xcd_remap(bid, n_main);
     gemm_tile<256, 256, NS, PP>(a, (vid % a.n_co_tiles) * 256, (vid / a.n_co_tiles) * 256);
     return;
   }

@@ -70,13 +70,6 @@ __device__ __forceinline__ u32x4 add_chunks<bf16>(u32x4 a, u32x4 b) {
   return __builtin_bit_cast(u32x4, r);
 }
 
-// Bijective XCD-aware remap (blocks b and b+8 share an XCD's L2): consecutive virtual ids stay on one XCD, so
-// the co-tiles that re-read one activation row tile hit that XCD's L2.
-__device__ __forceinline__ int xcd_remap(int bid, int nwg) {
-  const int q = nwg >> 3, r = nwg & 7, xcd = bid & 7, seq = bid >> 3;
-  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + seq;
-}
-
 // Fixed-order reduce-scatter over the 32 lanes of one half wave (lanes that share `lane >> 5`): every lane brings 16
 // values; afterwards lane l holds, for value index (l >> 1) & 15, the sum over the 32 lanes (both lanes of a pair hold
 // the same number).  16 cross-lane moves instead of 16 x 5 for one butterfly per value.

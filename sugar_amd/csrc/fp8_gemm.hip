@@ -31,13 +31,6 @@ struct LinearArgs {
 // ReLU in one instruction that hands NaN on (a maximum, not a maxNum)
 __device__ __forceinline__ float relu_nan(float v) { return __builtin_elementwise_maximum(v, 0.f); }
 
-__device__ __forceinline__ int swz(int row, int chunk) { return row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4); }
-
-__device__ __forceinline__ int xcd_remap(int bid, int nwg) {
-  const int q = nwg >> 3, r = nwg & 7, xcd = bid & 7, seq = bid >> 3;
-  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + seq;
-}
-
 // Memory -> LDS, BYTES a lane to consecutive LDS addresses: uniform base (in scalar registers, kept apart from the lane's
 // 32-bit offset: hipcc would otherwise carry a 64-bit address per instruction through the k-loop and spill) + offset.
 template <int BYTES>

@@ -53,13 +53,6 @@ constexpr int POOL_SEG = 1024;   // frames per time segment (multiple of PT)
 
 __device__ __forceinline__ int pool_slot(const int32_t* row_off, int b) { return row_off[b] / POOL_SEG + b; }
 
-// launch index -> work index, bijective on [0, nwg): the workgroups of XCD x (launch indices x, x + 8, ...) get a
-// contiguous run of work indices
-__device__ __forceinline__ int pool_xcd_remap(int bid, int nwg) {
-  const int q = nwg >> 3, r = nwg & 7, xcd = bid & 7, seq = bid >> 3;
-  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + seq;
-}
-
 template <typename T>
 __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 2) void pool_stats_kernel(const T* __restrict__ a, int lda, const T* __restrict__ h,
                                                          int ldh, const T* __restrict__ w2, int ccat_p,
@@ -81,7 +74,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 4 : 2) void pool_stats_kernel(
   // HBM once per slab (PMC: 362 MB fetched for 257 MB algorithmic).  Renumber the launch plane so that consecutive
   // workgroups of ONE XCD take the slabs of one utterance: a is fetched once and re-read from that XCD's L2.
   const int n_slab = gridDim.x, plane = gridDim.x * gridDim.y;
-  const int vid = pool_xcd_remap(blockIdx.x + n_slab * blockIdx.y, plane);
+  const int vid = xcd_remap(blockIdx.x + n_slab * blockIdx.y, plane);
   const int b = vid / n_slab, slab = vid - b * n_slab;
   const int s_utt = row_off[b], n_utt = row_off[b + 1] - s_utt;
   const int seg0 = blockIdx.z * POOL_SEG;
