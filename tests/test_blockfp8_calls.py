@@ -188,3 +188,25 @@ def test_the_widest_operands():
     assert torch.equal(block_fp8_linear(a[253:257], w, out_dtype=torch.float32).double(), want[253:257])
     with pytest.raises(ValueError, match="too large"):                     # weights of 4 GiB and more
         block_fp8_linear(w, a)
+
+
+@gpu
+@pytest.mark.parametrize("n,k", [(5, 100), (700, 300)])
+def test_row_strides_of_many_megabytes(n, k):
+    """Rows 32 MiB apart: a launch takes 127 of them (32-bit offsets), by the direct kernel or in tiles.  The same rows behind one
+    another, handed over in the same portions, give the same bits."""
+    r, step = 300, 1 << 25
+    raw = torch.zeros(r, step, dtype=torch.uint8, device="cuda")
+    q = quantize_block_fp8(rows_of(1, r, k).cuda())
+    width = q.data.shape[1]
+    raw[:, 64:64 + width] = q.data.view(torch.uint8)
+    raw[:, 4096:4100] = q.exponent
+    far = BlockFP8(raw[:, 64:64 + width].view(torch.float8_e4m3fn), raw[:, 4096:4100], k)
+    w = quantize_block_fp8(rows_of(2, n, k).cuda() / k ** 0.5)
+    for dtype in (torch.bfloat16, torch.float32):
+        want = torch.cat([block_fp8_linear(q[lo:min(lo + 127, r)], w, out_dtype=dtype) for lo in range(0, r, 127)])
+        assert torch.equal(block_fp8_linear(far, w, out_dtype=dtype), want)
+        assert torch.equal(far.dequantize(dtype), q.dequantize(dtype))
+    raw.zero_()
+    quantize_block_fp8(rows_of(1, r, k).cuda(), out=far)
+    assert torch.equal(far.data.view(torch.uint8), q.data.view(torch.uint8)) and torch.equal(far.exponent, q.exponent)
