@@ -780,6 +780,8 @@ int launch_rows(const LinearArgs& p, hipStream_t s) {
   //   4816 x 1536 -> 1536     -  | 22.7 | 20.7 | 20.5 | 16.1        23001 x 1149 -> 264      -  | 18.0 | 16.0 | 17.0 | 18.9
   //   77056 x 768 -> 768      -  |  -   |  -   |  -   | 61.3 | 65.8   154112 x 128 -> 192    -  | 20.0 | 18.5 | 17.6 | 19.8
   //   77056 x 1152 -> 1152    -  |  -   |  -   |  -   | 125.9 | 118.6   77056 x 1536 -> 1536  -  |  -  |  -   |  -   | 231.9 | 180.8
+  //   77056 x 1536 (128 x 128 | persist)  -> 264 59.5 | 67.5, -> 384 59.0 | 64.4, -> 520 85.1 | 97.7, -> 640 87.0 | 100.5,
+  //     -> 776 115.6 | 118.9;   77056 x 1152 -> 264 42.3 | 50.4, -> 520 68.5 | 79.0;   77056 x 2048 -> 264 65.8 | 76.0, -> 520 108 | 120
   // float32 outputs (64 x 64 by 8 waves | by 4 | 64 x 128 | 128 x 128 by 4):
   //   301 x 1536 -> 1536     8.0 | 9.3 | 11.3                       13446 x 704 -> 373      16.0 | 14.1 | 15.7 | 17.4
   //   4816 x 1536 -> 1536    38.6 | 33.2 | 32.6 | 27.8              154112 x 128 -> 192     26.8 | 24.1 | 26.6 | 29.4
@@ -787,7 +789,8 @@ int launch_rows(const LinearArgs& p, hipStream_t s) {
   //   77056 x 384 -> 384 24.9 | 22.8;  77056 x 128 -> 512 18.3 | 19.6;  38528 x 512 -> 512 19.8 | 19.3
   // so: direct while its workgroups (each streams its 16 channels' weights once per 16 rows) are at most two a CU; weights in
   // registers for K <= 512 where two slabs or more are three quarters full and walk rows enough to pay for their fetch; the
-  // persistent kernel where k-loops are long enough to hide its epilogue and two rounds of tiles or more are there.  Of the tiles
+  // persistent kernel where k-loops are long enough to hide its epilogue and two rounds of tiles or more are there (its rule does
+  // not look at how full the last of its 256 channels are: at the widths of the last two lines it costs 3 .. 19 %).  Of the tiles
   // 128 x 128 once they give every CU one, unless the CU with the most of them has more to do than it has with 64 x 128, half the
   // work and a fifth more time for it (channels that end early in a tile, a second round for a few tiles); 64 x 64 below, by 8
   // waves (and in steps of four k-tiles, 128 KiB of LDS, where there are four) while there is no more than one a CU.
